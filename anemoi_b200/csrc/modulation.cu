@@ -1,0 +1,664 @@
+// The gated residual behind a block, the norm and the modulation in front of the next one, in one pass over the rows, and
+// its gradient.  Per row of C channels, the modulation shared by `n` consecutive rows:
+//
+//   post(y) = y,  or  N(y) * post_weight
+//   x'      = x + gate * post(y)
+//   h       = N(x') * weight * (1 + scale) + shift
+//   N(t)    = t / sqrt(mean(t^2) + eps)                                   "rms"
+//           = (t - mean(t)) / sqrt(mean((t - mean(t))^2) + eps)           "layer"
+//
+// (formulas of the reference's residual + gate + RMSNorm + modulate fusion,
+// anemoi/models/minimax_h3/solengine/models/minimax_h3/optimized/fusions.py:1-23, and of layer norm).  Everything is
+// computed in fp32 from the 16-bit inputs and rounded once; h is the norm of x' before its rounding.
+//
+// Gradient, from the gradients e of x' and d of h (a = N(x'), r = the reciprocal root in N):
+//   shift: sum d      scale: sum d * a * weight      weight: sum d * (1 + scale) * a
+//   g  = d * (1 + scale) * weight
+//   dx = e + r * (g - a * mean(g * a) [- mean(g), "layer"])
+//   u  = gate * dx    gate: sum dx * post(y)         post_weight: sum u * N(y)
+//   dy = u, or with b = N(y), q = its root: q * (u' - b * mean(u' * b) [- mean(u')]), u' = u * post_weight
+// The statistics are formed again from x' and y, which are in registers anyway: keeping them would be two more arrays for
+// a user to hold and saves no byte of x' or y.
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/anemoi_sm100.h"
+#include "rows.cuh"
+
+namespace {
+
+using namespace rows;
+
+enum Norm { kNone = 0, kRms = 1, kLayer = 2 };
+
+struct ForwardParams {
+  const void *x, *y, *gate, *scale, *shift, *weight, *post_weight;
+  void *x_out, *h_out;
+  int64_t x_stride, y_stride, gate_stride, scale_stride, shift_stride;  // of rows, in elements
+  int64_t rows, per_group;
+  int width, norm, post;
+  float eps;
+};
+
+struct BackwardParams {
+  const void *dx_out, *dh, *x, *y, *gate, *scale, *weight, *post_weight;
+  void *dx, *dy, *dgate, *dscale, *dshift;
+  float *partial;         // [segments][3][C] where a group has several segments
+  float *weight_partial;  // [workers][2][C] where a weight's gradient is wanted
+  int64_t dx_out_stride, dh_stride, x_stride, y_stride, gate_stride, scale_stride;
+  int64_t rows, per_group, segments;
+  int per_group_segments, workers, width, norm, post;
+  float eps;
+};
+
+// Most threads of a block.  Narrow rows: 128.  Wide rows, up to 1,024 pieces of 8 channels: as many threads as the vectors
+// of a thread leave.
+__host__ __device__ constexpr int forward_threads(int vectors, bool wide) { return !wide ? 128 : vectors == 1 ? 1024 : 352; }
+// The gradient holds three column sums per channel: one vector per thread up to 704 pieces (88 registers each), two above.
+constexpr int kOnePiece = 704;
+__host__ __device__ constexpr int backward_threads(int vectors, bool wide) { return !wide ? 128 : vectors == 1 ? kOnePiece : 512; }
+// (and blocks per SM that its registers are to leave room for)
+__host__ __device__ constexpr int backward_blocks(int vectors, bool wide) {
+  return wide ? 1 : vectors == 1 ? 6 : vectors == 2 ? 4 : 2;
+}
+
+// Sum over the threads of one row, in each of them.  Narrow rows: kLanes lanes of a warp.  Wide rows: the block; `buffer`
+// alternates between two places, so that one barrier per sum is enough (a thread that writes a place the second time
+// has passed the barrier behind everyone's reads of its first use).
+template <bool kWide>
+struct RowSum {
+  float* buffer;
+  int lanes;
+  int turn = 0;
+  __device__ __forceinline__ float operator()(float v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+      if (kWide || off < lanes) v += __shfl_xor_sync(0xffffffffu, v, off);
+    if (kWide) {
+      const int warps = (blockDim.x + 31) >> 5;
+      float* b = buffer + turn * 32;
+      turn ^= 1;
+      if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = (threadIdx.x & 31) < warps ? b[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    }
+    return v;
+  }
+  // two sums at once
+  __device__ __forceinline__ float2 operator()(float2 v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+      if (kWide || off < lanes) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
+      }
+    if (kWide) {
+      const int warps = (blockDim.x + 31) >> 5;
+      float2* b = reinterpret_cast<float2*>(buffer + 64) + turn * 32;
+      turn ^= 1;
+      if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = (threadIdx.x & 31) < warps ? b[threadIdx.x & 31] : make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
+      }
+    }
+    return v;
+  }
+};
+constexpr int kBuffer = 64 + 128;
+
+// Normalises v in place; returns the reciprocal root.  Channels that the thread does not have are zeros and stay so.
+template <int V, bool kWide>
+__device__ __forceinline__ float normalise(float (&v)[V][8], const bool (&has)[V], int kind, int width, float eps,
+                                           RowSum<kWide>& sum) {
+  const float inv = 1.0f / (float)width;
+  if (kind == kLayer) {
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[j][i];
+    const float mean = sum(s) * inv;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = has[j] ? v[j][i] - mean : 0.0f;
+  }
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(v[j][i], v[j][i], s);
+  const float r = 1.0f / sqrtf(fmaf(sum(s), inv, eps));
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[j][i] *= r;
+  return r;
+}
+
+// One row per `lanes` threads.  HBM bound: 2 C bytes of each of x, y in, x', h out.
+template <typename T, typename M, int V, bool kWide>
+__global__ void __launch_bounds__(forward_threads(V, kWide)) forward_kernel(const __grid_constant__ ForwardParams p, int lanes) {
+  __shared__ float buffer[kBuffer];
+  const int lane = kWide ? threadIdx.x : threadIdx.x % lanes;
+  const int64_t row_in = kWide ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+  const bool live = row_in < p.rows;
+  const int64_t row = live ? row_in : p.rows - 1;
+  RowSum<kWide> sum{buffer, lanes};
+  bool has[V];
+  int at[V];
+  uint4 xr[V], yr[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    at[j] = (j * lanes + lane) * 8;
+    has[j] = at[j] < p.width;
+    xr[j] = yr[j] = make_uint4(0, 0, 0, 0);
+    if (has[j]) {
+      xr[j] = load_stream(static_cast<const T*>(p.x) + row * p.x_stride + at[j]);
+      if (p.y != nullptr) yr[j] = load_stream(static_cast<const T*>(p.y) + row * p.y_stride + at[j]);
+    }
+  }
+  const int64_t group = row / p.per_group;
+  float x[V][8];
+#pragma unroll
+  for (int j = 0; j < V; ++j) open8<T>(xr[j], x[j]);
+  if (p.y != nullptr) {
+    float y[V][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j) open8<T>(yr[j], y[j]);
+    if (p.post != kNone) normalise<V, kWide>(y, has, p.post, p.width, p.eps, sum);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!has[j]) continue;
+      if (p.post_weight != nullptr) {
+        float w[8];
+        shared8(static_cast<const T*>(p.post_weight) + at[j], w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[j][i] *= w[i];
+      }
+      float g[8];
+      shared8(static_cast<const M*>(p.gate) + group * p.gate_stride + at[j], g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] = fmaf(g[i], y[j][i], x[j][i]);
+      if (live) *reinterpret_cast<uint4*>(static_cast<T*>(p.x_out) + row * p.width + at[j]) = round8<T>(x[j]);
+    }
+  }
+  if (p.h_out == nullptr) return;
+  normalise<V, kWide>(x, has, p.norm, p.width, p.eps, sum);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (!has[j]) continue;
+    float f[8];
+    if (p.weight != nullptr) {
+      shared8(static_cast<const T*>(p.weight) + at[j], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] *= f[i];
+    }
+    if (p.scale != nullptr) {
+      shared8(static_cast<const M*>(p.scale) + group * p.scale_stride + at[j], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] = fmaf(x[j][i], f[i], x[j][i]);
+    }
+    if (p.shift != nullptr) {
+      shared8(static_cast<const M*>(p.shift) + group * p.shift_stride + at[j], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] += f[i];
+    }
+    if (live) *reinterpret_cast<uint4*>(static_cast<T*>(p.h_out) + row * p.width + at[j]) = round8<T>(x[j]);
+  }
+}
+
+// Gradient of N: v = the gradient of the normalised row `hat`, turned into that of the row itself.
+template <int V, bool kWide>
+__device__ __forceinline__ void normalise_gradient(float (&v)[V][8], const float (&hat)[V][8], const bool (&has)[V],
+                                                   float r, int kind, int width, RowSum<kWide>& sum) {
+  float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s.x = fmaf(v[j][i], hat[j][i], s.x);
+      s.y += v[j][i];
+    }
+  s = sum(s);
+  const float inv = 1.0f / (float)width, along = s.x * inv, mean = kind == kLayer ? s.y * inv : 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[j][i] = has[j] ? r * (v[j][i] - fmaf(hat[j][i], along, mean)) : 0.0f;
+}
+
+// A worker (a block, or `lanes` threads of a warp) walks whole segments: consecutive rows of one modulation group, whose
+// column sums it holds in registers: A = sum d * a, S = sum d, B = sum dx * N(y).  scale's gradient is weight * A, weight's
+// sum over the groups of (1 + scale) * A, and so for gate and post_weight with B.  A group of one segment is finished by its
+// worker, other groups and the weights by sums_kernel, in a fixed order.
+template <typename T, typename M, int V, bool kWide>
+__global__ void __launch_bounds__(backward_threads(V, kWide), backward_blocks(V, kWide)) backward_kernel(const __grid_constant__ BackwardParams p, int lanes) {
+  extern __shared__ __align__(16) float weight_sums[];  // per worker [2][V * lanes * 8], where weights are given
+  __shared__ float buffer[kBuffer];
+  const int lane = kWide ? threadIdx.x : threadIdx.x % lanes;
+  const int slots = kWide ? 1 : blockDim.x / lanes, slot = kWide ? 0 : threadIdx.x / lanes;
+  const int worker = blockIdx.x * slots + slot;
+  RowSum<kWide> sum{buffer, lanes};
+  bool has[V];
+  int at[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    at[j] = (j * lanes + lane) * 8;
+    has[j] = at[j] < p.width;
+  }
+  const bool weights = p.weight_partial != nullptr;
+  float* own = weight_sums + (int64_t)slot * 2 * V * lanes * 8;
+  if (weights)
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) own[at[j] + i] = own[V * lanes * 8 + at[j] + i] = 0.0f;
+  // all workers of a block walk the same number of segments (lanes of a warp meet in its shuffles)
+  const int64_t turns = (p.segments + p.workers - 1) / p.workers;
+  for (int64_t turn = 0; turn < turns; ++turn) {
+    const int64_t segment = turn * p.workers + worker;
+    const bool live = segment < p.segments && worker < p.workers;
+    const int64_t group = live ? segment / p.per_group_segments : 0;
+    const int64_t part = live ? segment - group * p.per_group_segments : 0;
+    const int64_t first = group * p.per_group + p.per_group * part / p.per_group_segments;
+    const int64_t count = live ? group * p.per_group + p.per_group * (part + 1) / p.per_group_segments - first : 0;
+    // (the longest segment: every worker takes as many steps)
+    const int64_t steps = (p.per_group + p.per_group_segments - 1) / p.per_group_segments;
+    float a_sum[V][8] = {}, s_sum[V][8] = {}, b_sum[V][8] = {};
+    uint4 raw[4][V];
+    auto fetch = [&](int64_t step) {
+      const int64_t row = first + step;
+      const bool in = step < count;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        raw[0][j] = raw[1][j] = raw[2][j] = raw[3][j] = make_uint4(0, 0, 0, 0);
+        if (!in || !has[j]) continue;
+        raw[0][j] = load_stream(static_cast<const T*>(p.x) + row * p.x_stride + at[j]);
+        if (p.dh != nullptr) raw[1][j] = load_stream(static_cast<const T*>(p.dh) + row * p.dh_stride + at[j]);
+        if (p.dx_out != nullptr) raw[2][j] = load_stream(static_cast<const T*>(p.dx_out) + row * p.dx_out_stride + at[j]);
+        if (p.y != nullptr) raw[3][j] = load_stream(static_cast<const T*>(p.y) + row * p.y_stride + at[j]);
+      }
+    };
+    fetch(0);
+    for (int64_t step = 0; step < steps; ++step) {
+      const int64_t row = first + step;
+      const bool in = step < count;
+      float dx[V][8], y[V][8];
+      {
+        float x[V][8], d[V][8];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          open8<T>(raw[0][j], x[j]);
+          open8<T>(raw[1][j], d[j]);
+          open8<T>(raw[2][j], dx[j]);
+          open8<T>(raw[3][j], y[j]);
+        }
+        if (step + 1 < steps) fetch(step + 1);
+        if (p.dh != nullptr) {
+          const float r = normalise<V, kWide>(x, has, p.norm, p.width, p.eps, sum);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              a_sum[j][i] = fmaf(d[j][i], x[j][i], a_sum[j][i]);
+              s_sum[j][i] += d[j][i];
+            }
+            if (!has[j]) continue;
+            float f[8];
+            if (p.weight != nullptr) {
+              shared8(static_cast<const T*>(p.weight) + at[j], f);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) d[j][i] *= f[i];
+            }
+            if (p.scale != nullptr) {
+              shared8(static_cast<const M*>(p.scale) + group * p.scale_stride + at[j], f);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) d[j][i] = fmaf(d[j][i], f[i], d[j][i]);
+            }
+          }
+          normalise_gradient<V, kWide>(d, x, has, r, p.norm, p.width, sum);
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dx[j][i] += d[j][i];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (in && has[j]) *reinterpret_cast<uint4*>(static_cast<T*>(p.dx) + row * p.width + at[j]) = round8<T>(dx[j]);
+      if (p.y == nullptr) continue;
+      float r = 0.0f;
+      if (p.post != kNone) r = normalise<V, kWide>(y, has, p.post, p.width, p.eps, sum);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b_sum[j][i] = fmaf(dx[j][i], y[j][i], b_sum[j][i]);
+        if (!has[j]) continue;
+        float f[8];
+        shared8(static_cast<const M*>(p.gate) + group * p.gate_stride + at[j], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dx[j][i] *= f[i];
+        if (p.post_weight != nullptr) {
+          shared8(static_cast<const T*>(p.post_weight) + at[j], f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dx[j][i] *= f[i];
+        }
+      }
+      if (p.post != kNone) normalise_gradient<V, kWide>(dx, y, has, r, p.post, p.width, sum);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (in && has[j]) *reinterpret_cast<uint4*>(static_cast<T*>(p.dy) + row * p.width + at[j]) = round8<T>(dx[j]);
+    }
+    if (!live) continue;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!has[j]) continue;
+      float f[8];
+      if (weights) {
+        float* mine = own + at[j];
+        if (p.scale != nullptr) shared8(static_cast<const M*>(p.scale) + group * p.scale_stride + at[j], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[i] += p.scale != nullptr ? fmaf(a_sum[j][i], f[i], a_sum[j][i]) : a_sum[j][i];
+        if (p.y != nullptr) {
+          shared8(static_cast<const M*>(p.gate) + group * p.gate_stride + at[j], f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mine[V * lanes * 8 + i] = fmaf(b_sum[j][i], f[i], mine[V * lanes * 8 + i]);
+        }
+      }
+      if (p.per_group_segments > 1) {
+        float* out = p.partial + segment * 3 * p.width + at[j];
+        store8(out, a_sum[j]);
+        store8(out + p.width, s_sum[j]);
+        store8(out + 2 * (int64_t)p.width, b_sum[j]);
+        continue;
+      }
+      const int64_t out = group * p.width + at[j];
+      if (p.dshift != nullptr) store8(static_cast<M*>(p.dshift) + out, s_sum[j]);
+      if (p.dscale != nullptr) {
+        if (p.weight != nullptr) {
+          shared8(static_cast<const T*>(p.weight) + at[j], f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a_sum[j][i] *= f[i];
+        }
+        store8(static_cast<M*>(p.dscale) + out, a_sum[j]);
+      }
+      if (p.dgate != nullptr) {
+        if (p.post_weight != nullptr) {
+          shared8(static_cast<const T*>(p.post_weight) + at[j], f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b_sum[j][i] *= f[i];
+        }
+        store8(static_cast<M*>(p.dgate) + out, b_sum[j]);
+      }
+    }
+  }
+  if (weights && worker < p.workers)
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (has[j]) {
+        float* out = p.weight_partial + (int64_t)worker * 2 * p.width + at[j];
+        const float* mine = own + at[j];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          out[i] = mine[i];
+          out[p.width + i] = mine[V * lanes * 8 + i];
+        }
+      }
+}
+
+struct SumsParams {
+  const float *partial, *weight_partial;
+  const void *weight, *post_weight;
+  void *dgate, *dscale, *dshift, *dweight, *dpost_weight;
+  int64_t groups;
+  int per_group_segments, workers, width;
+};
+
+// blockIdx.y: the groups' A, S, B sums (where groups have several segments), then the two weights' sums.
+template <typename T, typename M>
+__global__ void sums_kernel(const __grid_constant__ SumsParams p) {
+  const int column = blockIdx.x * 32 + threadIdx.x;
+  const bool in = column < p.width;
+  const int64_t job = blockIdx.y + (int64_t)blockIdx.z * 32768;
+  const int64_t group_jobs = p.per_group_segments > 1 ? p.groups * 3 : 0;
+  if (job < group_jobs) {
+    const int64_t group = job / 3;
+    const int which = (int)(job - group * 3);
+    void* out = which == 0 ? p.dscale : which == 1 ? p.dshift : p.dgate;
+    if (out == nullptr) return;
+    float v = column_sum(p.partial + (group * p.per_group_segments * 3 + which) * p.width, 3 * (int64_t)p.width,
+                         p.per_group_segments, column, in);
+    if (threadIdx.y != 0 || !in) return;
+    const void* w = which == 0 ? p.weight : which == 2 ? p.post_weight : nullptr;
+    if (w != nullptr) v *= load1(static_cast<const T*>(w) + column);
+    store1(static_cast<M*>(out) + group * p.width + column, v);
+    return;
+  }
+  const int which = (int)(job - group_jobs);
+  void* out = which == 0 ? p.dweight : which == 1 ? p.dpost_weight : nullptr;
+  if (out == nullptr) return;
+  const float v = column_sum(p.weight_partial + (int64_t)which * p.width, 2 * (int64_t)p.width, p.workers, column, in);
+  if (threadIdx.y == 0 && in) store1(static_cast<T*>(out) + column, v);
+}
+
+// How a row lies on threads: `lanes` threads of `vectors` pieces of 8 channels each.
+struct RowShape {
+  bool wide;
+  int vectors, lanes, threads;
+};
+
+constexpr int kMostWidth = 8192;
+
+// Up to 1,024 channels a row has a power of two of lanes of one warp.  Wider rows have a block, of at least as many threads
+// as `vectors` pieces each need.
+RowShape shape_of(int width, int vectors) {
+  const int pieces = width / 8;
+  RowShape s{};
+  if (pieces <= 128) {
+    s.vectors = pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4;
+    s.lanes = 32;
+    while (s.lanes > 4 && s.lanes / 2 * s.vectors >= pieces) s.lanes /= 2;
+    s.threads = 128;
+    return s;
+  }
+  s.wide = true;
+  s.vectors = vectors;
+  s.lanes = s.threads = ((pieces + vectors - 1) / vectors + 31) / 32 * 32;
+  return s;
+}
+int backward_vectors(int width) { return width / 8 <= kOnePiece ? 1 : 2; }
+
+struct Split {
+  int workers, blocks, per_group_segments;
+  int64_t segments;
+};
+
+// Segments of the gradient: as many as there are workers, or a small multiple where the groups divide them better; none
+// shorter than a row.
+Split split_of(const RowShape& s, int64_t rows, int64_t groups, int blocks_per_sm) {
+  const int slots = s.wide ? 1 : s.threads / s.lanes;
+  const int64_t per_group = rows / groups, most = (int64_t)kSms * blocks_per_sm * slots;
+  Split out{};
+  int64_t best = 1;
+  double best_share = 0.0;
+  for (int64_t turns = 1; turns <= 4; ++turns) {
+    const int64_t each = std::min(per_group, std::max<int64_t>(1, turns * most / groups));
+    const int64_t total = each * groups, walks = (total + most - 1) / most;
+    // rows that the longest worker walks, against an even share
+    const double longest = (double)walks * (double)((per_group + each - 1) / each);
+    const double share = (double)rows / (double)most / longest;
+    if (share > best_share * 1.02) {
+      best_share = share;
+      best = each;
+    }
+  }
+  out.per_group_segments = (int)best;
+  out.segments = best * groups;
+  const int64_t needed = (std::min(out.segments, most) + slots - 1) / slots;
+  out.blocks = (int)needed;
+  out.workers = (int)std::min<int64_t>(needed * slots, most);
+  return out;
+}
+
+int backward_blocks_per_sm(const RowShape& s) {
+  return s.wide ? std::max(1, backward_threads(s.vectors, true) / s.threads) : backward_blocks(s.vectors, false);
+}
+
+template <typename T, typename M, int V, bool kWide>
+int forward_launch(const ForwardParams& p, const RowShape& s, cudaStream_t st) {
+  const int64_t per_block = s.wide ? 1 : s.threads / s.lanes;
+  const int64_t blocks = (p.rows + per_block - 1) / per_block;
+  if (blocks > 0x7fffffffLL) return ANEMOI_SM100_ELIMIT;
+  forward_kernel<T, M, V, kWide><<<(unsigned)blocks, s.threads, 0, st>>>(p, s.lanes);
+  return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
+}
+
+template <typename T, typename M, int V, bool kWide>
+int backward_launch(const BackwardParams& p, const RowShape& s, const Split& split, cudaStream_t st) {
+  const int slots = s.wide ? 1 : s.threads / s.lanes;
+  const size_t smem = p.weight_partial != nullptr ? (size_t)slots * 2 * V * s.lanes * 8 * sizeof(float) : 0;
+  auto kernel = backward_kernel<T, M, V, kWide>;
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return ANEMOI_SM100_ELAUNCH;
+  kernel<<<split.blocks, s.threads, smem, st>>>(p, s.lanes);
+  return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
+}
+
+template <typename T, typename M>
+int forward_typed(const ForwardParams& p, const RowShape& s, cudaStream_t st) {
+  if (!s.wide) {
+    if (s.vectors == 1) return forward_launch<T, M, 1, false>(p, s, st);
+    if (s.vectors == 2) return forward_launch<T, M, 2, false>(p, s, st);
+    return forward_launch<T, M, 4, false>(p, s, st);
+  }
+  return s.vectors == 1 ? forward_launch<T, M, 1, true>(p, s, st) : forward_launch<T, M, 3, true>(p, s, st);
+}
+
+template <typename T, typename M>
+int backward_typed(const BackwardParams& p, const SumsParams& q, const RowShape& s, const Split& split, cudaStream_t st) {
+  int code;
+  if (!s.wide)
+    code = s.vectors == 1   ? backward_launch<T, M, 1, false>(p, s, split, st)
+           : s.vectors == 2 ? backward_launch<T, M, 2, false>(p, s, split, st)
+                            : backward_launch<T, M, 4, false>(p, s, split, st);
+  else
+    code = s.vectors == 1 ? backward_launch<T, M, 1, true>(p, s, split, st) : backward_launch<T, M, 2, true>(p, s, split, st);
+  if (code != ANEMOI_SM100_OK) return code;
+  const int64_t jobs = (split.per_group_segments > 1 ? 3 * q.groups : 0) + (q.weight_partial != nullptr ? 2 : 0);
+  if (jobs == 0) return ANEMOI_SM100_OK;
+  const dim3 grid((unsigned)((q.width + 31) / 32), (unsigned)std::min<int64_t>(jobs, 32768),
+                  (unsigned)((jobs + 32767) / 32768));
+  sums_kernel<T, M><<<grid, dim3(32, kSlices), 0, st>>>(q);
+  return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int check(const anemoi_sm100_rows* r) {
+  if (r == nullptr || r->rows < 0 || r->groups <= 0 || r->width <= 0 || r->width % 8 || !(r->eps >= 0.0f))
+    return ANEMOI_SM100_EINVAL;
+  if (r->rows % r->groups || (r->norm != kRms && r->norm != kLayer) || r->post < kNone || r->post > kLayer)
+    return ANEMOI_SM100_EINVAL;
+  return r->width > kMostWidth ? ANEMOI_SM100_ELIMIT : ANEMOI_SM100_OK;
+}
+
+// Three pieces per thread where there are rows for every SM; a few rows are done sooner by as many threads as they have
+// pieces.
+int forward_vectors(int64_t rows) { return rows <= 2 * kSms ? 1 : 3; }
+
+}  // namespace
+
+extern "C" int anemoi_sm100_gate_norm_modulate(const anemoi_sm100_rows* r, const void* x, const void* y, const void* gate,
+                                               const void* scale, const void* shift, const void* weight,
+                                               const void* post_weight, const int64_t* strides, void* x_out, void* h_out,
+                                               void* stream) {
+  const int bad = check(r);
+  if (bad != ANEMOI_SM100_OK) return bad;
+  if (!x || !strides || (!y && !h_out) || (y != nullptr && (!gate || !x_out)) || (!y && (r->post != kNone || post_weight)))
+    return ANEMOI_SM100_EINVAL;
+  if (post_weight != nullptr && r->post == kNone) return ANEMOI_SM100_EINVAL;
+  for (const void* t : {x, y, gate, scale, shift, weight, post_weight, (const void*)x_out, (const void*)h_out})
+    if (!aligned(t)) return ANEMOI_SM100_EINVAL;
+  for (int i = 0; i < 5; ++i)
+    if (strides[i] < 0 || strides[i] % (i >= 2 && r->mod_is_fp32 ? 4 : 8)) return ANEMOI_SM100_EINVAL;
+  if (r->rows == 0) return ANEMOI_SM100_OK;
+  ForwardParams p{x, y, gate, scale, shift, weight, post_weight, y ? x_out : nullptr, h_out, strides[0], strides[1],
+                  strides[2], strides[3], strides[4], r->rows, r->rows / r->groups, r->width, r->norm, r->post, r->eps};
+  const RowShape s = shape_of(r->width, forward_vectors(r->rows));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (r->is_bf16)
+    return r->mod_is_fp32 ? forward_typed<__nv_bfloat16, float>(p, s, st)
+                          : forward_typed<__nv_bfloat16, __nv_bfloat16>(p, s, st);
+  return r->mod_is_fp32 ? forward_typed<__half, float>(p, s, st) : forward_typed<__half, __half>(p, s, st);
+}
+
+namespace {
+struct BackwardPlan {
+  RowShape shape;
+  Split split;
+  int64_t partial, weight_partial;  // floats
+};
+BackwardPlan plan_of(const anemoi_sm100_rows* r, bool weights) {
+  BackwardPlan plan{};
+  plan.shape = shape_of(r->width, backward_vectors(r->width));
+  plan.split = split_of(plan.shape, r->rows, r->groups, backward_blocks_per_sm(plan.shape));
+  plan.partial = plan.split.per_group_segments > 1 ? plan.split.segments * 3 * r->width : 0;
+  plan.weight_partial = weights ? (int64_t)plan.split.workers * 2 * r->width : 0;
+  return plan;
+}
+}  // namespace
+
+extern "C" int64_t anemoi_sm100_gate_norm_modulate_backward_workspace(const anemoi_sm100_rows* r, int weights) {
+  const int bad = check(r);
+  if (bad != ANEMOI_SM100_OK) return bad;
+  if (r->rows == 0) return 0;
+  const BackwardPlan plan = plan_of(r, weights != 0);
+  return (plan.partial + plan.weight_partial) * (int64_t)sizeof(float);
+}
+
+extern "C" int anemoi_sm100_gate_norm_modulate_backward(
+    const anemoi_sm100_rows* r, const void* dx_out, const void* dh, const void* x, const void* y, const void* gate,
+    const void* scale, const void* weight, const void* post_weight, const int64_t* strides, void* dx, void* dy, void* dgate,
+    void* dscale, void* dshift, void* dweight, void* dpost_weight, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int bad = check(r);
+  if (bad != ANEMOI_SM100_OK) return bad;
+  if (!x || !dx || !strides || (!dx_out && !dh) || (y != nullptr && (!gate || !dy))) return ANEMOI_SM100_EINVAL;
+  if (!y && (r->post != kNone || post_weight || dgate || dpost_weight)) return ANEMOI_SM100_EINVAL;
+  if (!dh && (dscale || dshift || dweight)) return ANEMOI_SM100_EINVAL;
+  if (post_weight != nullptr && r->post == kNone) return ANEMOI_SM100_EINVAL;
+  if ((dweight && !weight) || (dpost_weight && !post_weight)) return ANEMOI_SM100_EINVAL;
+  for (const void* t : {dx_out, dh, x, y, gate, scale, weight, post_weight, (const void*)dx, (const void*)dy,
+                        (const void*)dgate, (const void*)dscale, (const void*)dshift, (const void*)dweight,
+                        (const void*)dpost_weight, (const void*)workspace})
+    if (!aligned(t)) return ANEMOI_SM100_EINVAL;
+  for (int i = 0; i < 6; ++i)
+    if (strides[i] < 0 || strides[i] % (i >= 4 && r->mod_is_fp32 ? 4 : 8)) return ANEMOI_SM100_EINVAL;
+  if (r->rows == 0) return ANEMOI_SM100_EINVAL;  // (the sums of no rows are the caller's zeros)
+  const bool weights = dweight != nullptr || dpost_weight != nullptr;
+  const BackwardPlan plan = plan_of(r, weights);
+  const int64_t needed = (plan.partial + plan.weight_partial) * (int64_t)sizeof(float);
+  if (needed > 0 && (workspace == nullptr || workspace_bytes < needed)) return ANEMOI_SM100_EINVAL;
+  float* partial = static_cast<float*>(workspace);
+  float* weight_partial = weights ? partial + plan.partial : nullptr;
+  BackwardParams p{dx_out, dh, x, y, gate, scale, weight, post_weight, dx, dy, dgate, dscale, dshift, partial,
+                   weight_partial, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], r->rows,
+                   r->rows / r->groups, plan.split.segments, plan.split.per_group_segments, plan.split.workers, r->width,
+                   r->norm, r->post, r->eps};
+  const SumsParams q{partial, weight_partial, weight, post_weight, dgate, dscale, dshift, dweight, dpost_weight, r->groups,
+                     plan.split.per_group_segments, plan.split.workers, r->width};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (r->is_bf16)
+    return r->mod_is_fp32 ? backward_typed<__nv_bfloat16, float>(p, q, plan.shape, plan.split, st)
+                          : backward_typed<__nv_bfloat16, __nv_bfloat16>(p, q, plan.shape, plan.split, st);
+  return r->mod_is_fp32 ? backward_typed<__half, float>(p, q, plan.shape, plan.split, st)
+                        : backward_typed<__half, __half>(p, q, plan.shape, plan.split, st);
+}

@@ -77,6 +77,21 @@ class LayerPlan(C.Structure):
                 ("maxpool_weight", C.c_float)]
 
 
+class Rows(C.Structure):
+    """Rows of channels and what they share (``anemoi_sm100_rows``)."""
+
+    _fields_ = [("rows", C.c_int64), ("groups", C.c_int64), ("width", C.c_int32), ("norm", C.c_int32),
+                ("post", C.c_int32), ("is_bf16", C.c_int32), ("mod_is_fp32", C.c_int32), ("eps", C.c_float)]
+
+
+class AxialRopeShape(C.Structure):
+    """Queries and keys of the axial rotary embedding (``anemoi_sm100_axial_rope_shape``)."""
+
+    _fields_ = [("batch", C.c_int64), ("tokens", C.c_int64), ("q_heads", C.c_int32), ("k_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("axes", C.c_int32), ("sections", C.c_int32 * 4), ("interleaved", C.c_int32),
+                ("positions_type", C.c_int32), ("is_bf16", C.c_int32), ("eps", C.c_float)]
+
+
 @lru_cache(maxsize=1)
 def library() -> C.CDLL:
     """Load the in-tree shared library; raise if it has not been built."""
@@ -88,7 +103,7 @@ def library() -> C.CDLL:
         )
     lib = C.CDLL(str(path))
     P, I32, I64, F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
-    SP, OP = C.POINTER(Shape), C.POINTER(Operands)
+    SP, OP, RP, AP = C.POINTER(Shape), C.POINTER(Operands), C.POINTER(Rows), C.POINTER(AxialRopeShape)
     signatures = {
         "anemoi_sm100_arch": (C.c_int, []),
         "anemoi_sm100_operand_bytes": (I64, [SP, C.c_int]),
@@ -147,6 +162,14 @@ def library() -> C.CDLL:
         "anemoi_sm100_tensor_peak": (C.c_int, [I32, I32, P, C.POINTER(C.c_double), P]),
         "anemoi_sm100_qknorm_rope": (C.c_int, [P, P, P, P, I64, I32, I32, I32, C.c_float, I32,
                                                C.POINTER(C.c_int64), P]),
+        "anemoi_sm100_gate_norm_modulate": (C.c_int, [RP, P, P, P, P, P, P, P, C.POINTER(I64), P, P, P]),
+        "anemoi_sm100_gate_norm_modulate_backward_workspace": (I64, [RP, C.c_int]),
+        "anemoi_sm100_gate_norm_modulate_backward": (C.c_int, [RP, P, P, P, P, P, P, P, P, C.POINTER(I64), P, P, P, P, P, P,
+                                                               P, P, I64, P]),
+        "anemoi_sm100_axial_rope": (C.c_int, [AP, P, P, P, P, P, I64, C.POINTER(C.c_double), C.POINTER(I64), P, P, P]),
+        "anemoi_sm100_axial_rope_backward_workspace": (I64, [AP]),
+        "anemoi_sm100_axial_rope_backward": (C.c_int, [AP, P, P, P, P, P, P, P, I64, C.POINTER(C.c_double), C.POINTER(I64),
+                                                       P, P, P, P, P, I64, P]),
     }
     for name, (restype, argtypes) in signatures.items():
         fn = getattr(lib, name)
@@ -176,6 +199,9 @@ EXPORTED = (
     "anemoi_sm100_wait_selftest", "anemoi_sm100_copy_rows", "anemoi_sm100_push_qkv",
     "anemoi_sm100_push_qkv_norm", "anemoi_sm100_push_out", "anemoi_sm100_wait_flags", "anemoi_sm100_peer_alloc", "anemoi_sm100_peer_open",
     "anemoi_sm100_peer_close", "anemoi_sm100_peer_free",
+    "anemoi_sm100_gate_norm_modulate", "anemoi_sm100_gate_norm_modulate_backward_workspace",
+    "anemoi_sm100_gate_norm_modulate_backward", "anemoi_sm100_axial_rope", "anemoi_sm100_axial_rope_backward_workspace",
+    "anemoi_sm100_axial_rope_backward",
 )
 
 
@@ -727,3 +753,62 @@ def qknorm_rope_(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
         (C.c_int64 * 2)(x.stride(0), x.stride(1)), torch.cuda.current_stream(device).cuda_stream),
            "anemoi_sm100_qknorm_rope")
     return x
+
+
+def _at(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor | None:
+    """Scratch of one call, from torch's allocator (which keeps it for the stream of the call)."""
+    if nbytes < 0:
+        raise RuntimeError(f"workspace query failed: {ERRORS.get(nbytes, nbytes)}")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def gate_norm_modulate(rows: Rows, x, y, gate, scale, shift, weight, post_weight, strides, x_out, h_out) -> None:
+    with torch.cuda.device(x.device):
+        _count("gate_norm_modulate", 1 if rows.rows else 0)
+        _check(library().anemoi_sm100_gate_norm_modulate(
+            C.byref(rows), _at(x), _at(y), _at(gate), _at(scale), _at(shift), _at(weight), _at(post_weight),
+            (C.c_int64 * 5)(*strides), _at(x_out), _at(h_out), torch.cuda.current_stream().cuda_stream),
+            "anemoi_sm100_gate_norm_modulate")
+
+
+def gate_norm_modulate_backward(rows: Rows, dx_out, dh, x, y, gate, scale, weight, post_weight, strides, dx, dy, dgate,
+                                dscale, dshift, dweight, dpost_weight) -> None:
+    lib = library()
+    with torch.cuda.device(x.device):
+        nbytes = int(lib.anemoi_sm100_gate_norm_modulate_backward_workspace(
+            C.byref(rows), int(dweight is not None or dpost_weight is not None)))
+        space = _workspace(nbytes, x.device)
+        _count("gate_norm_modulate_backward", 2 if nbytes else 1)
+        _check(lib.anemoi_sm100_gate_norm_modulate_backward(
+            C.byref(rows), _at(dx_out), _at(dh), _at(x), _at(y), _at(gate), _at(scale), _at(weight), _at(post_weight),
+            (C.c_int64 * 6)(*strides), _at(dx), _at(dy), _at(dgate), _at(dscale), _at(dshift), _at(dweight),
+            _at(dpost_weight), _at(space), nbytes, torch.cuda.current_stream().cuda_stream),
+            "anemoi_sm100_gate_norm_modulate_backward")
+
+
+def axial_rope(shape: AxialRopeShape, q, k, q_weight, k_weight, positions, position_batch: int, turns, strides, q_out,
+               k_out) -> None:
+    with torch.cuda.device(q.device):
+        _count("axial_rope", 1)
+        _check(library().anemoi_sm100_axial_rope(
+            C.byref(shape), _at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions), position_batch, turns,
+            (C.c_int64 * 12)(*strides), _at(q_out), _at(k_out), torch.cuda.current_stream().cuda_stream),
+            "anemoi_sm100_axial_rope")
+
+
+def axial_rope_backward(shape: AxialRopeShape, dq_out, dk_out, q, k, q_weight, k_weight, positions, position_batch: int,
+                        turns, strides, dq, dk, dq_weight, dk_weight) -> None:
+    lib = library()
+    weights = dq_weight is not None or dk_weight is not None
+    with torch.cuda.device(dq_out.device):
+        nbytes = int(lib.anemoi_sm100_axial_rope_backward_workspace(C.byref(shape))) if weights else 0
+        space = _workspace(nbytes, dq_out.device)
+        _count("axial_rope_backward", 2 if weights else 1)
+        _check(lib.anemoi_sm100_axial_rope_backward(
+            C.byref(shape), _at(dq_out), _at(dk_out), _at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions),
+            position_batch, turns, (C.c_int64 * 18)(*strides), _at(dq), _at(dk), _at(dq_weight), _at(dk_weight),
+            _at(space), nbytes, torch.cuda.current_stream().cuda_stream), "anemoi_sm100_axial_rope_backward")

@@ -6,9 +6,18 @@ Triton-backed function
 head, then rotary embedding of the leading ``rotary_dim`` channels, for ``(B, seq, heads, D)``.
 It runs as one CUDA kernel of this library (``anemoi_sm100_qknorm_rope``); there is no eager
 fallback.
+
+``fused_qknorm_axial_rope`` does the same for positions with several axes (time, height, width): it takes the positions
+themselves instead of tables, forms each token's angles once for all heads of queries and keys, and is differentiable
+(``anemoi_sm100_axial_rope``, ``anemoi_sm100_axial_rope_backward``).
 """
 
 from __future__ import annotations
+
+import ctypes as C
+import math
+from dataclasses import dataclass
+from functools import cached_property
 
 import torch
 
@@ -39,4 +48,177 @@ def fused_qknorm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, 
     return x
 
 
-__all__ = ["fused_qknorm_rope"]
+@dataclass(frozen=True)
+class AxialRotary:
+    """How the channels of a head turn with a token's position.
+
+    ``sections[a]`` pairs of channels turn with axis a, in the order of the axes (1 to 4 of them; all together P pairs,
+    2 P <= head_dim).  Pair i of an axis with n pairs turns by ``position * theta ** (-i / n)``; with
+    ``shared_frequencies`` by ``position * theta ** (-j / P)``, j its place among all pairs.  A pair is the channels
+    (i, i + P), or (2 i, 2 i + 1) with ``interleaved``; channels from 2 P on are not turned."""
+
+    sections: tuple[int, ...]
+    theta: float = 10000.0
+    interleaved: bool = False
+    shared_frequencies: bool = False
+
+    def __post_init__(self):
+        if not 1 <= len(self.sections) <= 4 or any(type(n) is not int or n < 0 for n in self.sections):
+            raise ValueError("sections must be 1 to 4 non-negative ints")
+        if self.pairs > 64 or self.pairs % (4 if self.interleaved else 8):
+            raise ValueError("the sections must add up to at most 64 pairs, a multiple of 8 (of 4 with interleaved pairs): "
+                             "the sm_100a kernel moves whole 8-channel vectors")
+        if not (self.theta > 0.0 and math.isfinite(self.theta)):
+            raise ValueError("theta must be positive")
+
+    @property
+    def pairs(self) -> int:
+        return sum(self.sections)
+
+    @cached_property
+    def _turns(self):
+        """Full turns per unit of position of every pair, as the library takes them."""
+        out, first = [], 0
+        for n in self.sections:
+            for i in range(n):
+                power = (first + i) / self.pairs if self.shared_frequencies else i / n
+                out.append(self.theta ** -power / (2.0 * math.pi))
+            first += n
+        return (C.c_double * max(1, len(out)))(*out)
+
+
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
+    if t.ndim != 4 or t.dtype not in (torch.float16, torch.bfloat16) or t.shape[-1] not in (64, 128):
+        raise ValueError(f"{name} must be (B, seq, heads, 64 or 128) in fp16 or bf16")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape[:2] != like.shape[:2]
+                             or t.shape[-1] != like.shape[-1]):
+        raise ValueError(f"{name} must have q's dtype, device, batch, sequence and head dimension")
+    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16
+                      or any(t.stride(i) % 8 for i in range(3) if t.size(i) > 1)):
+        raise ValueError(f"the heads of {name} must be contiguous and start on 16 bytes")
+    return t
+
+
+def _head_strides(t: torch.Tensor | None):
+    return (0, 0, 0) if t is None else tuple(t.stride(i) if t.size(i) > 1 else 0 for i in range(3))
+
+
+class _AxialCall:
+    """One call's arguments, checked and laid out as the kernels read them."""
+
+    def __init__(self, q, k, q_weight, k_weight, positions, rotary, eps):
+        if not isinstance(rotary, AxialRotary):
+            raise TypeError("rotary must be an AxialRotary")
+        _heads(q, "q")
+        if k is not None:
+            _heads(k, "k", q)
+        if not q.is_cuda:
+            raise ValueError("q must be on a CUDA device")
+        dim = q.shape[-1]
+        if 2 * rotary.pairs > dim:
+            raise ValueError(f"{rotary.pairs} pairs of channels do not fit a head of {dim}")
+        if k is not None and (q_weight is None) != (k_weight is None) or k is None and k_weight is not None:
+            raise ValueError("q_weight and k_weight go together")
+        weights = []
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None and (w.shape != (dim,) or w.dtype != q.dtype or w.device != q.device):
+                raise ValueError(f"{name} must be (head_dim,) of q's dtype, on its device")
+            w = None if w is None else w.contiguous()
+            weights.append(w.clone() if w is not None and w.data_ptr() % 16 else w)
+        self.q_weight, self.k_weight = weights
+        batch, tokens = q.shape[:2]
+        axes = len(rotary.sections)
+        if (positions.dtype not in _POSITION_TYPES or positions.device != q.device
+                or positions.shape not in ((tokens, axes), (batch, tokens, axes))):
+            raise ValueError("positions must be (seq, axes) or (B, seq, axes), int32, int64 or float32, on q's device")
+        if not (eps >= 0.0):
+            raise ValueError("eps must not be negative")
+        self.positions = positions.contiguous()
+        self.position_batch = tokens * axes if positions.ndim == 3 else 0
+        self.turns = rotary._turns
+        self.empty = batch == 0 or tokens == 0
+        self.shape = native.AxialRopeShape(
+            batch=batch, tokens=tokens, q_heads=q.size(2), k_heads=0 if k is None else k.size(2), head_dim=dim, axes=axes,
+            sections=(C.c_int32 * 4)(*rotary.sections), interleaved=int(rotary.interleaved),
+            positions_type=_POSITION_TYPES[positions.dtype], is_bf16=int(q.dtype == torch.bfloat16), eps=float(eps))
+        if q.size(2) == 0 or (k is not None and k.size(2) == 0):
+            raise ValueError("q and k need at least one head")
+
+
+def _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, inplace):
+    c = _AxialCall(q, k, q_weight, k_weight, positions, rotary, eps)
+    q_out = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = k if inplace or k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if not c.empty:
+        strides = [s for t in (q, k, q_out, k_out) for s in _head_strides(t)]
+        native.axial_rope(c.shape, q, k, c.q_weight, c.k_weight, c.positions, c.position_batch, c.turns, strides, q_out,
+                          k_out)
+    return q_out, k_out
+
+
+def _axial_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, rotary, eps, wanted=(True, True)):
+    c = _AxialCall(q, k, q_weight, k_weight, positions, rotary, eps)
+    for name, t, like in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
+        if (t is None) != (like is None) or t is not None and t.shape != like.shape:
+            raise ValueError(f"{name} must have the shape of the output")
+        if t is not None:
+            _heads(t, name, q)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    make = torch.zeros if c.empty else torch.empty
+    dq_weight, dk_weight = (None if w is None or not want else make(w.shape, dtype=w.dtype, device=w.device)
+                            for w, want in zip((c.q_weight, c.k_weight), wanted))
+    if not c.empty:
+        strides = [s for t in (dq_out, dk_out, q, k, dq, dk) for s in _head_strides(t)]
+        native.axial_rope_backward(c.shape, dq_out, dk_out, q, k, c.q_weight, c.k_weight, c.positions, c.position_batch,
+                                   c.turns, strides, dq, dk, dq_weight, dk_weight)
+    return dq, dk, dq_weight, dk_weight
+
+
+class _AxialRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, rotary, eps):
+        q_out, k_out = _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, False)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions)
+        ctx.options = (rotary, eps)
+        return q_out, k_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        grads = [None if t is None else t.contiguous() for t in (dq_out, dk_out)]
+        grads = [t.clone() if t is not None and t.data_ptr() % 16 else t for t in grads]
+        q, k, *_ = ctx.saved_tensors
+        if k is None:
+            grads[1] = None
+        out = _axial_backward(*grads, *ctx.saved_tensors, *ctx.options, wanted=ctx.needs_input_grad[2:4])
+        return (*(g if need else None for g, need in zip(out, ctx.needs_input_grad)), None, None, None)
+
+
+def fused_qknorm_axial_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None,
+                            k_weight: torch.Tensor | None, positions: torch.Tensor, rotary: AxialRotary,
+                            eps: float = 1e-6, *, inplace: bool = False):
+    """RMSNorm per head (none if both weights are None), then rotary positions, of ``(B, seq, heads, head_dim)`` queries and
+    keys (their numbers of heads may differ; k may be None).  Returns ``(q_out, k_out)``.
+
+    ``positions``: ``(seq, axes)`` or ``(B, seq, axes)``, whole or fractional.  New tensors, recorded by autograd; with
+    ``inplace`` q and k are overwritten, as ``fused_qknorm_rope`` does, which autograd cannot go through."""
+    if inplace:
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+            raise ValueError("inplace=True overwrites what the gradient needs")
+        return _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, True)
+    return _AxialRope.apply(q, k, q_weight, k_weight, positions, rotary, eps)
+
+
+def fused_qknorm_axial_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor | None, q: torch.Tensor,
+                                     k: torch.Tensor | None, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                                     positions: torch.Tensor, rotary: AxialRotary, eps: float = 1e-6):
+    """``(dq, dk, dq_weight, dk_weight)`` of ``fused_qknorm_axial_rope`` from the gradients of its outputs; ``q`` and ``k``
+    are its inputs.  Equal calls give equal bits."""
+    return _axial_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, rotary, eps)
+
+
+__all__ = ["AxialRotary", "fused_qknorm_axial_rope", "fused_qknorm_axial_rope_backward", "fused_qknorm_rope"]

@@ -447,6 +447,75 @@ int anemoi_sm100_qknorm_rope(void* x, const void* weight, const float* cos_table
 int anemoi_sm100_tensor_peak(int32_t kind, int32_t iterations, int32_t* status, double* flops,
                              void* stream);
 
+/* ---- the operators around a block's attention, with their gradients ---- */
+
+/* Rows of channels and what they share. */
+typedef struct anemoi_sm100_rows {
+  int64_t rows;         /* R */
+  int64_t groups;       /* G: modulation rows; R / G consecutive rows share one */
+  int32_t width;        /* C: a multiple of 8, at most 8,192 */
+  int32_t norm;         /* of the sum: 1 RMS norm, 2 layer norm */
+  int32_t post;         /* of y before the gate: 0 none, 1 RMS norm, 2 layer norm */
+  int32_t is_bf16;      /* type of the rows and weights: 1 bf16, 0 fp16 */
+  int32_t mod_is_fp32;  /* gate, scale, shift: 1 fp32, 0 the rows' type */
+  float eps;
+} anemoi_sm100_rows;
+
+/* x_out = x + gate * post(y); h_out = norm(x_out) * weight * (1 + scale) + shift.  `y` may be null (then `gate` and
+ * `post_weight`, too: h_out = the norm of x itself), `h_out` may be null (the residual alone), and so may scale, shift,
+ * weight and post_weight.  strides: of the rows of x, y, gate, scale, shift, in elements (multiples of 16 bytes; zero
+ * repeats a row); outputs are contiguous [R][C].  Every pointer on 16 bytes.  x_out may be x, and h_out y, where their rows are
+ * contiguous. */
+int anemoi_sm100_gate_norm_modulate(const anemoi_sm100_rows* r, const void* x, const void* y, const void* gate,
+                                    const void* scale, const void* shift, const void* weight, const void* post_weight,
+                                    const int64_t* strides, void* x_out, void* h_out, void* stream);
+
+/* Bytes of workspace of the gradient; `weights`: whether dweight or dpost_weight is wanted. */
+int64_t anemoi_sm100_gate_norm_modulate_backward_workspace(const anemoi_sm100_rows* r, int weights);
+
+/* Gradients from those of x_out and h_out (one of the two may be null).  `x` is the x_out of the call before (x itself
+ * without y); dx is both the gradient of x and of x_out.  dgate, dscale, dshift: contiguous [G][C] in the modulation's type,
+ * dweight, dpost_weight: [C] in the rows' type; each may be null, and then is not formed.  strides: of the rows of dx_out,
+ * dh, x, y, gate, scale.  The sums over rows are formed in a fixed order: equal calls give equal bits. */
+int anemoi_sm100_gate_norm_modulate_backward(const anemoi_sm100_rows* r, const void* dx_out, const void* dh, const void* x,
+                                             const void* y, const void* gate, const void* scale, const void* weight,
+                                             const void* post_weight, const int64_t* strides, void* dx, void* dy,
+                                             void* dgate, void* dscale, void* dshift, void* dweight, void* dpost_weight,
+                                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Queries and keys of the axial rotary embedding. */
+typedef struct anemoi_sm100_axial_rope_shape {
+  int64_t batch, tokens;
+  int32_t q_heads, k_heads;   /* k_heads 0: queries alone */
+  int32_t head_dim;           /* 64 or 128 */
+  int32_t axes;               /* 1 to 4 */
+  int32_t sections[4];        /* pairs of channels that each axis turns */
+  int32_t interleaved;        /* pairs: 0 channels i and i + P, 1 channels 2 i and 2 i + 1 (P: all pairs) */
+  int32_t positions_type;     /* 0 int32, 1 int64, 2 fp32 */
+  int32_t is_bf16;
+  float eps;
+} anemoi_sm100_axial_rope_shape;
+
+/* RMS norm per head with a weight (both weights null: none), then the rotation of pair i by
+ * positions[b][t][axis(i)] * 2 pi * turns[i].  `turns`: P doubles on the host, read before the call returns.
+ * positions: [batch][tokens][axes], `position_batch` elements from one sample to the next (0: shared).  P is a multiple of 8
+ * (4 with interleaved pairs).  strides: batch, token and head strides of q, k, q_out, k_out, multiples of 8 elements; every
+ * pointer on 16 bytes.  q_out / k_out may be q / k with the same strides. */
+int anemoi_sm100_axial_rope(const anemoi_sm100_axial_rope_shape* s, const void* q, const void* k, const void* q_weight,
+                            const void* k_weight, const void* positions, int64_t position_batch, const double* turns,
+                            const int64_t* strides, void* q_out, void* k_out, void* stream);
+
+/* Bytes of workspace of the gradient (the weights' partial sums). */
+int64_t anemoi_sm100_axial_rope_backward_workspace(const anemoi_sm100_axial_rope_shape* s);
+
+/* Gradients of q, k and the weights from those of the outputs.  Without weights q and k are not read and may be null.
+ * strides: batch, token and head strides of dq_out, dk_out, q, k, dq, dk.  Equal calls give equal bits. */
+int anemoi_sm100_axial_rope_backward(const anemoi_sm100_axial_rope_shape* s, const void* dq_out, const void* dk_out,
+                                     const void* q, const void* k, const void* q_weight, const void* k_weight,
+                                     const void* positions, int64_t position_batch, const double* turns,
+                                     const int64_t* strides, void* dq, void* dk, void* dq_weight, void* dk_weight,
+                                     void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
