@@ -1,0 +1,1459 @@
+// Dense softmax attention of [batch][tokens][heads][D] tensors in 16 bits (D = 64 or 128), with log-sum-exps, and its
+// backward pass, which recomputes the probabilities.
+//
+//   s_ij = scale * q_i . k_j,   P_ij = exp(s_ij - lse_i),   o_i = sum_j P_ij v_j,   lse_i = log sum_j exp(s_ij)
+//   dV = P^T dO     dP = dO V^T     delta_i = dO_i . o_i     dS = P (dP - delta)     dQ = scale dS K     dK = scale dS^T Q
+//
+// Query heads share key heads in equal groups.  Sample b has q_len[b] queries and k_len[b] keys (the tensors' lengths where
+// none are given); with `causal` query i sees the keys j <= i + k_len - q_len.  A query without a key has o = 0, lse = -inf
+// and no gradient; rows behind a length are written as zeros (lse: -inf) and what the inputs hold there is not used, be
+// it NaN: tiles that cross a length have those rows cleared in shared memory.
+//
+// All products run on tcgen05 (M = 128, fp32 accumulators in tensor memory), fed by tiled TMA with 128-byte swizzle straight
+// from the caller's strided tensors.  The backward pass is two kernels: one CTA per key tile sums dK and dV over the queries,
+// one per query tile sums dQ over the keys.  That forms S and dP twice (7 products instead of 5), but every sum is one CTA's,
+// in a fixed order: equal calls give equal bits, which atomic additions into dQ would not.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/anemoi_sm100.h"
+#include "bounded_wait.cuh"
+#include "layer.cuh"
+#include "packed.cuh"
+#include "rows.cuh"
+#include "sm100_primitives.cuh"
+
+namespace {
+
+using namespace sm100;
+
+constexpr int kThreads = 384, kTile = 128;
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kStatWarp = 10;
+constexpr uint64_t kDrainNs = 100000000ull;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Geometry {
+  const int32_t *q_lengths, *k_lengths;
+  int32_t* status;
+  uint64_t wait_ns;
+  int batch, q_heads, k_heads, q_tokens, k_tokens, causal, splits;
+  float scale;
+};
+
+struct Strides {
+  int64_t batch, token, head;
+};
+
+struct ForwardParams {
+  CUtensorMap q, k, v;
+  Geometry g;
+  void* out;
+  float* lse;
+  float* partial;  // with splits: [splits][B][H][q_tokens][D], then their lse [splits][B][H][q_tokens]
+  Strides o;
+};
+
+struct BackwardParams {
+  CUtensorMap q, k, v, dout;
+  Geometry g;                  // (splits: of the key tiles' queries)
+  const void *q_rows, *do_rows;
+  const float *lse2, *delta;   // [B][H][q_tokens]
+  const uint32_t* norms;       // fp16: largest |dO_i|^2 and |v_j|^2 per (sample, key head)
+  void *dq, *dk, *dv;
+  float *q_partial, *k_partial;  // with splits: [splits][B][H][q_tokens][D]; [splits][dV, dK][B][Hk][k_tokens][D]
+  Strides sq, sdo, sdq, sdk, sdv;
+  int q_splits, key_tiles, query_tiles, key_ctas;
+};
+
+__device__ __forceinline__ int length_of(const int32_t* lengths, int b, int tokens) {
+  return lengths == nullptr ? tokens : min(max(lengths[b], 0), tokens);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// 64 channels of 128 tokens of one head and sample: rows of 128 bytes, 16-byte pieces swizzled within groups of eight rows.
+__device__ __forceinline__ void tensor_g2s(uint8_t* dst, const CUtensorMap* map, int channel, int head, int token, int batch,
+                                           uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(channel), "r"(head), "r"(token), "r"(batch), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int D>
+constexpr int kTileBytes = kTile * D * 2;
+
+// One thread: a tile's copies.
+template <int D>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, int head, int token, int batch,
+                                          uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, kTileBytes<D>);
+#pragma unroll
+  for (int c = 0; c < D; c += 64) tensor_g2s(dst + c * (kTile * 2), map, c, head, token, batch, bar);
+}
+
+// A warp: a tile of which only the first `valid` rows count.  The copy lands on `side`; then the other rows are cleared and
+// `bar` is told.  (Rows behind the tensor's last token arrive as zeros, but rows between a length and that are the
+// caller's, and zero times NaN is NaN.)
+template <int D>
+__device__ __forceinline__ void load_cut_tile(uint8_t* dst, const CUtensorMap* map, int head, int token, int batch,
+                                              int valid, uint64_t* side, uint32_t& side_uses, uint64_t* bar,
+                                              WaitContext* wc) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) load_tile<D>(dst, map, head, token, batch, side);
+  __syncwarp();
+  wait(wc, side, side_uses & 1, 40);
+  ++side_uses;
+  for (int i = valid * 8 + lane; i < kTile * 8; i += 32)
+#pragma unroll
+    for (int c = 0; c < D; c += 64)
+      *reinterpret_cast<uint4*>(dst + c * (kTile * 2) + i * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+// Descriptors of a tile as operand: its channels as K (row major), or its tokens as K.
+__device__ __forceinline__ uint64_t by_channels(uint32_t addr) { return smem_desc(addr, 16, 1024) | (2ull << 61); }
+__device__ __forceinline__ uint64_t by_tokens(uint32_t addr) { return smem_desc(addr, kTile * 128, 1024) | (2ull << 61); }
+
+template <bool kBf16>
+constexpr uint32_t kFormat = kBf16 ? kFmtBF16 : kFmtF16;
+
+// acc[128 x 128] = A B^T over D channels, both tiles in shared memory.  One thread.
+template <int D, bool kBf16>
+__device__ __forceinline__ void scores_ss(uint32_t acc, uint32_t a, uint32_t b) {
+  constexpr uint32_t idesc = instr_desc(kFormat<kBf16>, kFormat<kBf16>, kAccF32, 128, 128, 0, 0);
+  const uint64_t ad = by_channels(a), bd = by_channels(b);
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    const uint32_t step = k / 4 * (kTile * 128 / 16) + k % 4 * 2;
+    mma_f16_ss(acc, ad + step, bd + step, idesc, k > 0);
+  }
+}
+// The same, A in tensor memory.
+template <int D, bool kBf16>
+__device__ __forceinline__ void scores_ts(uint32_t acc, uint32_t a, uint32_t b) {
+  constexpr uint32_t idesc = instr_desc(kFormat<kBf16>, kFormat<kBf16>, kAccF32, 128, 128, 0, 0);
+  const uint64_t bd = by_channels(b);
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k)
+    mma_f16_ts(acc, a + k * 8, bd + k / 4 * (kTile * 128 / 16) + k % 4 * 2, idesc, k > 0);
+}
+// acc[128 x D] += A B over 128 tokens: A in tensor memory, its columns in two halves `half` columns apart.
+template <int D, bool kBf16>
+__device__ __forceinline__ void gather_ts(uint32_t acc, uint32_t a, uint32_t half, uint32_t b, bool accumulate) {
+  constexpr uint32_t idesc = instr_desc(kFormat<kBf16>, kFormat<kBf16>, kAccF32, 128, D, 0, 1);
+  const uint64_t bd = by_tokens(b);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    mma_f16_ts(acc, a + k / 4 * half + k % 4 * 8, bd + k * (2 * 1024 / 16), idesc, k > 0 || accumulate);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return kBf16 ? rows::Pair<__nv_bfloat16>::round(a, b) : rows::Pair<__half>::round(a, b);
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// 32 accumulator columns of the thread's row, times `factor`, as 16-bit values to `dst`.
+template <bool kBf16>
+__device__ __forceinline__ void store32(const uint32_t (&r)[32], float factor, uint16_t* dst) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = pack2<kBf16>(__uint_as_float(r[i + 2 * j]) * factor, __uint_as_float(r[i + 2 * j + 1]) * factor);
+    *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+__device__ __forceinline__ void store32_fp32(const uint32_t (&r)[32], float factor, float* dst) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4)
+    *reinterpret_cast<float4*>(dst + i) =
+        make_float4(__uint_as_float(r[i]) * factor, __uint_as_float(r[i + 1]) * factor, __uint_as_float(r[i + 2]) * factor,
+                    __uint_as_float(r[i + 3]) * factor);
+}
+
+struct SharedHead {
+  WaitContext wc;
+  uint32_t tmem_base;
+};
+
+// Common start: barriers initialised by thread 0, tensor memory allocated by the MMA warp.
+__device__ __forceinline__ uint32_t tmem_begin(SharedHead* s) {
+  if (threadIdx.x >> 5 == kMmaWarp) {
+    tmem_alloc(&s->tmem_base, 512);
+    tmem_relinquish();
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  tc_fence_after_sync();
+  return s->tmem_base;
+}
+__device__ __forceinline__ void tmem_end(uint32_t base) {
+  tc_fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x >> 5 == kMmaWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc(base, 512);
+  }
+}
+__device__ __forceinline__ void begin_waits(SharedHead* s, const Geometry& g) {
+  s->wc.abort = 0;
+  s->wc.status = g.status;
+  s->wc.limit_ns = g.wait_ns;
+}
+// After a give-up anywhere on the device the status word stays set: CTAs that start later leave at once.
+__device__ __forceinline__ bool given_up(const Geometry& g) {
+  return __syncthreads_or(threadIdx.x == 0 && *reinterpret_cast<volatile int32_t*>(g.status) != 0);
+}
+// Once per warp: what the warp did to tensor memory and its reads of it come before the arrival.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  tc_fence_before_sync();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// Keys that a query tile's rows may see: [0, end).
+__device__ __forceinline__ int key_end(const Geometry& g, int q0, int q_len, int k_len) {
+  if (!g.causal) return k_len;
+  const int last = min(q0, q_len) - 1 + k_len - q_len;  // q0: the first row behind the tile
+  return max(0, min(k_len, last + 1));
+}
+
+// ------------------------------------------------------------------------------------------
+// forward
+// ------------------------------------------------------------------------------------------
+// A CTA has two tiles of 128 queries, a softmax warpgroup each; keys and values come in stages of 128.  While one tile's
+// probabilities are formed, the tensor core runs the other tile's products.  Tensor memory: scores of the tiles at columns
+// 0 and 128 (their probabilities replace them, 64 columns), outputs at 256 and 256 + D.
+template <int D>
+struct ForwardShared {
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  SharedHead head;
+  uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_ready[2], o_done[2],
+      side;
+};
+template <int D>
+constexpr int kForwardTiles = 2 + 2 * ForwardShared<D>::kStages;
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_constant__ ForwardParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  static_assert(256 + 2 * D <= 512, "scores and outputs of two tiles");
+  constexpr int kStages = ForwardShared<D>::kStages, kBytes = kTileBytes<D>;
+  auto* s = reinterpret_cast<ForwardShared<D>*>(smem + kForwardTiles<D> * kBytes);
+  const Geometry& g = p.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z / g.splits, split = blockIdx.z % g.splits, h = blockIdx.y, hk = h / (g.q_heads / g.k_heads);
+  // (the longest walks first)
+  const int q0 = (g.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * 2 * kTile;
+  const int q_len = length_of(g.q_lengths, b, g.q_tokens), k_len = length_of(g.k_lengths, b, g.k_tokens);
+  const int keys = q0 < q_len ? key_end(g, q0 + 2 * kTile, q_len, k_len) : 0;
+  const int all = (keys + kTile - 1) / kTile;
+  const int first = (int)((int64_t)all * split / g.splits), n = (int)((int64_t)all * (split + 1) / g.splits) - first;
+  const int tiles = q0 + kTile < q_len ? 2 : 1;
+  if (given_up(g)) return;
+  if (threadIdx.x == 0) {
+    begin_waits(&s->head, g);
+    mbar_init(&s->q_full, 2);
+    mbar_init(&s->side, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s->k_full[i], 1);
+      mbar_init(&s->k_empty[i], 1);
+      mbar_init(&s->v_full[i], 1);
+      mbar_init(&s->v_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s->s_full[t], 1);
+      mbar_init(&s->p_ready[t], 4);
+      mbar_init(&s->o_done[t], 1);
+    }
+    mbar_init_fence();
+  }
+  const uint32_t tmem = tmem_begin(&s->head);
+  WaitContext* wc = &s->head.wc;
+  uint8_t *k_tiles = smem + 2 * kBytes, *v_tiles = k_tiles + kStages * kBytes;
+
+  if (warp == kLoadWarp) {
+    if (n > 0) {
+      uint32_t side_uses = 0;
+      if (lane == 0)
+        for (int t = 0; t < 2; ++t) load_tile<D>(smem + t * kBytes, &p.q, h, min(q0 + t * kTile, g.q_tokens), b, &s->q_full);
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int st = i % kStages, use = i / kStages, token = (first + i) * kTile;
+        if (use > 0) wait(wc, &s->k_empty[st], (use - 1) & 1, 41);
+        if (lane == 0) load_tile<D>(k_tiles + st * kBytes, &p.k, hk, token, b, &s->k_full[st]);
+        __syncwarp();
+        if (use > 0) wait(wc, &s->v_empty[st], (use - 1) & 1, 42);
+        if (token + kTile > k_len && k_len < g.k_tokens) {
+          load_cut_tile<D>(v_tiles + st * kBytes, &p.v, hk, token, b, k_len - token, &s->side, side_uses, &s->v_full[st], wc);
+        } else if (lane == 0) {
+          load_tile<D>(v_tiles + st * kBytes, &p.v, hk, token, b, &s->v_full[st]);
+        }
+        __syncwarp();
+      }
+      if (wc->abort) {
+        // unwinding: the copies in flight have to land before the CTA gives its shared memory back
+        drain_wait(&s->q_full, 0, kDrainNs);
+        for (int i = max(0, n - kStages); i < n; ++i) {
+          drain_wait(&s->k_full[i % kStages], (i / kStages) & 1, kDrainNs);
+          drain_wait(&s->v_full[i % kStages], (i / kStages) & 1, kDrainNs);
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (n > 0) {
+      const bool leader = elect_one();
+      const uint32_t qa = smem_u32(smem), ka = smem_u32(k_tiles), va = smem_u32(v_tiles);
+      wait(wc, &s->q_full, 0, 43);
+      wait(wc, &s->k_full[0], 0, 44);
+      tc_fence_after_sync();
+      if (leader) {
+        for (int t = 0; t < tiles; ++t) {
+          scores_ss<D, kBf16>(tmem + t * 128, qa + t * kBytes, ka);
+          mma_commit(&s->s_full[t]);
+        }
+        mma_commit(&s->k_empty[0]);
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int st = i % kStages, next = (i + 1) % kStages;
+        wait(wc, &s->v_full[st], (i / kStages) & 1, 45);
+#pragma unroll 1
+        for (int t = 0; t < tiles; ++t) {
+          wait(wc, &s->p_ready[t], i & 1, 46);
+          tc_fence_after_sync();
+          if (leader) {
+            gather_ts<D, kBf16>(tmem + 256 + t * D, tmem + t * 128, 32, va + st * kBytes, i > 0);
+            mma_commit(&s->o_done[t]);
+          }
+          __syncwarp();
+          if (i + 1 < n) {
+            if (t == 0) {
+              wait(wc, &s->k_full[next], ((i + 1) / kStages) & 1, 47);
+              tc_fence_after_sync();
+            }
+            // (the probabilities in this place: read by the products issued just before, which run first)
+            if (leader) {
+              scores_ss<D, kBf16>(tmem + t * 128, qa + t * kBytes, ka + next * kBytes);
+              mma_commit(&s->s_full[t]);
+            }
+            __syncwarp();
+          }
+        }
+        if (leader) {
+          mma_commit(&s->v_empty[st]);
+          if (i + 1 < n) mma_commit(&s->k_empty[next]);
+        }
+        __syncwarp();
+      }
+      if (wc->abort) {
+        // the last v_empty follows everything issued
+        drain_wait(&s->v_empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, kDrainNs);
+      }
+    }
+  } else if (warp < 8) {
+    const int t = warp >> 2, row = q0 + t * kTile + (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t scores = tmem + lanes + t * 128, acc = tmem + lanes + 256 + t * D;
+    const float c = g.scale * kLog2e;
+    const int seen = g.causal ? min(k_len, row + 1 + k_len - q_len) : k_len;  // keys that this row sees
+    // (a warp masks a stage that one of its rows does not see whole)
+    const int least = __reduce_min_sync(0xffffffffu, seen);
+    float m = -INFINITY, sum = 0.0f;
+    const bool live = t < tiles && n > 0;
+    if (live) {
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        wait(wc, &s->s_full[t], i & 1, 48);
+        tc_fence_after_sync();
+        float v[128];
+#pragma unroll
+        for (int c0 = 0; c0 < 128; c0 += 32) tmem_ld32(scores + c0, *reinterpret_cast<uint32_t(*)[32]>(v + c0));
+        tmem_wait_ld();
+        const int key0 = (first + i) * kTile;
+        if (key0 + kTile > least) {
+          const int valid = seen - key0;
+#pragma unroll
+          for (int j = 0; j < 128; ++j) v[j] = j < valid ? v[j] : -INFINITY;
+        }
+        float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int j = 4; j < 128; j += 4)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], v[j + k]);
+        const float m_new = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
+        // The maximum that the sums refer to is kept while the true one is less than 2^8 above it: the probabilities
+        // then reach 256 at most, which the types hold, and sum and outputs stay relative to each other.
+        const bool move = i == 0 || (m_new - m) * c > 8.0f || (m == -INFINITY && m_new != -INFINITY);
+        if (i == 0) {
+          m = m_new;
+        } else if (__any_sync(0xffffffffu, move)) {
+          const float alpha = move ? exp2_approx((m - m_new) * c) : 1.0f;
+          wait(wc, &s->o_done[t], (i - 1) & 1, 49);
+          tc_fence_after_sync();
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            uint32_t r[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                  "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                : "r"(acc + c0)
+                : "memory");
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
+            tmem_st16(acc + c0, r);
+          }
+          sum *= alpha;
+          if (move) m = m_new;
+        }
+        const float base = m == -INFINITY ? 0.0f : -m * c;
+        const float2 c2 = make_float2(c, c), base2 = make_float2(base, base);
+        float2 sum2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float2 e = ffma2(make_float2(v[c0 + j], v[c0 + j + 1]), c2, base2);
+            e.x = exp2_approx(e.x);
+            e.y = exp2_approx(e.y);
+            sum2 = fadd2(sum2, e);
+            packed[j / 2] = pack2<kBf16>(e.x, e.y);
+          }
+          tmem_st16(scores + c0 / 2, packed);
+        }
+        sum += sum2.x + sum2.y;
+        tmem_wait_st();
+        warp_arrive(&s->p_ready[t]);
+      }
+      wait(wc, &s->o_done[t], (n - 1) & 1, 50);
+      tc_fence_after_sync();
+    }
+    // all lanes read (the loads are the warp's), rows that exist are written
+    const bool given = live && row < q_len && sum != 0.0f;  // (NaN is an answer, too)
+    const float factor = given ? 1.0f / sum : 0.0f, lse = given ? (m * c + log2f(sum)) * kLn2 : -INFINITY;
+    const int64_t flat = ((int64_t)b * g.q_heads + h) * g.q_tokens + row;
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 32) {
+      uint32_t r[32];
+      if (live) {
+        tmem_ld32(acc + c0, r);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (!given) r[j] = 0u;
+      if (row < g.q_tokens) {
+        if (g.splits > 1) {
+          const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens;
+          store32_fp32(r, factor, p.partial + ((int64_t)split * rows_all + flat) * D + c0);
+        } else {
+          store32<kBf16>(r, factor,
+                         static_cast<uint16_t*>(p.out) + b * p.o.batch + (int64_t)row * p.o.token + h * p.o.head + c0);
+        }
+      }
+    }
+    if (row < g.q_tokens) {
+      if (g.splits > 1) {
+        const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens;
+        p.partial[(int64_t)g.splits * rows_all * D + (int64_t)split * rows_all + flat] = lse;
+      } else if (p.lse != nullptr) {
+        p.lse[flat] = lse;
+      }
+    }
+  }
+  tmem_end(tmem);
+}
+
+// Joins a row's parts, in order: weights exp(lse_s - lse).  D / 4 threads per row.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(128) join_forward_kernel(const float* partial, int splits, int64_t rows_all, int q_heads,
+                                                           int q_tokens, Strides o, void* out, float* lse_out) {
+  layer::grid_dependency_wait();
+  constexpr int kLanes = D / 4;
+  const int64_t flat = (int64_t)blockIdx.x * (128 / kLanes) + threadIdx.x / kLanes;
+  if (flat >= rows_all) return;
+  const int c = threadIdx.x % kLanes * 4;
+  const float* lses = partial + (int64_t)splits * rows_all * D + flat;
+  float top = -INFINITY;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, lses[(int64_t)s * rows_all]);
+  float sum = 0.0f, v[4] = {};
+  const float base = top == -INFINITY ? 0.0f : top;
+  for (int s = 0; s < splits; ++s) {
+    const float w = exp2_approx((lses[(int64_t)s * rows_all] - base) * kLog2e);
+    const float4 o4 = *reinterpret_cast<const float4*>(partial + ((int64_t)s * rows_all + flat) * D + c);
+    sum += w;
+    v[0] = fmaf(w, o4.x, v[0]);
+    v[1] = fmaf(w, o4.y, v[1]);
+    v[2] = fmaf(w, o4.z, v[2]);
+    v[3] = fmaf(w, o4.w, v[3]);
+  }
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int64_t bh = flat / q_tokens, row = flat - bh * q_tokens, b = bh / q_heads, h = bh - b * q_heads;
+  uint16_t* dst = static_cast<uint16_t*>(out) + b * o.batch + row * o.token + h * o.head + c;
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(pack2<kBf16>(v[0] * inverse, v[1] * inverse), pack2<kBf16>(v[2] * inverse, v[3] * inverse));
+  if (c == 0 && lse_out != nullptr) lse_out[flat] = sum == 0.0f ? -INFINITY : base + log2f(sum) * kLn2;
+}
+
+// ------------------------------------------------------------------------------------------
+// backward: what the kernels need of each row
+// ------------------------------------------------------------------------------------------
+struct RowParams {
+  const void *out, *dout, *v;
+  const float* lse;
+  float *lse2, *delta;
+  uint32_t* norms;
+  Strides so, sd, sv;
+  const int32_t *q_lengths, *k_lengths;
+  int batch, q_heads, k_heads, q_tokens, k_tokens, q_blocks;
+};
+
+// delta_i and the log-sum-exp in units of log 2 (+inf where the row has no gradient: its probabilities then come out as
+// zeros).  fp16: the largest |dO_i|^2 and |v_j|^2 of each key head, too (a maximum does not depend on the order of atomics).
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowParams p) {
+  using T = std::conditional_t<kBf16, __nv_bfloat16, __half>;
+  constexpr int kLanes = D / 8;
+  const bool values = (int)blockIdx.x >= p.q_blocks;
+  const int64_t at = (int64_t)(values ? blockIdx.x - p.q_blocks : blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes, heads = values ? p.k_heads : p.q_heads, tokens = values ? p.k_tokens : p.q_tokens;
+  const bool in = at < (int64_t)p.batch * heads * tokens;
+  const int64_t token_row = in ? at / heads : 0;  // rows in memory order: heads of a token, tokens, samples
+  const int h = in ? (int)(at - token_row * heads) : 0, b = (int)(token_row / tokens), i = (int)(token_row - (int64_t)b * tokens);
+  const bool live = in && i < length_of(values ? p.k_lengths : p.q_lengths, b, tokens);
+  float d[8] = {}, o[8] = {};
+  if (live) {
+    const Strides& sd = values ? p.sv : p.sd;
+    rows::open8<T>(rows::load_stream(static_cast<const T*>(values ? p.v : p.dout) + b * sd.batch + (int64_t)i * sd.token +
+                                     h * sd.head + lane * 8),
+                   d);
+    if (!values)
+      rows::open8<T>(rows::load_stream(static_cast<const T*>(p.out) + b * p.so.batch + (int64_t)i * p.so.token +
+                                       h * p.so.head + lane * 8),
+                     o);
+  }
+  float dot = 0.0f, norm = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    dot = fmaf(d[j], o[j], dot);
+    norm = fmaf(d[j], d[j], norm);
+  }
+#pragma unroll
+  for (int off = kLanes / 2; off > 0; off >>= 1) {
+    dot += __shfl_xor_sync(0xffffffffu, dot, off);
+    norm += __shfl_xor_sync(0xffffffffu, norm, off);
+  }
+  if (!in || lane != 0) return;
+  if (!values) {
+    const int64_t flat = ((int64_t)b * p.q_heads + h) * p.q_tokens + i;
+    const float lse = live ? p.lse[flat] : -INFINITY;
+    p.lse2[flat] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+    p.delta[flat] = live && lse != -INFINITY ? dot : 0.0f;
+  }
+  if (p.norms != nullptr && live)
+    atomicMax(p.norms + 2 * (b * p.k_heads + (values ? h : h / (p.q_heads / p.k_heads))) + (values ? 1 : 0),
+              __float_as_uint(norm));
+}
+
+// Powers of two that keep the 16-bit operands P and dS inside fp16's range.  fp16 has no exponents below 2^-14, and over a
+// long sequence P is about 1 / keys and dS that times a gradient: both would lose their bits or vanish.  P <= 1 goes in
+// times 2^15.  |dP_ij - delta_i| <= 2 |dO_i| |v_j|, so dS goes in times the largest power of two that keeps that bound below
+// 2^15.  bf16 has the exponents of fp32: no factors.  Without more than one key the probability is constant and dS = 0,
+// which a factor of zero makes exact.
+struct Scaling {
+  float p_shift;  // log2 of P's factor
+  float ds;       // dS operand = P operand * (dP * ds - delta * ds)
+  float dv, dk;   // of the accumulators
+};
+template <bool kBf16>
+__device__ __forceinline__ Scaling scaling(const BackwardParams& p, int b, int hk, int k_len) {
+  Scaling s{0.0f, k_len > 1 ? 1.0f : 0.0f, 1.0f, p.g.scale};
+  if (kBf16) return s;
+  const float bound = sqrtf(__uint_as_float(p.norms[2 * (b * p.g.k_heads + hk)])) *
+                      sqrtf(__uint_as_float(p.norms[2 * (b * p.g.k_heads + hk) + 1]));
+  int e = 0;
+  if (bound > 0.0f && bound < INFINITY) e = min(60, max(-60, 13 - ilogbf(bound)));  // 2^e * 2 * bound <= 2^15
+  s.p_shift = 15.0f;
+  s.dv = 1.0f / 32768.0f;
+  if (k_len > 1) s.ds = exp2f((float)(e - 15));
+  s.dk = p.g.scale * exp2f((float)-e);
+  return s;
+}
+
+// ------------------------------------------------------------------------------------------
+// backward: dK and dV of a key tile
+// ------------------------------------------------------------------------------------------
+// Rows of the accumulators are keys, columns queries: S^T = K Q^T, dP^T = V dO^T, then P^T and dS^T are operands in tensor
+// memory as they stand, and the tiles of Q and dO serve both ways (channels as K, tokens as K).  Two warpgroups take
+// 64 columns each.  Tensor memory: S^T [0, 128), dP^T [128, 256) (P^T and dS^T replace them, each half's 32 columns at the
+// half's start), dV at 256, dK at 256 + D.  Order of the tensor core: dV(i), S(i + 1) | dK(i), dP(i + 1): the first pair
+// runs while dS(i) is formed, the second while P(i + 1) is.
+template <int D>
+struct KeyShared {
+  SharedHead head;
+  uint64_t kv_full, q_full[2], q_empty[2], do_full[2], do_empty[2], stat_full[2], stat_empty[2], s_full, p_ready, dp_full,
+      ds_ready, all_done, side[2];
+  float lse2[2][kTile], delta[2][kTile];
+};
+
+template <int D, bool kBf16>
+__device__ __forceinline__ void key_tile(const BackwardParams& p, uint8_t* smem, int tile, int hk, int b, int split) {
+  constexpr int kBytes = kTileBytes<D>;
+  auto* s = reinterpret_cast<KeyShared<D>*>(smem + 6 * kBytes);
+  const Geometry& g = p.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = g.q_heads / g.k_heads, k0 = tile * kTile;
+  const int q_len = length_of(g.q_lengths, b, g.q_tokens), k_len = length_of(g.k_lengths, b, g.k_tokens);
+  // query tiles that see a key of this tile, of each head of the group
+  const int q_tiles = k0 < k_len ? (q_len + kTile - 1) / kTile : 0;
+  const int q_first = g.causal ? min(q_tiles, max(0, k0 - (k_len - q_len)) / kTile) : 0;
+  const int per_head = q_tiles - q_first, all = per_head * group;
+  const int first = (int)((int64_t)all * split / g.splits), n = (int)((int64_t)all * (split + 1) / g.splits) - first;
+  if (threadIdx.x == 0) {
+    begin_waits(&s->head, g);
+    mbar_init(&s->kv_full, 2);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s->q_full[i], 1);
+      mbar_init(&s->q_empty[i], 1);
+      mbar_init(&s->do_full[i], 1);
+      mbar_init(&s->do_empty[i], 1);
+      mbar_init(&s->stat_full[i], 1);
+      mbar_init(&s->stat_empty[i], 8);
+      mbar_init(&s->side[i], 1);
+    }
+    mbar_init(&s->s_full, 1);
+    mbar_init(&s->p_ready, 8);
+    mbar_init(&s->dp_full, 1);
+    mbar_init(&s->ds_ready, 8);
+    mbar_init(&s->all_done, 1);
+    mbar_init_fence();
+  }
+  const uint32_t tmem = tmem_begin(&s->head);
+  WaitContext* wc = &s->head.wc;
+  uint8_t *k_tile = smem, *v_tile = smem + kBytes, *q_tiles_at = smem + 2 * kBytes, *do_tiles_at = smem + 4 * kBytes;
+  const Scaling f = scaling<kBf16>(p, b, hk, k_len);
+
+  if (warp == kLoadWarp) {
+    if (n > 0) {
+      uint32_t side_uses[2] = {0, 0};
+      if (lane == 0) {
+        load_tile<D>(k_tile, &p.k, hk, k0, b, &s->kv_full);
+        load_tile<D>(v_tile, &p.v, hk, k0, b, &s->kv_full);
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int st = i & 1, use = i >> 1, h = hk * group + (first + i) / per_head;
+        const int token = (q_first + (first + i) % per_head) * kTile;
+        const bool cut = token + kTile > q_len && q_len < g.q_tokens;
+        if (use > 0) wait(wc, &s->q_empty[st], (use - 1) & 1, 51);
+        if (cut) {
+          load_cut_tile<D>(q_tiles_at + st * kBytes, &p.q, h, token, b, q_len - token, &s->side[0], side_uses[0],
+                           &s->q_full[st], wc);
+        } else if (lane == 0) {
+          load_tile<D>(q_tiles_at + st * kBytes, &p.q, h, token, b, &s->q_full[st]);
+        }
+        __syncwarp();
+        if (use > 0) wait(wc, &s->do_empty[st], (use - 1) & 1, 52);
+        if (cut) {
+          load_cut_tile<D>(do_tiles_at + st * kBytes, &p.dout, h, token, b, q_len - token, &s->side[1], side_uses[1],
+                           &s->do_full[st], wc);
+        } else if (lane == 0) {
+          load_tile<D>(do_tiles_at + st * kBytes, &p.dout, h, token, b, &s->do_full[st]);
+        }
+        __syncwarp();
+      }
+      if (wc->abort) {
+        drain_wait(&s->kv_full, 0, kDrainNs);
+        for (int i = max(0, n - 2); i < n; ++i) {
+          drain_wait(&s->q_full[i & 1], (i >> 1) & 1, kDrainNs);
+          drain_wait(&s->do_full[i & 1], (i >> 1) & 1, kDrainNs);
+        }
+      }
+    }
+  } else if (warp == kStatWarp) {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1, use = i >> 1, h = hk * group + (first + i) / per_head;
+      const int token = (q_first + (first + i) % per_head) * kTile;
+      const int64_t flat = ((int64_t)b * g.q_heads + h) * g.q_tokens;
+      float l[4], d[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = token + j * 32 + lane;
+        l[j] = row < g.q_tokens ? p.lse2[flat + row] - f.p_shift : INFINITY;
+        d[j] = row < g.q_tokens ? p.delta[flat + row] * f.ds : 0.0f;
+      }
+      if (use > 0) wait(wc, &s->stat_empty[st], (use - 1) & 1, 53);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s->lse2[st][j * 32 + lane] = -l[j];
+        s->delta[st][j * 32 + lane] = -d[j];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s->stat_full[st]);
+    }
+  } else if (warp == kMmaWarp) {
+    if (n > 0) {
+      const bool leader = elect_one();
+      const uint32_t ka = smem_u32(k_tile), va = smem_u32(v_tile), qa = smem_u32(q_tiles_at), da = smem_u32(do_tiles_at);
+      wait(wc, &s->kv_full, 0, 54);
+      wait(wc, &s->q_full[0], 0, 55);
+      tc_fence_after_sync();
+      if (leader) {
+        scores_ss<D, kBf16>(tmem, ka, qa);
+        mma_commit(&s->s_full);
+      }
+      __syncwarp();
+      wait(wc, &s->do_full[0], 0, 56);
+      tc_fence_after_sync();
+      if (leader) {
+        scores_ss<D, kBf16>(tmem + 128, va, da);
+        mma_commit(&s->dp_full);
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int st = i & 1, next = st ^ 1;
+        wait(wc, &s->p_ready, i & 1, 57);
+        tc_fence_after_sync();
+        if (leader) {
+          gather_ts<D, kBf16>(tmem + 256, tmem, 64, da + st * kBytes, i > 0);
+          mma_commit(&s->do_empty[st]);
+        }
+        __syncwarp();
+        if (i + 1 < n) {
+          wait(wc, &s->q_full[next], ((i + 1) >> 1) & 1, 58);
+          tc_fence_after_sync();
+          if (leader) {
+            scores_ss<D, kBf16>(tmem, ka, qa + next * kBytes);
+            mma_commit(&s->s_full);
+          }
+          __syncwarp();
+        }
+        wait(wc, &s->ds_ready, i & 1, 59);
+        tc_fence_after_sync();
+        if (leader) {
+          gather_ts<D, kBf16>(tmem + 256 + D, tmem + 128, 64, qa + st * kBytes, i > 0);
+          mma_commit(&s->q_empty[st]);
+        }
+        __syncwarp();
+        if (i + 1 < n) {
+          wait(wc, &s->do_full[next], ((i + 1) >> 1) & 1, 60);
+          tc_fence_after_sync();
+          if (leader) {
+            scores_ss<D, kBf16>(tmem + 128, va, da + next * kBytes);
+            mma_commit(&s->dp_full);
+          }
+          __syncwarp();
+        }
+      }
+      if (leader) mma_commit(&s->all_done);
+      __syncwarp();
+      if (wc->abort) drain_wait(&s->all_done, 0, kDrainNs);
+    }
+  } else if (warp < 8) {
+    const int half = warp >> 2, row = k0 + (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t scores = tmem + lanes + half * 64, grads = scores + 128;
+    const float c = g.scale * kLog2e;
+    const float2 c2 = make_float2(c, c), ds2 = make_float2(f.ds, f.ds);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1;
+      const int token = (q_first + (first + i) % per_head) * kTile + half * 64;
+      wait(wc, &s->stat_full[st], (i >> 1) & 1, 61);
+      wait(wc, &s->s_full, i & 1, 62);
+      tc_fence_after_sync();
+      float v[64];
+      tmem_ld32(scores, *reinterpret_cast<uint32_t(*)[32]>(v));
+      tmem_ld32(scores + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+      tmem_wait_ld();
+      const float4* l4 = reinterpret_cast<const float4*>(s->lse2[st] + half * 64);
+#pragma unroll
+      for (int j = 0; j < 64; j += 4) {
+        const float4 l = l4[j / 4];
+        const float2 a = ffma2(make_float2(v[j], v[j + 1]), c2, make_float2(l.x, l.y));
+        const float2 e = ffma2(make_float2(v[j + 2], v[j + 3]), c2, make_float2(l.z, l.w));
+        v[j] = exp2_approx(a.x);
+        v[j + 1] = exp2_approx(a.y);
+        v[j + 2] = exp2_approx(e.x);
+        v[j + 3] = exp2_approx(e.y);
+      }
+      if (g.causal) {
+        // query token + j sees key `row` from j >= hidden on
+        const int hidden = row - (k_len - q_len) - token;
+        if (__any_sync(0xffffffffu, hidden > 0)) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] = j >= hidden ? v[j] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) packed[j] = pack2<kBf16>(v[c0 + 2 * j], v[c0 + 2 * j + 1]);
+        tmem_st16(scores + c0 / 2, packed);
+      }
+      tmem_wait_st();
+      warp_arrive(&s->p_ready);
+      wait(wc, &s->dp_full, i & 1, 63);
+      tc_fence_after_sync();
+      const float4* d4 = reinterpret_cast<const float4*>(s->delta[st] + half * 64);
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t r[32], packed[16];
+        tmem_ld32(grads + c0, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 d = d4[(c0 + j) / 4];
+          const float2 a = ffma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), ds2, make_float2(d.x, d.y));
+          const float2 e =
+              ffma2(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), ds2, make_float2(d.z, d.w));
+          const float2 x = fmul2(a, make_float2(v[c0 + j], v[c0 + j + 1]));
+          const float2 y = fmul2(e, make_float2(v[c0 + j + 2], v[c0 + j + 3]));
+          packed[j / 2] = pack2<kBf16>(x.x, x.y);
+          packed[j / 2 + 1] = pack2<kBf16>(y.x, y.y);
+        }
+        // (the first 32 columns' results go where the warp has read already)
+        tmem_st16(grads + c0 / 2, packed);
+      }
+      tmem_wait_st();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s->stat_empty[st]);
+      warp_arrive(&s->ds_ready);
+    }
+    if (n > 0) {
+      wait(wc, &s->all_done, 0, 64);
+      tc_fence_after_sync();
+    }
+    // the first warpgroup writes dV, the second dK
+    const bool live = n > 0 && row < k_len;
+    const float factor = half == 0 ? f.dv : f.dk;
+    const Strides& out = half == 0 ? p.sdv : p.sdk;
+    uint16_t* dst = static_cast<uint16_t*>(half == 0 ? p.dv : p.dk) + b * out.batch + (int64_t)row * out.token + hk * out.head;
+    const int64_t rows_all = (int64_t)g.batch * g.k_heads * g.k_tokens;
+    float* part = p.k_partial + (((int64_t)split * 2 + half) * rows_all + ((int64_t)b * g.k_heads + hk) * g.k_tokens + row) * D;
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 32) {
+      uint32_t r[32];
+      if (n > 0) {
+        tmem_ld32(tmem + lanes + 256 + half * D + c0, r);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (!live) r[j] = 0u;
+      if (row < g.k_tokens) {
+        if (g.splits > 1) {
+          store32_fp32(r, factor, part + c0);
+        } else {
+          store32<kBf16>(r, factor, dst + c0);
+        }
+      }
+    }
+  }
+  tmem_end(tmem);
+}
+
+// ------------------------------------------------------------------------------------------
+// backward: dQ of a query tile
+// ------------------------------------------------------------------------------------------
+// Rows are queries, columns keys.  Q and dO are operands in tensor memory (columns 384 and 384 + D / 2), so that a stage of
+// 128 keys reads K twice and V once from shared memory.  S [0, 128), dP [128, 256) (dS replaces it), dQ at 256.  The
+// scores of the next stage are computed as soon as this one's have been read.
+template <int D>
+struct QueryShared {
+  static constexpr int kStages = 3;
+  SharedHead head;
+  uint64_t moved, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full, s_read, dp_full, ds_ready,
+      all_done, side;
+};
+
+template <int D, bool kBf16>
+__device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* smem, int tile, int h, int b, int split) {
+  constexpr int kBytes = kTileBytes<D>, kStages = QueryShared<D>::kStages;
+  auto* s = reinterpret_cast<QueryShared<D>*>(smem + 2 * kStages * kBytes);
+  const Geometry& g = p.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = h / (g.q_heads / g.k_heads), q0 = tile * kTile;
+  const int q_len = length_of(g.q_lengths, b, g.q_tokens), k_len = length_of(g.k_lengths, b, g.k_tokens);
+  const int keys = q0 < q_len ? key_end(g, q0 + kTile, q_len, k_len) : 0, all = (keys + kTile - 1) / kTile;
+  const int first = (int)((int64_t)all * split / p.q_splits), n = (int)((int64_t)all * (split + 1) / p.q_splits) - first;
+  if (threadIdx.x == 0) {
+    begin_waits(&s->head, g);
+    mbar_init(&s->moved, 8);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s->k_full[i], 1);
+      mbar_init(&s->k_empty[i], 1);
+      mbar_init(&s->v_full[i], 1);
+      mbar_init(&s->v_empty[i], 1);
+    }
+    mbar_init(&s->s_full, 1);
+    mbar_init(&s->s_read, 8);
+    mbar_init(&s->dp_full, 1);
+    mbar_init(&s->ds_ready, 8);
+    mbar_init(&s->all_done, 1);
+    mbar_init(&s->side, 1);
+    mbar_init_fence();
+  }
+  const uint32_t tmem = tmem_begin(&s->head);
+  WaitContext* wc = &s->head.wc;
+  uint8_t *k_tiles = smem, *v_tiles = smem + kStages * kBytes;
+  const uint32_t q_at = tmem + 384, do_at = tmem + 384 + D / 2;
+  const Scaling f = scaling<kBf16>(p, b, hk, k_len);
+
+  if (warp == kLoadWarp) {
+    uint32_t side_uses = 0;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int st = i % kStages, use = i / kStages, token = (first + i) * kTile;
+      if (use > 0) wait(wc, &s->k_empty[st], (use - 1) & 1, 71);
+      if (token + kTile > k_len && k_len < g.k_tokens) {
+        load_cut_tile<D>(k_tiles + st * kBytes, &p.k, hk, token, b, k_len - token, &s->side, side_uses, &s->k_full[st], wc);
+      } else if (lane == 0) {
+        load_tile<D>(k_tiles + st * kBytes, &p.k, hk, token, b, &s->k_full[st]);
+      }
+      __syncwarp();
+      if (use > 0) wait(wc, &s->v_empty[st], (use - 1) & 1, 72);
+      if (lane == 0) load_tile<D>(v_tiles + st * kBytes, &p.v, hk, token, b, &s->v_full[st]);
+      __syncwarp();
+    }
+    if (wc->abort)
+      for (int i = max(0, n - kStages); i < n; ++i) {
+        drain_wait(&s->k_full[i % kStages], (i / kStages) & 1, kDrainNs);
+        drain_wait(&s->v_full[i % kStages], (i / kStages) & 1, kDrainNs);
+      }
+  } else if (warp == kMmaWarp) {
+    if (n > 0) {
+      const bool leader = elect_one();
+      const uint32_t ka = smem_u32(k_tiles), va = smem_u32(v_tiles);
+      wait(wc, &s->moved, 0, 73);
+      wait(wc, &s->k_full[0], 0, 74);
+      tc_fence_after_sync();
+      if (leader) {
+        scores_ts<D, kBf16>(tmem, q_at, ka);
+        mma_commit(&s->s_full);
+      }
+      __syncwarp();
+      wait(wc, &s->v_full[0], 0, 75);
+      tc_fence_after_sync();
+      if (leader) {
+        scores_ts<D, kBf16>(tmem + 128, do_at, va);
+        mma_commit(&s->dp_full);
+        mma_commit(&s->v_empty[0]);
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int st = i % kStages, next = (i + 1) % kStages, parity = ((i + 1) / kStages) & 1;
+        if (i + 1 < n) {
+          wait(wc, &s->s_read, i & 1, 76);
+          wait(wc, &s->k_full[next], parity, 77);
+          tc_fence_after_sync();
+          if (leader) {
+            scores_ts<D, kBf16>(tmem, q_at, ka + next * kBytes);
+            mma_commit(&s->s_full);
+          }
+          __syncwarp();
+        }
+        wait(wc, &s->ds_ready, i & 1, 78);
+        tc_fence_after_sync();
+        if (leader) {
+          gather_ts<D, kBf16>(tmem + 256, tmem + 128, 64, ka + st * kBytes, i > 0);
+          mma_commit(&s->k_empty[st]);
+        }
+        __syncwarp();
+        if (i + 1 < n) {
+          wait(wc, &s->v_full[next], parity, 79);
+          tc_fence_after_sync();
+          if (leader) {
+            scores_ts<D, kBf16>(tmem + 128, do_at, va + next * kBytes);
+            mma_commit(&s->dp_full);
+            mma_commit(&s->v_empty[next]);
+          }
+          __syncwarp();
+        }
+      }
+      if (leader) mma_commit(&s->all_done);
+      __syncwarp();
+      if (wc->abort) drain_wait(&s->all_done, 0, kDrainNs);
+    }
+  } else if (warp < 8) {
+    const int half = warp >> 2, local = (warp & 3) * 32 + lane, row = q0 + local;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t scores = tmem + lanes + half * 64, grads = scores + 128;
+    const float c = g.scale * kLog2e;
+    const int64_t flat = ((int64_t)b * g.q_heads + h) * g.q_tokens + row;
+    const bool in = row < q_len;
+    const float lse2 = in ? f.p_shift - p.lse2[flat] : -INFINITY, delta = in ? -p.delta[flat] * f.ds : 0.0f;
+    if (n > 0) {
+      // the first warpgroup's threads read their row of Q, the second's of dO, and move it to tensor memory
+      const Strides& st = half == 0 ? p.sq : p.sdo;
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(half == 0 ? p.q_rows : p.do_rows) +
+                                                        b * st.batch + (int64_t)row * st.token + h * st.head);
+      const uint32_t dst = (half == 0 ? q_at : do_at) + lanes;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t r[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 v = in ? __ldg(src + c0 / 8 + j) : make_uint4(0, 0, 0, 0);
+          r[4 * j] = v.x;
+          r[4 * j + 1] = v.y;
+          r[4 * j + 2] = v.z;
+          r[4 * j + 3] = v.w;
+        }
+        tmem_st16(dst + c0 / 2, r);
+      }
+      tmem_wait_st();
+      warp_arrive(&s->moved);
+    }
+    const int seen = g.causal ? min(k_len, row + 1 + k_len - q_len) : k_len;
+    const int least = __reduce_min_sync(0xffffffffu, seen);
+    const float2 c2 = make_float2(c, c), l2 = make_float2(lse2, lse2), ds2 = make_float2(f.ds, f.ds),
+                 d2 = make_float2(delta, delta);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      wait(wc, &s->s_full, i & 1, 80);
+      tc_fence_after_sync();
+      float v[64];
+      tmem_ld32(scores, *reinterpret_cast<uint32_t(*)[32]>(v));
+      tmem_ld32(scores + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+      tmem_wait_ld();
+      warp_arrive(&s->s_read);
+#pragma unroll
+      for (int j = 0; j < 64; j += 2) {
+        const float2 a = ffma2(make_float2(v[j], v[j + 1]), c2, l2);
+        v[j] = exp2_approx(a.x);
+        v[j + 1] = exp2_approx(a.y);
+      }
+      const int key0 = (first + i) * kTile + half * 64;
+      const bool masked = key0 + 64 > least;
+      wait(wc, &s->dp_full, i & 1, 81);
+      tc_fence_after_sync();
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t r[32], packed[16];
+        tmem_ld32(grads + c0, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 a = ffma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), ds2, d2);
+          float2 x = fmul2(a, make_float2(v[c0 + j], v[c0 + j + 1]));
+          if (masked) {
+            // (what stands behind the keys may be NaN)
+            x.x = key0 + c0 + j < seen ? x.x : 0.0f;
+            x.y = key0 + c0 + j + 1 < seen ? x.y : 0.0f;
+          }
+          packed[j / 2] = pack2<kBf16>(x.x, x.y);
+        }
+        tmem_st16(grads + c0 / 2, packed);
+      }
+      tmem_wait_st();
+      warp_arrive(&s->ds_ready);
+    }
+    if (n > 0) {
+      wait(wc, &s->all_done, 0, 82);
+      tc_fence_after_sync();
+    }
+    // each warpgroup writes half of the channels
+    uint16_t* dst = static_cast<uint16_t*>(p.dq) + b * p.sdq.batch + (int64_t)row * p.sdq.token + h * p.sdq.head;
+    float* part = p.q_partial + (int64_t)split * g.batch * g.q_heads * g.q_tokens * D + flat * D;
+#pragma unroll 1
+    for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
+      uint32_t r[32];
+      if (n > 0) {
+        tmem_ld32(tmem + lanes + 256 + c0, r);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (n == 0 || !in) r[j] = 0u;
+      if (row < g.q_tokens) {
+        if (p.q_splits > 1) {
+          store32_fp32(r, f.dk, part + c0);
+        } else {
+          store32<kBf16>(r, f.dk, dst + c0);
+        }
+      }
+    }
+  }
+  tmem_end(tmem);
+}
+
+// Both kinds of tiles in one launch: the query tiles fill the SMs that the last key tiles leave.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1) backward_kernel(const __grid_constant__ BackwardParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  layer::grid_dependency_wait();
+  if (given_up(p.g)) return;
+  int at = blockIdx.x;
+  if (at < p.key_ctas) {
+    const int tile = at % p.key_tiles;
+    at /= p.key_tiles;
+    const int hk = at % p.g.k_heads;
+    at /= p.g.k_heads;
+    key_tile<D, kBf16>(p, smem, tile, hk, at / p.g.splits, at % p.g.splits);
+    return;
+  }
+  at -= p.key_ctas;
+  const int tile = at % p.query_tiles;
+  at /= p.query_tiles;
+  const int h = at % p.g.q_heads;
+  at /= p.g.q_heads;
+  query_tile<D, kBf16>(p, smem, p.g.causal ? p.query_tiles - 1 - tile : tile, h, at / p.q_splits, at % p.q_splits);
+}
+
+// Adds the parts of gradient rows, in order.  D / 4 threads per row; blockIdx.y: which of `kinds` gradients.
+struct JoinParams {
+  const float* partial;
+  void* out[2];
+  Strides strides[2];
+  int64_t rows_all;
+  int splits, kinds, heads, tokens;
+};
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ JoinParams p) {
+  layer::grid_dependency_wait();
+  constexpr int kLanes = D / 4;
+  const int64_t flat = (int64_t)blockIdx.x * (128 / kLanes) + threadIdx.x / kLanes;
+  if (flat >= p.rows_all) return;
+  const int c = threadIdx.x % kLanes * 4, kind = blockIdx.y;
+  float v[4] = {};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(p.partial + (((int64_t)s * p.kinds + kind) * p.rows_all + flat) * D + c);
+    v[0] += x.x;
+    v[1] += x.y;
+    v[2] += x.z;
+    v[3] += x.w;
+  }
+  const int64_t bh = flat / p.tokens, row = flat - bh * p.tokens, b = bh / p.heads, h = bh - b * p.heads;
+  const Strides& o = p.strides[kind];
+  uint16_t* dst = static_cast<uint16_t*>(p.out[kind]) + b * o.batch + row * o.token + h * o.head + c;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBf16>(v[0], v[1]), pack2<kBf16>(v[2], v[3]));
+}
+
+// ------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) == cudaSuccess &&
+                   found == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeTiled>(f)
+               : nullptr;
+  }();
+  return fn;
+}
+
+struct Tensor {
+  const void* at;
+  int heads, tokens;
+  Strides s;
+};
+
+bool encode(CUtensorMap* map, const Tensor& t, bool bf16, int d, int batch) {
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)t.heads, (cuuint64_t)t.tokens, (cuuint64_t)batch};
+  const cuuint64_t strides[3] = {(cuuint64_t)t.s.head * 2, (cuuint64_t)t.s.token * 2, (cuuint64_t)t.s.batch * 2};
+  const cuuint32_t box[4] = {64, 1, kTile, 1}, step[4] = {1, 1, 1, 1};
+  return encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                        const_cast<void*>(t.at), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A tensor's strides as TMA takes them: a dimension of one entry may have any, and gets its packed one.
+bool tensor_of(Tensor* t, const void* at, int heads, int tokens, int d, const int64_t* strides, int batch) {
+  t->at = at;
+  t->heads = heads;
+  t->tokens = tokens;
+  t->s.head = heads == 1 ? d : strides[2];
+  t->s.token = tokens == 1 ? (int64_t)heads * d : strides[1];
+  t->s.batch = batch == 1 ? (int64_t)tokens * heads * d : strides[0];
+  for (int64_t v : {t->s.head, t->s.token, t->s.batch})
+    if (v <= 0 || v % 8 || v >= (1ll << 39)) return false;
+  return reinterpret_cast<uintptr_t>(at) % 16 == 0;
+}
+
+int check(const anemoi_sm100_dense_shape* s) {
+  if (s == nullptr || s->batch <= 0 || s->q_heads <= 0 || s->k_heads <= 0 || s->q_heads % s->k_heads || s->q_tokens <= 0 ||
+      s->k_tokens <= 0 || (s->head_dim != 64 && s->head_dim != 128) || !(s->scale > 0.0f) || !(s->scale < INFINITY))
+    return ANEMOI_SM100_EINVAL;
+  // tile and row counts in 32 bits, with room for the splits
+  if (s->q_tokens > 0x3fffffff || s->k_tokens > 0x3fffffff || s->q_heads > 65535 || s->batch > 4095 ||
+      (int64_t)s->batch * s->q_heads * ((std::max(s->q_tokens, s->k_tokens) + kTile - 1) / kTile) > (1 << 25))
+    return ANEMOI_SM100_ELIMIT;
+  return ANEMOI_SM100_OK;
+}
+
+int tiles_of(int tokens) { return (tokens + kTile - 1) / kTile; }
+
+// Parts of a walk of `steps` tiles by each of `ctas` CTAs: where these leave SMs idle, each walk is cut so that all have a
+// part, of two steps at least.  By the shape alone (a sample's lengths may be shorter).
+int parts_of(int64_t ctas, int steps) {
+  if (ctas >= rows::kSms) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(rows::kSms / ctas, steps / 2));
+}
+
+struct Plan {
+  int forward_splits, key_splits, query_splits;
+};
+Plan plan_of(const anemoi_sm100_dense_shape* s) {
+  const int64_t qt = tiles_of(s->q_tokens), kt = tiles_of(s->k_tokens), b = s->batch;
+  const int group = s->q_heads / s->k_heads;
+  Plan p;
+  p.forward_splits = parts_of((qt + 1) / 2 * s->q_heads * b, (int)kt);
+  p.key_splits = parts_of(kt * s->k_heads * b, (int)std::min<int64_t>(1 << 20, qt * group));
+  p.query_splits = parts_of(qt * s->q_heads * b, (int)kt);
+  return p;
+}
+
+void geometry(Geometry& g, const anemoi_sm100_dense_shape* s, const int32_t* q_lengths, const int32_t* k_lengths,
+              int32_t* status) {
+  g.q_lengths = q_lengths;
+  g.k_lengths = k_lengths;
+  g.status = status;
+  g.wait_ns = layer::wait_limit_ns();
+  g.batch = s->batch;
+  g.q_heads = s->q_heads;
+  g.k_heads = s->k_heads;
+  g.q_tokens = s->q_tokens;
+  g.k_tokens = s->k_tokens;
+  g.causal = s->causal != 0;
+  g.scale = s->scale;
+}
+
+template <int D, bool kBf16>
+int forward_launch(ForwardParams& p, cudaStream_t st) {
+  auto kernel = forward_kernel<D, kBf16>;
+  const size_t smem = (size_t)kForwardTiles<D> * kTileBytes<D> + sizeof(ForwardShared<D>);
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return ANEMOI_SM100_ELAUNCH;
+  const Geometry& g = p.g;
+  kernel<<<dim3((g.q_tokens + 2 * kTile - 1) / (2 * kTile), g.q_heads, g.batch * g.splits), kThreads, smem, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+  if (g.splits == 1) return ANEMOI_SM100_OK;
+  const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens, per_block = 128 / (D / 4);
+  if (layer::launch(join_forward_kernel<D, kBf16>, dim3((unsigned)((rows_all + per_block - 1) / per_block)), dim3(128), 0, st,
+                    (const float*)p.partial, g.splits, rows_all, g.q_heads, g.q_tokens, p.o, p.out, p.lse) != cudaSuccess)
+    return ANEMOI_SM100_ELAUNCH;
+  return ANEMOI_SM100_OK;
+}
+
+template <int D, bool kBf16>
+int backward_launch(const BackwardParams& p, const RowParams& r, cudaStream_t st) {
+  const Geometry& g = p.g;
+  const int64_t per_block = 256 / (D / 8);
+  const int64_t q_blocks = ((int64_t)g.batch * g.q_heads * g.q_tokens + per_block - 1) / per_block;
+  const int64_t v_blocks = kBf16 ? 0 : ((int64_t)g.batch * g.k_heads * g.k_tokens + per_block - 1) / per_block;
+  if (q_blocks + v_blocks > 0x7fffffffLL) return ANEMOI_SM100_ELIMIT;
+  RowParams rp = r;
+  rp.q_blocks = (int)q_blocks;
+  if (!kBf16 && cudaMemsetAsync(rp.norms, 0, (size_t)g.batch * g.k_heads * 2 * sizeof(uint32_t), st) != cudaSuccess)
+    return ANEMOI_SM100_ELAUNCH;
+  row_kernel<D, kBf16><<<(unsigned)(q_blocks + v_blocks), 256, 0, st>>>(rp);
+  if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+  auto kernel = backward_kernel<D, kBf16>;
+  const size_t smem = 6 * (size_t)kTileBytes<D> + std::max(sizeof(KeyShared<D>), sizeof(QueryShared<D>));
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return ANEMOI_SM100_ELAUNCH;
+  const int64_t ctas = p.key_ctas + (int64_t)p.query_tiles * g.q_heads * g.batch * p.q_splits;
+  if (layer::launch(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, st, p) != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+  for (int which = 0; which < 2; ++which) {
+    const bool keys = which == 0;
+    if ((keys ? g.splits : p.q_splits) == 1) continue;
+    JoinParams j{};
+    j.partial = keys ? p.k_partial : p.q_partial;
+    j.out[0] = keys ? p.dv : p.dq;
+    j.out[1] = p.dk;
+    j.strides[0] = keys ? p.sdv : p.sdq;
+    j.strides[1] = p.sdk;
+    j.heads = keys ? g.k_heads : g.q_heads;
+    j.tokens = keys ? g.k_tokens : g.q_tokens;
+    j.rows_all = (int64_t)g.batch * j.heads * j.tokens;
+    j.splits = keys ? g.splits : p.q_splits;
+    j.kinds = keys ? 2 : 1;
+    const int64_t join_rows = 128 / (D / 4);
+    if (layer::launch(join_kernel<D, kBf16>, dim3((unsigned)((j.rows_all + join_rows - 1) / join_rows), j.kinds), dim3(128), 0,
+                      st, j) != cudaSuccess)
+      return ANEMOI_SM100_ELAUNCH;
+  }
+  return ANEMOI_SM100_OK;
+}
+
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+
+extern "C" int64_t anemoi_sm100_dense_attention_workspace(const anemoi_sm100_dense_shape* s) {
+  const int bad = check(s);
+  if (bad != ANEMOI_SM100_OK) return bad;
+  const Plan plan = plan_of(s);
+  const int64_t rows_all = (int64_t)s->batch * s->q_heads * s->q_tokens;
+  return plan.forward_splits > 1 ? plan.forward_splits * rows_all * (s->head_dim + 1) * (int64_t)sizeof(float) : 0;
+}
+
+extern "C" int anemoi_sm100_dense_attention(const anemoi_sm100_dense_shape* s, const void* q, const void* k, const void* v,
+                                            const int32_t* q_lengths, const int32_t* k_lengths, const int64_t* strides,
+                                            void* out, float* lse, void* workspace, int64_t workspace_bytes, int32_t* status,
+                                            void* stream) {
+  const int bad = check(s);
+  if (bad != ANEMOI_SM100_OK) return bad;
+  if (!q || !k || !v || !out || !strides || !status) return ANEMOI_SM100_EINVAL;
+  const int64_t needed = anemoi_sm100_dense_attention_workspace(s);
+  if (needed > 0 && (!workspace || workspace_bytes < needed || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return ANEMOI_SM100_EINVAL;
+  const int d = s->head_dim;
+  Tensor tq, tk, tv, to;
+  if (!tensor_of(&tq, q, s->q_heads, s->q_tokens, d, strides, s->batch) ||
+      !tensor_of(&tk, k, s->k_heads, s->k_tokens, d, strides + 3, s->batch) ||
+      !tensor_of(&tv, v, s->k_heads, s->k_tokens, d, strides + 6, s->batch) ||
+      !tensor_of(&to, out, s->q_heads, s->q_tokens, d, strides + 9, s->batch))
+    return ANEMOI_SM100_EINVAL;
+  if (encode_tiled() == nullptr) return ANEMOI_SM100_ELAUNCH;
+  ForwardParams p{};
+  const bool bf16 = s->is_bf16 != 0;
+  if (!encode(&p.q, tq, bf16, d, s->batch) || !encode(&p.k, tk, bf16, d, s->batch) || !encode(&p.v, tv, bf16, d, s->batch))
+    return ANEMOI_SM100_EINVAL;
+  geometry(p.g, s, q_lengths, k_lengths, status);
+  p.g.splits = plan_of(s).forward_splits;
+  p.out = out;
+  p.lse = lse;
+  p.partial = static_cast<float*>(workspace);
+  p.o = to.s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (d == 64) return bf16 ? forward_launch<64, true>(p, st) : forward_launch<64, false>(p, st);
+  return bf16 ? forward_launch<128, true>(p, st) : forward_launch<128, false>(p, st);
+}
+
+extern "C" int64_t anemoi_sm100_dense_attention_backward_workspace(const anemoi_sm100_dense_shape* s) {
+  const int bad = check(s);
+  if (bad != ANEMOI_SM100_OK) return bad;
+  const Plan plan = plan_of(s);
+  const int64_t q_rows = (int64_t)s->batch * s->q_heads * s->q_tokens, k_rows = (int64_t)s->batch * s->k_heads * s->k_tokens;
+  int64_t bytes = 2 * round16(q_rows * 4) + round16((int64_t)s->batch * s->k_heads * 8);
+  if (plan.query_splits > 1) bytes += plan.query_splits * q_rows * s->head_dim * 4;
+  if (plan.key_splits > 1) bytes += plan.key_splits * 2 * k_rows * s->head_dim * 4;
+  return bytes;
+}
+
+extern "C" int anemoi_sm100_dense_attention_backward(const anemoi_sm100_dense_shape* s, const void* dout, const void* q,
+                                                     const void* k, const void* v, const void* out, const float* lse,
+                                                     const int32_t* q_lengths, const int32_t* k_lengths,
+                                                     const int64_t* strides, void* dq, void* dk, void* dv, void* workspace,
+                                                     int64_t workspace_bytes, int32_t* status, void* stream) {
+  const int bad = check(s);
+  if (bad != ANEMOI_SM100_OK) return bad;
+  if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv || !strides || !status || !workspace)
+    return ANEMOI_SM100_EINVAL;
+  if (workspace_bytes < anemoi_sm100_dense_attention_backward_workspace(s) || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return ANEMOI_SM100_EINVAL;
+  const int d = s->head_dim;
+  Tensor t[8];
+  const void* at[8] = {dout, q, k, v, out, dq, dk, dv};
+  for (int i = 0; i < 8; ++i) {
+    const bool of_q = i == 0 || i == 1 || i == 4 || i == 5;
+    if (!tensor_of(&t[i], at[i], of_q ? s->q_heads : s->k_heads, of_q ? s->q_tokens : s->k_tokens, d, strides + 3 * i,
+                   s->batch))
+      return ANEMOI_SM100_EINVAL;
+  }
+  if (encode_tiled() == nullptr) return ANEMOI_SM100_ELAUNCH;
+  BackwardParams p{};
+  const bool bf16 = s->is_bf16 != 0;
+  if (!encode(&p.dout, t[0], bf16, d, s->batch) || !encode(&p.q, t[1], bf16, d, s->batch) ||
+      !encode(&p.k, t[2], bf16, d, s->batch) || !encode(&p.v, t[3], bf16, d, s->batch))
+    return ANEMOI_SM100_EINVAL;
+  geometry(p.g, s, q_lengths, k_lengths, status);
+  const Plan plan = plan_of(s);
+  p.g.splits = plan.key_splits;
+  p.q_splits = plan.query_splits;
+  p.key_tiles = tiles_of(s->k_tokens);
+  p.query_tiles = tiles_of(s->q_tokens);
+  p.key_ctas = p.key_tiles * s->k_heads * s->batch * plan.key_splits;
+  const int64_t q_rows = (int64_t)s->batch * s->q_heads * s->q_tokens;
+  char* w = static_cast<char*>(workspace);
+  float* lse2 = reinterpret_cast<float*>(w);
+  w += round16(q_rows * 4);
+  float* delta = reinterpret_cast<float*>(w);
+  w += round16(q_rows * 4);
+  uint32_t* norms = reinterpret_cast<uint32_t*>(w);
+  w += round16((int64_t)s->batch * s->k_heads * 8);
+  p.q_partial = reinterpret_cast<float*>(w);
+  p.k_partial = p.q_partial + (plan.query_splits > 1 ? plan.query_splits * q_rows * d : 0);
+  p.q_rows = q;
+  p.do_rows = dout;
+  p.lse2 = lse2;
+  p.delta = delta;
+  p.norms = norms;
+  p.dq = dq;
+  p.dk = dk;
+  p.dv = dv;
+  p.sdo = t[0].s;
+  p.sq = t[1].s;
+  p.sdq = t[5].s;
+  p.sdk = t[6].s;
+  p.sdv = t[7].s;
+  RowParams r{};
+  r.out = out;
+  r.dout = dout;
+  r.v = v;
+  r.lse = lse;
+  r.lse2 = lse2;
+  r.delta = delta;
+  r.norms = bf16 ? nullptr : norms;
+  r.so = t[4].s;
+  r.sd = t[0].s;
+  r.sv = t[3].s;
+  r.q_lengths = q_lengths;
+  r.k_lengths = k_lengths;
+  r.batch = s->batch;
+  r.q_heads = s->q_heads;
+  r.k_heads = s->k_heads;
+  r.q_tokens = s->q_tokens;
+  r.k_tokens = s->k_tokens;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (d == 64) return bf16 ? backward_launch<64, true>(p, r, st) : backward_launch<64, false>(p, r, st);
+  return bf16 ? backward_launch<128, true>(p, r, st) : backward_launch<128, false>(p, r, st);
+}

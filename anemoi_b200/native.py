@@ -92,6 +92,13 @@ class AxialRopeShape(C.Structure):
                 ("positions_type", C.c_int32), ("is_bf16", C.c_int32), ("eps", C.c_float)]
 
 
+class DenseShape(C.Structure):
+    """Dense attention with a gradient (``anemoi_sm100_dense_shape``)."""
+
+    _fields_ = [(name, C.c_int32) for name in ("batch", "q_heads", "k_heads", "q_tokens", "k_tokens", "head_dim", "causal",
+                                               "is_bf16")] + [("scale", C.c_float)]
+
+
 @lru_cache(maxsize=1)
 def library() -> C.CDLL:
     """Load the in-tree shared library; raise if it has not been built."""
@@ -104,6 +111,7 @@ def library() -> C.CDLL:
     lib = C.CDLL(str(path))
     P, I32, I64, F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
     SP, OP, RP, AP = C.POINTER(Shape), C.POINTER(Operands), C.POINTER(Rows), C.POINTER(AxialRopeShape)
+    DP = C.POINTER(DenseShape)
     signatures = {
         "anemoi_sm100_arch": (C.c_int, []),
         "anemoi_sm100_operand_bytes": (I64, [SP, C.c_int]),
@@ -170,6 +178,11 @@ def library() -> C.CDLL:
         "anemoi_sm100_axial_rope_backward_workspace": (I64, [AP]),
         "anemoi_sm100_axial_rope_backward": (C.c_int, [AP, P, P, P, P, P, P, P, I64, C.POINTER(C.c_double), C.POINTER(I64),
                                                        P, P, P, P, P, I64, P]),
+        "anemoi_sm100_dense_attention_workspace": (I64, [DP]),
+        "anemoi_sm100_dense_attention": (C.c_int, [DP, P, P, P, P, P, C.POINTER(I64), P, P, P, I64, P, P]),
+        "anemoi_sm100_dense_attention_backward_workspace": (I64, [DP]),
+        "anemoi_sm100_dense_attention_backward": (C.c_int, [DP, P, P, P, P, P, P, P, P, C.POINTER(I64), P, P, P, P, I64, P,
+                                                            P]),
     }
     for name, (restype, argtypes) in signatures.items():
         fn = getattr(lib, name)
@@ -201,7 +214,8 @@ EXPORTED = (
     "anemoi_sm100_peer_close", "anemoi_sm100_peer_free",
     "anemoi_sm100_gate_norm_modulate", "anemoi_sm100_gate_norm_modulate_backward_workspace",
     "anemoi_sm100_gate_norm_modulate_backward", "anemoi_sm100_axial_rope", "anemoi_sm100_axial_rope_backward_workspace",
-    "anemoi_sm100_axial_rope_backward",
+    "anemoi_sm100_axial_rope_backward", "anemoi_sm100_dense_attention_workspace", "anemoi_sm100_dense_attention",
+    "anemoi_sm100_dense_attention_backward_workspace", "anemoi_sm100_dense_attention_backward",
 )
 
 
@@ -812,3 +826,28 @@ def axial_rope_backward(shape: AxialRopeShape, dq_out, dk_out, q, k, q_weight, k
             C.byref(shape), _at(dq_out), _at(dk_out), _at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions),
             position_batch, turns, (C.c_int64 * 18)(*strides), _at(dq), _at(dk), _at(dq_weight), _at(dk_weight),
             _at(space), nbytes, torch.cuda.current_stream().cuda_stream), "anemoi_sm100_axial_rope_backward")
+
+
+def dense_attention(shape: DenseShape, q, k, v, q_lengths, k_lengths, strides, out, lse, status) -> None:
+    lib = library()
+    with torch.cuda.device(q.device):
+        nbytes = int(lib.anemoi_sm100_dense_attention_workspace(C.byref(shape)))
+        space = _workspace(nbytes, q.device)
+        _count("dense_attention", 2 if nbytes else 1)
+        _check(lib.anemoi_sm100_dense_attention(
+            C.byref(shape), _at(q), _at(k), _at(v), _at(q_lengths), _at(k_lengths), (C.c_int64 * 12)(*strides), _at(out),
+            _at(lse), _at(space), nbytes, _at(status), torch.cuda.current_stream().cuda_stream),
+            "anemoi_sm100_dense_attention")
+
+
+def dense_attention_backward(shape: DenseShape, dout, q, k, v, out, lse, q_lengths, k_lengths, strides, dq, dk, dv,
+                             status) -> None:
+    lib = library()
+    with torch.cuda.device(q.device):
+        nbytes = int(lib.anemoi_sm100_dense_attention_backward_workspace(C.byref(shape)))
+        space = _workspace(nbytes, q.device)
+        _count("dense_attention_backward", 2)
+        _check(lib.anemoi_sm100_dense_attention_backward(
+            C.byref(shape), _at(dout), _at(q), _at(k), _at(v), _at(out), _at(lse), _at(q_lengths), _at(k_lengths),
+            (C.c_int64 * 24)(*strides), _at(dq), _at(dk), _at(dv), _at(space), nbytes, _at(status),
+            torch.cuda.current_stream().cuda_stream), "anemoi_sm100_dense_attention_backward")

@@ -516,6 +516,38 @@ int anemoi_sm100_axial_rope_backward(const anemoi_sm100_axial_rope_shape* s, con
                                      const int64_t* strides, void* dq, void* dk, void* dq_weight, void* dk_weight,
                                      void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Dense softmax attention with a gradient: [batch][tokens][heads][D] tensors. */
+typedef struct anemoi_sm100_dense_shape {
+  int32_t batch;
+  int32_t q_heads, k_heads;   /* q_heads a multiple of k_heads: head h reads key head h / (q_heads / k_heads) */
+  int32_t q_tokens, k_tokens;
+  int32_t head_dim;           /* 64 or 128 */
+  int32_t causal;             /* query i sees keys j <= i + (keys of the sample) - (queries of the sample) */
+  int32_t is_bf16;
+  float scale;                /* of q . k, positive */
+} anemoi_sm100_dense_shape;
+
+/* Bytes of workspace of the forward pass (zero where no walk over the keys is split). */
+int64_t anemoi_sm100_dense_attention_workspace(const anemoi_sm100_dense_shape* s);
+
+/* out = softmax(scale q k^T) v; lse [batch][q_heads][q_tokens] fp32, the rows' log-sum-exps (may be null).
+ * q_lengths, k_lengths: [batch] on the device, valid leading tokens of each sample (null: all; values are clamped to the
+ * tensors' lengths).  Rows of out behind a length, and those that see no key, are zeros, their lse -inf.  strides: batch,
+ * token and head strides of q, k, v, out, multiples of 8 elements; pointers on 16 bytes.  `status`: as of the attention
+ * kernels, non-zero after a bounded wait gave up. */
+int anemoi_sm100_dense_attention(const anemoi_sm100_dense_shape* s, const void* q, const void* k, const void* v,
+                                 const int32_t* q_lengths, const int32_t* k_lengths, const int64_t* strides, void* out,
+                                 float* lse, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+int64_t anemoi_sm100_dense_attention_backward_workspace(const anemoi_sm100_dense_shape* s);
+
+/* Gradients of q, k, v from that of out; `out` and `lse` are the forward pass's.  strides: of dout, q, k, v, out, dq, dk, dv.
+ * Rows behind a length get zeros.  No atomic additions: equal calls give equal bits. */
+int anemoi_sm100_dense_attention_backward(const anemoi_sm100_dense_shape* s, const void* dout, const void* q, const void* k,
+                                          const void* v, const void* out, const float* lse, const int32_t* q_lengths,
+                                          const int32_t* k_lengths, const int64_t* strides, void* dq, void* dk, void* dv,
+                                          void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
