@@ -544,49 +544,65 @@ struct RowParams {
 
 // delta_i and the log-sum-exp in units of log 2 (+inf where the row has no gradient: its probabilities then come out as
 // zeros).  fp16: the largest |dO_i|^2 and |v_j|^2 of each key head, too (a maximum does not depend on the order of atomics).
+// Rows in memory order (heads of a token, tokens, samples), kRowsEach at once per group of D/8 lanes: that many loads in flight.
+constexpr int kRowsEach = 4;
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowParams p) {
   using T = std::conditional_t<kBf16, __nv_bfloat16, __half>;
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 8, kGroups = 256 / kLanes;
   const bool values = (int)blockIdx.x >= p.q_blocks;
-  const int64_t at = (int64_t)(values ? blockIdx.x - p.q_blocks : blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
-  const int lane = threadIdx.x % kLanes, heads = values ? p.k_heads : p.q_heads, tokens = values ? p.k_tokens : p.q_tokens;
-  const bool in = at < (int64_t)p.batch * heads * tokens;
-  const int64_t token_row = in ? at / heads : 0;  // rows in memory order: heads of a token, tokens, samples
-  const int h = in ? (int)(at - token_row * heads) : 0, b = (int)(token_row / tokens), i = (int)(token_row - (int64_t)b * tokens);
-  const bool live = in && i < length_of(values ? p.k_lengths : p.q_lengths, b, tokens);
-  float d[8] = {}, o[8] = {};
-  if (live) {
-    const Strides& sd = values ? p.sv : p.sd;
-    rows::open8<T>(rows::load_stream(static_cast<const T*>(values ? p.v : p.dout) + b * sd.batch + (int64_t)i * sd.token +
-                                     h * sd.head + lane * 8),
-                   d);
-    if (!values)
-      rows::open8<T>(rows::load_stream(static_cast<const T*>(p.out) + b * p.so.batch + (int64_t)i * p.so.token +
-                                       h * p.so.head + lane * 8),
-                     o);
-  }
-  float dot = 0.0f, norm = 0.0f;
+  const uint32_t heads = values ? p.k_heads : p.q_heads, tokens = values ? p.k_tokens : p.q_tokens;
+  const uint32_t all = p.batch * heads * tokens;  // (below 2^32: the host's limit)
+  const uint32_t first = (uint32_t)(values ? blockIdx.x - p.q_blocks : blockIdx.x) * (kGroups * kRowsEach) + threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const Strides& sd = values ? p.sv : p.sd;
+  const T* d_all = static_cast<const T*>(values ? p.v : p.dout) + lane * 8;
+  const T* o_all = static_cast<const T*>(p.out) + lane * 8;
+  uint4 d_raw[kRowsEach], o_raw[kRowsEach];
+  uint32_t h[kRowsEach], b[kRowsEach], i[kRowsEach];
+  bool in[kRowsEach], live[kRowsEach];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    dot = fmaf(d[j], o[j], dot);
-    norm = fmaf(d[j], d[j], norm);
+  for (int n = 0; n < kRowsEach; ++n) {
+    const uint32_t at = first + n * kGroups;
+    in[n] = at < all;
+    const uint32_t token_row = in[n] ? at / heads : 0u;
+    h[n] = in[n] ? at - token_row * heads : 0u;
+    b[n] = token_row / tokens;
+    i[n] = token_row - b[n] * tokens;
+    live[n] = in[n] && (int)i[n] < length_of(values ? p.k_lengths : p.q_lengths, b[n], tokens);
+    d_raw[n] = o_raw[n] = make_uint4(0, 0, 0, 0);
+    if (live[n]) {
+      d_raw[n] = rows::load_stream(d_all + b[n] * sd.batch + i[n] * sd.token + h[n] * sd.head);
+      if (!values) o_raw[n] = rows::load_stream(o_all + b[n] * p.so.batch + i[n] * p.so.token + h[n] * p.so.head);
+    }
   }
 #pragma unroll
-  for (int off = kLanes / 2; off > 0; off >>= 1) {
-    dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    norm += __shfl_xor_sync(0xffffffffu, norm, off);
+  for (int n = 0; n < kRowsEach; ++n) {
+    float d[8], o[8];
+    rows::open8<T>(d_raw[n], d);
+    rows::open8<T>(o_raw[n], o);
+    float dot = 0.0f, norm = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dot = fmaf(d[j], o[j], dot);
+      norm = fmaf(d[j], d[j], norm);
+    }
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1) {
+      dot += __shfl_xor_sync(0xffffffffu, dot, off);
+      if (!kBf16) norm += __shfl_xor_sync(0xffffffffu, norm, off);
+    }
+    if (!in[n] || lane != 0) continue;
+    if (!values) {
+      const int64_t flat = ((int64_t)b[n] * p.q_heads + h[n]) * p.q_tokens + i[n];
+      const float lse = live[n] ? p.lse[flat] : -INFINITY;
+      p.lse2[flat] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+      p.delta[flat] = live[n] && lse != -INFINITY ? dot : 0.0f;
+    }
+    if (!kBf16 && live[n])
+      atomicMax(p.norms + 2 * (b[n] * p.k_heads + (values ? h[n] : h[n] / (p.q_heads / p.k_heads))) + (values ? 1 : 0),
+                __float_as_uint(norm));
   }
-  if (!in || lane != 0) return;
-  if (!values) {
-    const int64_t flat = ((int64_t)b * p.q_heads + h) * p.q_tokens + i;
-    const float lse = live ? p.lse[flat] : -INFINITY;
-    p.lse2[flat] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-    p.delta[flat] = live && lse != -INFINITY ? dot : 0.0f;
-  }
-  if (p.norms != nullptr && live)
-    atomicMax(p.norms + 2 * (b * p.k_heads + (values ? h : h / (p.q_heads / p.k_heads))) + (values ? 1 : 0),
-              __float_as_uint(norm));
 }
 
 // Powers of two that keep the 16-bit operands P and dS inside fp16's range.  fp16 has no exponents below 2^-14, and over a
@@ -1285,7 +1301,7 @@ int forward_launch(ForwardParams& p, cudaStream_t st) {
 template <int D, bool kBf16>
 int backward_launch(const BackwardParams& p, const RowParams& r, cudaStream_t st) {
   const Geometry& g = p.g;
-  const int64_t per_block = 256 / (D / 8);
+  const int64_t per_block = 256 / (D / 8) * kRowsEach;
   const int64_t q_blocks = ((int64_t)g.batch * g.q_heads * g.q_tokens + per_block - 1) / per_block;
   const int64_t v_blocks = kBf16 ? 0 : ((int64_t)g.batch * g.k_heads * g.k_tokens + per_block - 1) / per_block;
   if (q_blocks + v_blocks > 0x7fffffffLL) return ANEMOI_SM100_ELIMIT;

@@ -55,63 +55,77 @@ struct BackwardParams {
 // Most threads of a block.  Narrow rows: 128.  Wide rows, up to 1,024 pieces of 8 channels: as many threads as the vectors
 // of a thread leave.
 __host__ __device__ constexpr int forward_threads(int vectors, bool wide) { return !wide ? 128 : vectors == 1 ? 1024 : 352; }
-// The gradient holds three column sums per channel: one vector per thread up to 704 pieces (88 registers each), two above.
-constexpr int kOnePiece = 704;
-__host__ __device__ constexpr int backward_threads(int vectors, bool wide) { return !wide ? 128 : vectors == 1 ? kOnePiece : 512; }
+// The gradient holds three column sums per channel in registers, and takes kR rows at a time, so that the chain of a row's
+// sums through the block's barriers is paid once for them.  Wide rows: one piece per thread up to 352 threads, two above; two
+// rows where a thread may have 168 registers (12 warps), one above 352 threads of two pieces.  33,272 rows of 5,376 channels:
+// 672 threads of one piece, one row at a time, spilled at the 80 registers that are left for them, 784 us; 336 threads, one
+// row, copies ahead, 565.
+constexpr int kOnePiece = 352;
+__host__ __device__ constexpr int backward_threads(int rows, bool wide) { return !wide ? 128 : rows == 2 ? kOnePiece : 512; }
 // (and blocks per SM that its registers are to leave room for)
 __host__ __device__ constexpr int backward_blocks(int vectors, bool wide) {
-  return wide ? 1 : vectors == 1 ? 6 : vectors == 2 ? 4 : 2;
+  return wide ? 1 : vectors == 1 ? 5 : vectors == 2 ? 3 : 2;
 }
 
-// Sum over the threads of one row, in each of them.  Narrow rows: kLanes lanes of a warp.  Wide rows: the block; `buffer`
-// alternates between two places, so that one barrier per sum is enough (a thread that writes a place the second time
-// has passed the barrier behind everyone's reads of its first use).
+// Sums of N values over the threads of a row, in each of them.  Narrow rows: `lanes` lanes of a warp.  Wide rows: the block;
+// `buffer` alternates between two places, so that one barrier per sum is enough (a thread that writes a place the second
+// time has passed the barrier behind everyone's reads of its first use).  The lanes of a warp first share the values out, half
+// of them per step, so that N = 4 takes 6 shuffles instead of 20.
+constexpr int kMostWarps = 32, kBuffer = 2 * kMostWarps * 4;
 template <bool kWide>
 struct RowSum {
   float* buffer;
   int lanes;
   int turn = 0;
-  __device__ __forceinline__ float operator()(float v) {
+  template <int N>
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
+    static_assert(N == 1 || N == 2 || N == 4, "shared out by halves");
+    if constexpr (!kWide) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-      if (kWide || off < lanes) v += __shfl_xor_sync(0xffffffffu, v, off);
-    if (kWide) {
-      const int warps = (blockDim.x + 31) >> 5;
-      float* b = buffer + turn * 32;
-      turn ^= 1;
-      if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
-      __syncthreads();
-      v = (threadIdx.x & 31) < warps ? b[threadIdx.x & 31] : 0.0f;
+      for (int off = 16; off > 0; off >>= 1)
+        if (off < lanes)
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    }
-    return v;
-  }
-  // two sums at once
-  __device__ __forceinline__ float2 operator()(float2 v) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-      if (kWide || off < lanes) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
+          for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
+    } else {
+      const int lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
+      float mine = v[0];
+      if constexpr (N == 4) {
+        const bool high = lane & 16;
+        const float a = (high ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, high ? v[0] : v[2], 16);
+        const float b = (high ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, high ? v[1] : v[3], 16);
+        const bool next = lane & 8;
+        mine = (next ? b : a) + __shfl_xor_sync(0xffffffffu, next ? a : b, 8);
+      } else if constexpr (N == 2) {
+        const bool high = lane & 16;
+        mine = (high ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, high ? v[0] : v[1], 16);
       }
-    if (kWide) {
-      const int warps = (blockDim.x + 31) >> 5;
-      float2* b = reinterpret_cast<float2*>(buffer + 64) + turn * 32;
-      turn ^= 1;
-      if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
-      __syncthreads();
-      v = (threadIdx.x & 31) < warps ? b[threadIdx.x & 31] : make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
+      for (int off = N == 4 ? 4 : N == 2 ? 8 : 16; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
+      // value i of the warp is in lanes i * (32 / N) ...
+      float* b = buffer + turn * (kMostWarps * 4);
+      turn ^= 1;
+      if (lane % (32 / N) == 0) b[(threadIdx.x >> 5) * N + lane / (32 / N)] = mine;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 0.0f;
+      for (int w = 0; w < warps; ++w) {
+        if constexpr (N == 4) {
+          const float4 x = reinterpret_cast<const float4*>(b)[w];
+          v[0] += x.x;
+          v[1] += x.y;
+          v[2] += x.z;
+          v[3] += x.w;
+        } else if constexpr (N == 2) {
+          const float2 x = reinterpret_cast<const float2*>(b)[w];
+          v[0] += x.x;
+          v[1] += x.y;
+        } else {
+          v[0] += b[w];
+        }
       }
     }
-    return v;
   }
 };
-constexpr int kBuffer = 64 + 128;
 
 // Normalises v in place; returns the reciprocal root.  Channels that the thread does not have are zeros and stay so.
 template <int V, bool kWide>
@@ -124,7 +138,9 @@ __device__ __forceinline__ float normalise(float (&v)[V][8], const bool (&has)[V
     for (int j = 0; j < V; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += v[j][i];
-    const float mean = sum(s) * inv;
+    float all[1] = {s};
+    sum(all);
+    const float mean = all[0] * inv;
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
@@ -135,7 +151,9 @@ __device__ __forceinline__ float normalise(float (&v)[V][8], const bool (&has)[V
   for (int j = 0; j < V; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) s = fmaf(v[j][i], v[j][i], s);
-  const float r = 1.0f / sqrtf(fmaf(sum(s), inv, eps));
+  float all[1] = {s};
+  sum(all);
+  const float r = rsqrtf(fmaf(all[0], inv, eps));
 #pragma unroll
   for (int j = 0; j < V; ++j)
 #pragma unroll
@@ -146,7 +164,7 @@ __device__ __forceinline__ float normalise(float (&v)[V][8], const bool (&has)[V
 // One row per `lanes` threads.  HBM bound: 2 C bytes of each of x, y in, x', h out.
 template <typename T, typename M, int V, bool kWide>
 __global__ void __launch_bounds__(forward_threads(V, kWide)) forward_kernel(const __grid_constant__ ForwardParams p, int lanes) {
-  __shared__ float buffer[kBuffer];
+  __shared__ __align__(16) float buffer[kBuffer];
   const int lane = kWide ? threadIdx.x : threadIdx.x % lanes;
   const int64_t row_in = kWide ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
   const bool live = row_in < p.rows;
@@ -165,7 +183,7 @@ __global__ void __launch_bounds__(forward_threads(V, kWide)) forward_kernel(cons
       if (p.y != nullptr) yr[j] = load_stream(static_cast<const T*>(p.y) + row * p.y_stride + at[j]);
     }
   }
-  const int64_t group = row / p.per_group;
+  const int64_t group = quotient(row, p.per_group);
   float x[V][8];
 #pragma unroll
   for (int j = 0; j < V; ++j) open8<T>(xr[j], x[j]);
@@ -215,34 +233,78 @@ __global__ void __launch_bounds__(forward_threads(V, kWide)) forward_kernel(cons
   }
 }
 
-// Gradient of N: v = the gradient of the normalised row `hat`, turned into that of the row itself.
-template <int V, bool kWide>
-__device__ __forceinline__ void normalise_gradient(float (&v)[V][8], const float (&hat)[V][8], const bool (&has)[V],
-                                                   float r, int kind, int width, RowSum<kWide>& sum) {
-  float2 s = make_float2(0.0f, 0.0f);
+// What the gradient of N needs of kR rows: v (the rows, minus their means where that is "layer") and g (the gradients of the
+// normalised rows).  One sum over the threads for an RMS norm, as sum v^2 and sum g v go together; two for a layer norm, whose
+// squares need the mean first.  Leaves v normalised; a row's gradient is r * (g - (v * along + mean)).
+struct NormGradient {
+  float r, along, mean;
+};
+template <int V, int kR, bool kWide>
+__device__ __forceinline__ void gradient_of_norm(float (&v)[kR][V][8], const float (&g)[kR][V][8], const bool (&has)[V],
+                                                 int kind, int width, float eps, RowSum<kWide>& sum, NormGradient (&n)[kR]) {
+  const float inv = 1.0f / (float)width;
+  float s[2 * kR];
+  if (kind == kLayer) {
 #pragma unroll
-  for (int j = 0; j < V; ++j)
+    for (int k = 0; k < kR; ++k) {
+      s[2 * k] = s[2 * k + 1] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s.x = fmaf(v[j][i], hat[j][i], s.x);
-      s.y += v[j][i];
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          s[2 * k] += v[k][j][i];
+          s[2 * k + 1] += g[k][j][i];
+        }
     }
-  s = sum(s);
-  const float inv = 1.0f / (float)width, along = s.x * inv, mean = kind == kLayer ? s.y * inv : 0.0f;
+    sum(s);
 #pragma unroll
-  for (int j = 0; j < V; ++j)
+    for (int k = 0; k < kR; ++k) {
+      n[k].mean = s[2 * k + 1] * inv;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[j][i] = has[j] ? r * (v[j][i] - fmaf(hat[j][i], along, mean)) : 0.0f;
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[k][j][i] = has[j] ? v[k][j][i] - s[2 * k] * inv : 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kR; ++k) n[k].mean = 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < kR; ++k) {
+    s[2 * k] = s[2 * k + 1] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        s[2 * k] = fmaf(v[k][j][i], v[k][j][i], s[2 * k]);
+        s[2 * k + 1] = fmaf(g[k][j][i], v[k][j][i], s[2 * k + 1]);
+      }
+  }
+  sum(s);
+#pragma unroll
+  for (int k = 0; k < kR; ++k) {
+    n[k].r = rsqrtf(fmaf(s[2 * k], inv, eps));
+    n[k].along = s[2 * k + 1] * n[k].r * inv;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][j][i] *= n[k].r;
+  }
 }
 
 // A worker (a block, or `lanes` threads of a warp) walks whole segments: consecutive rows of one modulation group, whose
 // column sums it holds in registers: A = sum d * a, S = sum d, B = sum dx * N(y).  scale's gradient is weight * A, weight's
 // sum over the groups of (1 + scale) * A, and so for gate and post_weight with B.  A group of one segment is finished by its
 // worker, other groups and the weights by sums_kernel, in a fixed order.
-template <typename T, typename M, int V, bool kWide>
-__global__ void __launch_bounds__(backward_threads(V, kWide), backward_blocks(V, kWide)) backward_kernel(const __grid_constant__ BackwardParams p, int lanes) {
-  extern __shared__ __align__(16) float weight_sums[];  // per worker [2][V * lanes * 8], where weights are given
-  __shared__ float buffer[kBuffer];
+//
+// HBM bound by its bytes (four arrays in, two out).  The next rows are copied into a ring of shared memory meanwhile (kStages
+// steps of kR rows of each array, a thread's own channels, no registers held): at 5,376 channels two rows, 86 KB per SM, are on
+// their way, where HBM's latency asks for 45.
+template <typename T, typename M, int V, int kR, bool kWide, int kStages>
+__global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V, kWide)) backward_kernel(
+    const __grid_constant__ BackwardParams p, int lanes) {
+  extern __shared__ __align__(16) uint8_t shared[];
+  __shared__ __align__(16) float buffer[kBuffer];
   const int lane = kWide ? threadIdx.x : threadIdx.x % lanes;
   const int slots = kWide ? 1 : blockDim.x / lanes, slot = kWide ? 0 : threadIdx.x / lanes;
   const int worker = blockIdx.x * slots + slot;
@@ -254,121 +316,235 @@ __global__ void __launch_bounds__(backward_threads(V, kWide), backward_blocks(V,
     at[j] = (j * lanes + lane) * 8;
     has[j] = at[j] < p.width;
   }
+  // ring[stage][array][row][piece][thread]
+  enum { kX = 0, kDh = 1, kDx = 2, kY = 3 };
+  uint4* ring = reinterpret_cast<uint4*>(shared) + threadIdx.x;
+  const int threads = blockDim.x, step_of_stage = 4 * kR * V * threads;
+  auto place = [&](int array, int k, int j) { return ((array * kR + k) * V + j) * threads; };
   const bool weights = p.weight_partial != nullptr;
-  float* own = weight_sums + (int64_t)slot * 2 * V * lanes * 8;
+  // per worker [2][V * lanes * 8]
+  float* own = reinterpret_cast<float*>(shared + (size_t)kStages * step_of_stage * 16) + (int64_t)slot * 2 * V * lanes * 8;
   if (weights)
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) own[at[j] + i] = own[V * lanes * 8 + at[j] + i] = 0.0f;
-  // all workers of a block walk the same number of segments (lanes of a warp meet in its shuffles)
-  const int64_t turns = (p.segments + p.workers - 1) / p.workers;
-  for (int64_t turn = 0; turn < turns; ++turn) {
+  // (what no copy writes)
+  const bool given[4] = {true, p.dh != nullptr, p.dx_out != nullptr, p.y != nullptr};
+#pragma unroll
+  for (int s = 0; s < kStages; ++s)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (!given[a] || !has[j])
+#pragma unroll
+          for (int k = 0; k < kR; ++k) ring[s * step_of_stage + place(a, k, j)] = make_uint4(0, 0, 0, 0);
+  // all workers of a block walk the same number of segments (lanes of a warp meet in its shuffles), of as many steps
+  const int64_t turns = quotient(p.segments + p.workers - 1, p.workers);
+  const int64_t longest = quotient(p.per_group + p.per_group_segments - 1, p.per_group_segments);
+  const int steps = (int)((longest + kR - 1) / kR);
+  struct Segment {
+    int64_t group, first;
+    int count;
+  };
+  auto segment_of = [&](int64_t turn) {
     const int64_t segment = turn * p.workers + worker;
-    const bool live = segment < p.segments && worker < p.workers;
-    const int64_t group = live ? segment / p.per_group_segments : 0;
-    const int64_t part = live ? segment - group * p.per_group_segments : 0;
-    const int64_t first = group * p.per_group + p.per_group * part / p.per_group_segments;
-    const int64_t count = live ? group * p.per_group + p.per_group * (part + 1) / p.per_group_segments - first : 0;
-    // (the longest segment: every worker takes as many steps)
-    const int64_t steps = (p.per_group + p.per_group_segments - 1) / p.per_group_segments;
-    float a_sum[V][8] = {}, s_sum[V][8] = {}, b_sum[V][8] = {};
-    uint4 raw[4][V];
-    auto fetch = [&](int64_t step) {
-      const int64_t row = first + step;
-      const bool in = step < count;
+    Segment s{0, 0, 0};
+    if (segment < p.segments && worker < p.workers) {
+      s.group = quotient(segment, p.per_group_segments);
+      const int64_t part = segment - s.group * p.per_group_segments;
+      const int64_t begin = quotient(p.per_group * part, p.per_group_segments);
+      s.first = s.group * p.per_group + begin;
+      s.count = (int)(quotient(p.per_group * (part + 1), p.per_group_segments) - begin);
+    }
+    return s;
+  };
+  // the copies run kStages - 1 steps ahead, into the next segments, too
+  Segment ahead = segment_of(0);
+  int64_t ahead_turn = 0;
+  int ahead_step = 0, ahead_stage = 0;
+  auto copy_next = [&]() {
+#pragma unroll
+    for (int k = 0; k < kR; ++k) {
+      const int n = ahead_step * kR + k;
+      if (ahead_turn >= turns || n >= ahead.count) continue;
+      const int64_t row = ahead.first + n;
+      uint4* to = ring + ahead_stage * step_of_stage;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        raw[0][j] = raw[1][j] = raw[2][j] = raw[3][j] = make_uint4(0, 0, 0, 0);
-        if (!in || !has[j]) continue;
-        raw[0][j] = load_stream(static_cast<const T*>(p.x) + row * p.x_stride + at[j]);
-        if (p.dh != nullptr) raw[1][j] = load_stream(static_cast<const T*>(p.dh) + row * p.dh_stride + at[j]);
-        if (p.dx_out != nullptr) raw[2][j] = load_stream(static_cast<const T*>(p.dx_out) + row * p.dx_out_stride + at[j]);
-        if (p.y != nullptr) raw[3][j] = load_stream(static_cast<const T*>(p.y) + row * p.y_stride + at[j]);
+        if (!has[j]) continue;
+        copy_async16(to + place(kX, k, j), static_cast<const T*>(p.x) + row * p.x_stride + at[j]);
+        if (p.dh != nullptr) copy_async16(to + place(kDh, k, j), static_cast<const T*>(p.dh) + row * p.dh_stride + at[j]);
+        if (p.dx_out != nullptr)
+          copy_async16(to + place(kDx, k, j), static_cast<const T*>(p.dx_out) + row * p.dx_out_stride + at[j]);
+        if (p.y != nullptr) copy_async16(to + place(kY, k, j), static_cast<const T*>(p.y) + row * p.y_stride + at[j]);
       }
-    };
-    fetch(0);
-    for (int64_t step = 0; step < steps; ++step) {
-      const int64_t row = first + step;
-      const bool in = step < count;
-      float dx[V][8], y[V][8];
-      {
-        float x[V][8], d[V][8];
+    }
+    copy_commit();
+    ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
+    if (++ahead_step == steps) {
+      ahead_step = 0;
+      if (++ahead_turn < turns) ahead = segment_of(ahead_turn);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) copy_next();
+  int stage = 0;
+  for (int64_t turn = 0; turn < turns; ++turn) {
+    const Segment seg = segment_of(turn);
+    const int64_t group = seg.group;
+    const M* gates = static_cast<const M*>(p.gate) + group * p.gate_stride;
+    const M* scales = static_cast<const M*>(p.scale) + group * p.scale_stride;
+    float a_sum[V][8] = {}, s_sum[V][8] = {}, b_sum[V][8] = {};
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      // (into the place that was read in the step before, by this thread alone)
+      copy_next();
+      copy_wait<kStages - 1>();
+      const uint4* from = ring + stage * step_of_stage;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      const int rows_in = seg.count - step * kR;  // rows k < rows_in exist
+      auto read = [&](int array, int k, int j, float(&f)[8]) {
+        open8<T>(k < rows_in ? from[place(array, k, j)] : make_uint4(0, 0, 0, 0), f);
+      };
+      float dx[kR][V][8];
+      if (p.dh != nullptr) {
+        float x[kR][V][8], g[kR][V][8];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          open8<T>(raw[0][j], x[j]);
-          open8<T>(raw[1][j], d[j]);
-          open8<T>(raw[2][j], dx[j]);
-          open8<T>(raw[3][j], y[j]);
-        }
-        if (step + 1 < steps) fetch(step + 1);
-        if (p.dh != nullptr) {
-          const float r = normalise<V, kWide>(x, has, p.norm, p.width, p.eps, sum);
+          float f[8];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              a_sum[j][i] = fmaf(d[j][i], x[j][i], a_sum[j][i]);
-              s_sum[j][i] += d[j][i];
-            }
-            if (!has[j]) continue;
-            float f[8];
-            if (p.weight != nullptr) {
-              shared8(static_cast<const T*>(p.weight) + at[j], f);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) d[j][i] *= f[i];
-            }
+          for (int i = 0; i < 8; ++i) f[i] = 1.0f;
+          if (has[j]) {
             if (p.scale != nullptr) {
-              shared8(static_cast<const M*>(p.scale) + group * p.scale_stride + at[j], f);
+              shared8(scales + at[j], f);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) d[j][i] = fmaf(d[j][i], f[i], d[j][i]);
+              for (int i = 0; i < 8; ++i) f[i] += 1.0f;
+            }
+            if (p.weight != nullptr) {
+              float w[8];
+              shared8(static_cast<const T*>(p.weight) + at[j], w);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] *= w[i];
             }
           }
-          normalise_gradient<V, kWide>(d, x, has, r, p.norm, p.width, sum);
 #pragma unroll
-          for (int j = 0; j < V; ++j)
+          for (int k = 0; k < kR; ++k) {
+            read(kX, k, j, x[k][j]);
+            read(kDh, k, j, g[k][j]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dx[j][i] += d[j][i];
+            for (int i = 0; i < 8; ++i) {
+              s_sum[j][i] += g[k][j][i];
+              g[k][j][i] *= f[i];
+            }
+          }
         }
-      }
+        NormGradient n[kR];
+        gradient_of_norm<V, kR, kWide>(x, g, has, p.norm, p.width, p.eps, sum, n);
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (in && has[j]) *reinterpret_cast<uint4*>(static_cast<T*>(p.dx) + row * p.width + at[j]) = round8<T>(dx[j]);
+        for (int k = 0; k < kR; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            float d[8];
+            read(kDh, k, j, d);
+            read(kDx, k, j, dx[k][j]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              a_sum[j][i] = fmaf(d[i], x[k][j][i], a_sum[j][i]);
+              dx[k][j][i] = fmaf(n[k].r, g[k][j][i] - fmaf(x[k][j][i], n[k].along, n[k].mean), dx[k][j][i]);
+            }
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kR; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) read(kDx, k, j, dx[k][j]);
+      }
+      const int64_t row = seg.first + step * kR;
+#pragma unroll
+      for (int k = 0; k < kR; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (k < rows_in && has[j]) {
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.dx) + (row + k) * p.width + at[j]) = round8<T>(dx[k][j]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dx[k][j][i] = 0.0f;
+          }
+        }
       if (p.y == nullptr) continue;
-      float r = 0.0f;
-      if (p.post != kNone) r = normalise<V, kWide>(y, has, p.post, p.width, p.eps, sum);
+      float y[kR][V][8];
+#pragma unroll
+      for (int k = 0; k < kR; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) read(kY, k, j, y[k][j]);
+      if (p.post == kNone) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float f[8] = {};
+          if (has[j]) shared8(gates + at[j], f);
+#pragma unroll
+          for (int k = 0; k < kR; ++k) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              b_sum[j][i] = fmaf(dx[k][j][i], y[k][j][i], b_sum[j][i]);
+              dx[k][j][i] *= f[i];
+            }
+            if (k < rows_in && has[j])
+              *reinterpret_cast<uint4*>(static_cast<T*>(p.dy) + (row + k) * p.width + at[j]) = round8<T>(dx[k][j]);
+          }
+        }
+        continue;
+      }
+      // B takes dx before the gate: its sums over this step are formed with the normalised y, from dx = u / (gate * weight),
+      // which may be a division by zero, so both are kept
+      float u[kR][V][8];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
+        float f[8] = {};
+        if (has[j]) {
+          shared8(gates + at[j], f);
+          if (p.post_weight != nullptr) {
+            float w[8];
+            shared8(static_cast<const T*>(p.post_weight) + at[j], w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) b_sum[j][i] = fmaf(dx[j][i], y[j][i], b_sum[j][i]);
-        if (!has[j]) continue;
-        float f[8];
-        shared8(static_cast<const M*>(p.gate) + group * p.gate_stride + at[j], f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dx[j][i] *= f[i];
-        if (p.post_weight != nullptr) {
-          shared8(static_cast<const T*>(p.post_weight) + at[j], f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dx[j][i] *= f[i];
+            for (int i = 0; i < 8; ++i) f[i] *= w[i];
+          }
         }
-      }
-      if (p.post != kNone) normalise_gradient<V, kWide>(dx, y, has, r, p.post, p.width, sum);
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (in && has[j]) *reinterpret_cast<uint4*>(static_cast<T*>(p.dy) + row * p.width + at[j]) = round8<T>(dx[j]);
+        for (int k = 0; k < kR; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) u[k][j][i] = dx[k][j][i] * f[i];
+      }
+      NormGradient n[kR];
+      gradient_of_norm<V, kR, kWide>(y, u, has, p.post, p.width, p.eps, sum, n);
+#pragma unroll
+      for (int k = 0; k < kR; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            b_sum[j][i] = fmaf(dx[k][j][i], y[k][j][i], b_sum[j][i]);
+            u[k][j][i] = n[k].r * (u[k][j][i] - fmaf(y[k][j][i], n[k].along, n[k].mean));
+          }
+          if (k < rows_in && has[j])
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.dy) + (row + k) * p.width + at[j]) = round8<T>(u[k][j]);
+        }
     }
-    if (!live) continue;
+    if (seg.count == 0) continue;
+    const int64_t segment = turn * p.workers + worker;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       if (!has[j]) continue;
       float f[8];
       if (weights) {
         float* mine = own + at[j];
-        if (p.scale != nullptr) shared8(static_cast<const M*>(p.scale) + group * p.scale_stride + at[j], f);
+        if (p.scale != nullptr) shared8(scales + at[j], f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) mine[i] += p.scale != nullptr ? fmaf(a_sum[j][i], f[i], a_sum[j][i]) : a_sum[j][i];
         if (p.y != nullptr) {
-          shared8(static_cast<const M*>(p.gate) + group * p.gate_stride + at[j], f);
+          shared8(gates + at[j], f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) mine[V * lanes * 8 + i] = fmaf(b_sum[j][i], f[i], mine[V * lanes * 8 + i]);
         }
@@ -400,6 +576,7 @@ __global__ void __launch_bounds__(backward_threads(V, kWide), backward_blocks(V,
       }
     }
   }
+  copy_wait<0>();
   if (weights && worker < p.workers)
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -508,8 +685,10 @@ Split split_of(const RowShape& s, int64_t rows, int64_t groups, int blocks_per_s
   return out;
 }
 
+// Blocks per SM: 12 warps at 168 registers, 16 at 128.
 int backward_blocks_per_sm(const RowShape& s) {
-  return s.wide ? std::max(1, backward_threads(s.vectors, true) / s.threads) : backward_blocks(s.vectors, false);
+  if (!s.wide) return backward_blocks(s.vectors, false);
+  return std::max(1, (s.threads > kOnePiece ? 16 : 12) / ((s.threads + 31) / 32));
 }
 
 template <typename T, typename M, int V, bool kWide>
@@ -521,11 +700,12 @@ int forward_launch(const ForwardParams& p, const RowShape& s, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
 }
 
-template <typename T, typename M, int V, bool kWide>
+template <typename T, typename M, int V, int kR, bool kWide, int kStages>
 int backward_launch(const BackwardParams& p, const RowShape& s, const Split& split, cudaStream_t st) {
   const int slots = s.wide ? 1 : s.threads / s.lanes;
-  const size_t smem = p.weight_partial != nullptr ? (size_t)slots * 2 * V * s.lanes * 8 * sizeof(float) : 0;
-  auto kernel = backward_kernel<T, M, V, kWide>;
+  const size_t smem = (size_t)kStages * 4 * kR * V * s.threads * 16 +
+                      (p.weight_partial != nullptr ? (size_t)slots * 2 * V * s.lanes * 8 * sizeof(float) : 0);
+  auto kernel = backward_kernel<T, M, V, kR, kWide, kStages>;
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return ANEMOI_SM100_ELAUNCH;
@@ -546,12 +726,17 @@ int forward_typed(const ForwardParams& p, const RowShape& s, cudaStream_t st) {
 template <typename T, typename M>
 int backward_typed(const BackwardParams& p, const SumsParams& q, const RowShape& s, const Split& split, cudaStream_t st) {
   int code;
+  // (shared memory: 172 KB of ring at the widest two-row shape, 131 KB at the widest of all, and 8 bytes per channel for the
+  // weights' sums)
   if (!s.wide)
-    code = s.vectors == 1   ? backward_launch<T, M, 1, false>(p, s, split, st)
-           : s.vectors == 2 ? backward_launch<T, M, 2, false>(p, s, split, st)
-                            : backward_launch<T, M, 4, false>(p, s, split, st);
+    code = s.vectors == 1   ? backward_launch<T, M, 1, 1, false, 3>(p, s, split, st)
+           : s.vectors == 2 ? backward_launch<T, M, 2, 1, false, 3>(p, s, split, st)
+                            : backward_launch<T, M, 4, 1, false, 3>(p, s, split, st);
+  else if (s.vectors == 1)
+    code = backward_launch<T, M, 1, 2, true, 2>(p, s, split, st);
   else
-    code = s.vectors == 1 ? backward_launch<T, M, 1, true>(p, s, split, st) : backward_launch<T, M, 2, true>(p, s, split, st);
+    code = s.threads <= kOnePiece ? backward_launch<T, M, 2, 2, true, 2>(p, s, split, st)
+                                  : backward_launch<T, M, 2, 1, true, 2>(p, s, split, st);
   if (code != ANEMOI_SM100_OK) return code;
   const int64_t jobs = (split.per_group_segments > 1 ? 3 * q.groups : 0) + (q.weight_partial != nullptr ? 2 : 0);
   if (jobs == 0) return ANEMOI_SM100_OK;

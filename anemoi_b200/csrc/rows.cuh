@@ -19,6 +19,24 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {
   return v;
 }
 
+// The same into shared memory, without registers: per thread, in groups that complete in order.  (A thread reads back what
+// it copied itself, so that no barrier is needed.)
+__device__ __forceinline__ void copy_async16(void* smem, const void* p) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
+               "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLater>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLater) : "memory");
+}
+
+// a / b without a 64-bit division where both are below 2^32.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 template <typename T>
 struct Pair;
 template <>

@@ -17,6 +17,7 @@ are those of queries that see no key.  ``causal``: query i of a sample sees the 
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 
 import torch
 
@@ -24,16 +25,66 @@ from . import native
 from .executor import _status_word
 
 
-def _tensor(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
-    if not t.is_cuda or t.ndim != 4 or t.dtype not in (torch.float16, torch.bfloat16) or t.shape[-1] not in (64, 128):
+def _layout(t: torch.Tensor):
+    """What of a tensor decides how a call runs."""
+    return t.shape, t.stride(), t.dtype, t.device
+
+
+def _check_layout(layout, name, like=None) -> None:
+    shape, stride, dtype, device = layout
+    if device.type != "cuda" or len(shape) != 4 or dtype not in (torch.float16, torch.bfloat16) or shape[-1] not in (64, 128):
         raise ValueError(f"{name} must be [B, tokens, heads, 64 or 128] in fp16 or bf16, on a CUDA device")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape[0] != like.shape[0]
-                             or t.shape[-1] != like.shape[-1]):
+    if like is not None and (dtype != like[2] or device != like[3] or shape[0] != like[0][0] or shape[-1] != like[0][-1]):
         raise ValueError(f"{name} must have q's dtype, device, batch and head dimension")
-    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16
-                      or any(t.size(i) > 1 and (t.stride(i) <= 0 or t.stride(i) % 8) for i in range(3))):
+    if 0 not in shape and (stride[-1] != 1 or any(shape[i] > 1 and (stride[i] <= 0 or stride[i] % 8) for i in range(3))):
         raise ValueError(f"the heads of {name} must be contiguous and start on 16 bytes")
-    return t
+
+
+class _Plan:
+    """What calls on tensors of the same layout share; found by these layouts."""
+
+    def __init__(self, q, k, v, scale, causal):
+        _check_layout(q, "q")
+        _check_layout(k, "k", q)
+        _check_layout(v, "v", q)
+        (batch, q_tokens, q_heads, dim), dtype = q[0], q[2]
+        if k[0] != v[0]:
+            raise ValueError("k and v must share [B, tokens, heads, D]")
+        _, k_tokens, k_heads, _ = k[0]
+        if k_heads == 0 or q_heads == 0 or q_heads % k_heads:
+            raise ValueError("q's heads must be a multiple of k's")
+        scale = dim ** -0.5 if scale is None else float(scale)
+        if not (scale > 0.0 and math.isfinite(scale)):
+            raise ValueError("scale must be positive")
+        self.empty = 0 in (batch, q_tokens, k_tokens)
+        self.lse_shape = (batch, q_heads, q_tokens)
+        self.strides = (q[1][:3], k[1][:3], v[1][:3])
+        self.shape = native.DenseShape(batch=batch, q_heads=q_heads, k_heads=k_heads, q_tokens=q_tokens, k_tokens=k_tokens,
+                                       head_dim=dim, causal=int(bool(causal)), is_bf16=int(dtype == torch.bfloat16),
+                                       scale=scale)
+        self.forward_bytes, self.backward_bytes = (0, 0) if self.empty else native.dense_attention_bytes(self.shape)
+        packed = ((q_tokens * q_heads * dim, q_heads * dim, dim), (k_tokens * k_heads * dim, k_heads * dim, dim))
+        self.packed = packed
+        self.forward_strides = native.strides_array([n for t in (*self.strides, packed[0]) for n in t])
+
+    @lru_cache(maxsize=16)
+    def backward_strides(self, grad_out, out):
+        """Strides of the backward call, for these layouts of the output's gradient and the output."""
+        q, k = self.packed
+        for name, t in (("grad_out", grad_out), ("out", out)):
+            if t[0] != (self.shape.batch, self.shape.q_tokens, self.shape.q_heads, self.shape.head_dim):
+                raise ValueError(f"{name} must have q's shape")
+            _check_layout(t, name)
+        return native.strides_array([n for t in (grad_out[1][:3], *self.strides, out[1][:3], q, k, k) for n in t])
+
+
+_plan = lru_cache(maxsize=256)(_Plan)
+
+
+def _aligned(**tensors) -> None:
+    for name, t in tensors.items():
+        if t.data_ptr() % 16:
+            raise ValueError(f"the heads of {name} must be contiguous and start on 16 bytes")
 
 
 def _lengths(t: torch.Tensor | None, name: str, q: torch.Tensor) -> torch.Tensor | None:
@@ -44,36 +95,17 @@ def _lengths(t: torch.Tensor | None, name: str, q: torch.Tensor) -> torch.Tensor
     return t.contiguous()
 
 
-def _check(q, k, v, scale, causal, query_lengths, key_lengths):
-    _tensor(q, "q")
-    _tensor(k, "k", q)
-    _tensor(v, "v", q)
-    if k.shape != v.shape:
-        raise ValueError("k and v must share [B, tokens, heads, D]")
-    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError("q's heads must be a multiple of k's")
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError("scale must be positive")
-    shape = native.DenseShape(
-        batch=q.shape[0], q_heads=q.shape[2], k_heads=k.shape[2], q_tokens=q.shape[1], k_tokens=k.shape[1],
-        head_dim=q.shape[3], causal=int(bool(causal)), is_bf16=int(q.dtype == torch.bfloat16), scale=scale)
-    return shape, _lengths(query_lengths, "query_lengths", q), _lengths(key_lengths, "key_lengths", q)
-
-
-def _strides(*tensors):
-    return [s for t in tensors for s in t.stride()[:3]]
-
-
 def _forward(q, k, v, scale, causal, query_lengths, key_lengths):
-    shape, q_lengths, k_lengths = _check(q, k, v, scale, causal, query_lengths, key_lengths)
-    if q.numel() == 0 or k.numel() == 0:
-        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.full((q.shape[0], q.shape[2], q.shape[1]), -math.inf, dtype=torch.float32, device=q.device)
-        return out, lse
+    plan = _plan(_layout(q), _layout(k), _layout(v), scale, causal)
+    q_lengths, k_lengths = _lengths(query_lengths, "query_lengths", q), _lengths(key_lengths, "key_lengths", q)
+    if plan.empty:
+        return (torch.zeros(q.shape, dtype=q.dtype, device=q.device),
+                torch.full(plan.lse_shape, -math.inf, dtype=torch.float32, device=q.device))
+    _aligned(q=q, k=k, v=v)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
-    native.dense_attention(shape, q, k, v, q_lengths, k_lengths, _strides(q, k, v, out), out, lse, _status_word(q.device))
+    lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=q.device)
+    native.dense_attention(plan.shape, q, k, v, q_lengths, k_lengths, plan.forward_strides, out, lse, plan.forward_bytes,
+                           _status_word(q.device))
     return out, lse
 
 
@@ -82,19 +114,19 @@ def dense_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
                              query_lengths: torch.Tensor | None = None, key_lengths: torch.Tensor | None = None):
     """``(dq, dk, dv)`` from the gradient of ``out``; ``out`` and ``lse`` are what ``dense_attention`` gave for the same
     arguments.  Equal calls give equal bits."""
-    shape, q_lengths, k_lengths = _check(q, k, v, scale, causal, query_lengths, key_lengths)
-    for name, t in (("grad_out", grad_out), ("out", out)):
-        if t.shape != q.shape:
-            raise ValueError(f"{name} must have q's shape")
-        _tensor(t, name, q)
-    if (lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32 or lse.device != q.device
-            or not lse.is_contiguous()):
+    plan = _plan(_layout(q), _layout(k), _layout(v), scale, causal)
+    q_lengths, k_lengths = _lengths(query_lengths, "query_lengths", q), _lengths(key_lengths, "key_lengths", q)
+    if out.dtype != q.dtype or grad_out.dtype != q.dtype or out.device != q.device or grad_out.device != q.device:
+        raise ValueError("grad_out and out must have q's dtype and device")
+    strides = plan.backward_strides(_layout(grad_out), _layout(out))
+    if (lse.shape != plan.lse_shape or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous fp32 [B, heads, queries] on q's device")
-    make = torch.zeros if q.numel() == 0 or k.numel() == 0 else torch.empty
-    dq, dk, dv = (make(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    if make is torch.empty:
-        native.dense_attention_backward(shape, grad_out, q, k, v, out, lse, q_lengths, k_lengths,
-                                        _strides(grad_out, q, k, v, out, dq, dk, dv), dq, dk, dv, _status_word(q.device))
+    if plan.empty:
+        return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    _aligned(grad_out=grad_out, q=q, k=k, v=v, out=out)
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    native.dense_attention_backward(plan.shape, grad_out, q, k, v, out, lse, q_lengths, k_lengths, strides, dq, dk, dv,
+                                    plan.backward_bytes, _status_word(q.device))
     return dq, dk, dv
 
 
@@ -124,7 +156,10 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
                     return_lse: bool = False):
     """``out`` ``[B, Sq, Hq, D]`` (with ``return_lse`` also the rows' log-sum-exps ``[B, Hq, Sq]``, fp32, without a gradient
     of their own).  ``scale``: D ** -0.5 by default."""
-    out, lse = _DenseAttention.apply(q, k, v, query_lengths, key_lengths, scale, causal)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _DenseAttention.apply(q, k, v, query_lengths, key_lengths, scale, causal)
+    else:
+        out, lse = _forward(q, k, v, scale, causal, query_lengths, key_lengths)
     return (out, lse) if return_lse else out
 
 

@@ -17,6 +17,7 @@ frame; F = tokens: one per token).  Weights: ``[C]`` in the rows' type.
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -38,63 +39,83 @@ class GateNormGradients(NamedTuple):
     post_weight: torch.Tensor | None
 
 
-def _rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
-    """``t`` as rows ``[R, C]`` that the kernel can read, without a copy."""
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+def _layout(t: torch.Tensor | None):
+    """What of a tensor decides how a call runs."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _row_stride(layout, name: str, like=None) -> int:
+    """The distance of two rows of ``[..., C]``, all rows being that far apart."""
+    shape, stride, dtype, device = layout
+    if like is not None and (shape != like[0] or dtype != like[2] or device != like[3]):
         raise ValueError(f"{name} must have the shape, dtype and device of x")
-    if t.ndim < 1 or t.dtype not in (torch.float16, torch.bfloat16):
+    if len(shape) < 1 or dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"{name} must be [..., C] in fp16 or bf16")
-    width = t.shape[-1]
+    if device.type != "cuda":
+        raise ValueError(f"{name} must be on a CUDA device")
+    width = shape[-1]
     if width == 0 or width % 8 or width > 8192:
         raise ValueError(f"the channels of {name} must be a multiple of 8, at most 8192, got {width}")
-    if t.stride(-1) != 1:
+    if 0 in shape:
+        return width
+    if stride[-1] != 1:
         raise ValueError(f"{name} must be contiguous in its channels")
-    if t.numel() == 0:
-        return t.reshape(-1, width)
-    try:
-        flat = t.view(-1, width)
-    except RuntimeError:
-        raise ValueError(f"the rows of {name} must be one stride apart") from None
-    if flat.stride(0) % 8 or flat.data_ptr() % 16:
+    step, rows = None, 1
+    for size, n in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if size == 1:
+            continue
+        if step is None:
+            step = n
+        elif n != step * rows:
+            raise ValueError(f"the rows of {name} must be one stride apart")
+        rows *= size
+    step = width if step is None else step
+    if step < 0 or step % 8:
         raise ValueError(f"the rows of {name} must start on 16 bytes")
-    return flat
+    return step
 
 
-def _modulation(t: torch.Tensor, name: str, x: torch.Tensor) -> torch.Tensor:
-    """``t`` as ``[G, C]``, G dividing the rows of ``x``: consecutive rows share one."""
-    if t.dtype not in (x.dtype, torch.float32) or t.device != x.device or t.ndim < 1 or t.shape[-1] != x.shape[-1]:
+def _modulation_rows(layout, name: str, x) -> int:
+    """How many rows the modulation has: consecutive tokens share one."""
+    shape, _, dtype, device = layout
+    lead = x[0][:-1]
+    if dtype not in (x[2], torch.float32) or device != x[3] or len(shape) < 1 or shape[-1] != x[0][-1]:
         raise ValueError(f"{name} must be [..., C] on x's device, in x's dtype or fp32")
-    lead = x.shape[:-1]
-    if t.ndim == 1:
+    if len(shape) == 1:
         fits = True
-    elif t.ndim == x.ndim - 1:
-        fits = t.shape[:-1] == lead[:-1]
-    elif t.ndim == x.ndim:
-        # the token dimension may be cut into frames
-        fits = t.shape[:-2] == lead[:-1] and t.shape[-2] > 0 and lead[-1] % t.shape[-2] == 0
+    elif len(shape) == len(lead):
+        fits = shape[:-1] == lead[:-1]
     else:
-        fits = False
+        # the token dimension may be cut into frames
+        fits = (len(shape) == len(lead) + 1 and shape[:-2] == lead[:-1] and shape[-2] > 0 and lead[-1] % shape[-2] == 0)
     if not fits:
         raise ValueError(f"{name} must be [C], x's shape without its tokens, or x's shape with its tokens cut into frames; "
-                         f"got {tuple(t.shape)} for x {tuple(x.shape)}")
-    step = 16 // t.element_size()
-    flat = t.reshape(-1, t.shape[-1]) if t.numel() else t.new_zeros((1, x.shape[-1]))
-    if flat.stride(-1) != 1 or flat.stride(0) % step or flat.data_ptr() % 16:
-        flat = flat.contiguous() if flat.stride(-1) != 1 or flat.stride(0) % step else flat.clone()
-    return flat
+                         f"got {tuple(shape)} for x {tuple(x[0])}")
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    return rows
 
 
-def _weight(t: torch.Tensor | None, name: str, x: torch.Tensor) -> torch.Tensor | None:
-    if t is None:
+def _modulation_stride(layout) -> int | None:
+    """The distance of two modulation rows; None where the kernel cannot read them as they lie."""
+    shape, stride, dtype, _ = layout
+    if 0 in shape or stride[-1] != 1:
         return None
-    if t.shape != x.shape[-1:] or t.dtype != x.dtype or t.device != x.device:
-        raise ValueError(f"{name} must be [C] of x's dtype, on its device")
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
+    step, rows = 0, 1
+    for size, n in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if size == 1:
+            continue
+        if rows == 1:
+            step = n
+        elif n != step * rows:
+            return None
+        rows *= size
+    return None if step < 0 or step % (16 // dtype.itemsize) else step
 
 
-class _Call:
-    """One call's arguments, checked and laid out as the kernels read them."""
+class _Plan:
+    """What calls on tensors of the same layout share; found by these layouts."""
 
     def __init__(self, x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm):
         if norm not in ("rms", "layer") or post_norm not in _NORMS:
@@ -107,88 +128,132 @@ class _Call:
             raise ValueError("post_norm normalises y")
         if post_weight is not None and post_norm is None:
             raise ValueError("post_weight weighs the norm of y: it needs post_norm")
-        if not x.is_cuda:
-            raise ValueError("x must be on a CUDA device")
-        self.x = _rows(x, "x")
-        self.y = None if y is None else _rows(y, "y", x)
-        mods = {name: _modulation(t, name, x)
-                for name, t in (("gate", gate), ("scale", scale), ("shift", shift)) if t is not None}
-        if len({t.dtype for t in mods.values()}) > 1:
+        self.x_stride = _row_stride(x, "x")
+        self.y_stride = 0 if y is None else _row_stride(y, "y", x)
+        mods = {name: t for name, t in (("gate", gate), ("scale", scale), ("shift", shift)) if t is not None}
+        if len({t[2] for t in mods.values()}) > 1:
             raise ValueError("gate, scale and shift must have one dtype")
-        groups = max((t.size(0) for t in mods.values()), default=1)
-        for name, t in mods.items():
-            if t.size(0) not in (1, groups):
-                raise ValueError("gate, scale and shift must be given for the same tokens")
-        self.mods = mods
-        self.groups = groups
-        # one row for all groups: a stride of zero
-        self.strides = {name: 0 if t.size(0) < groups else t.stride(0) for name, t in mods.items()}
-        self.weight = _weight(weight, "weight", x)
-        self.post_weight = _weight(post_weight, "post_weight", x)
-        self.native = native.Rows(
-            rows=self.x.size(0), groups=groups, width=x.shape[-1], norm=_NORMS[norm], post=_NORMS[post_norm],
-            is_bf16=int(x.dtype == torch.bfloat16),
-            mod_is_fp32=int(any(t.dtype == torch.float32 for t in mods.values())), eps=float(eps))
+        rows = {name: _modulation_rows(t, name, x) for name, t in mods.items()}
+        self.groups = max(rows.values(), default=1)
+        if any(n not in (1, self.groups) for n in rows.values()):
+            raise ValueError("gate, scale and shift must be given for the same tokens")
+        for name, w in (("weight", weight), ("post_weight", post_weight)):
+            if w is not None and (w[0] != x[0][-1:] or w[2] != x[2] or w[3] != x[3]):
+                raise ValueError(f"{name} must be [C] of x's dtype, on its device")
+        self.width = x[0][-1]
+        self.rows = 0 if 0 in x[0] else 1
+        for n in x[0][:-1]:
+            self.rows *= n
+        # one modulation row for all groups: a stride of zero; None: a packed copy is read
+        self.mod_strides = {}
+        self.packs = set()
+        for name in ("gate", "scale", "shift"):
+            step = 0
+            if name in mods:
+                step = _modulation_stride(mods[name])
+                if step is None:
+                    self.packs.add(name)
+                    step = self.width
+                if rows[name] < self.groups:
+                    step = 0
+            self.mod_strides[name] = step
+        self.mod_rows = rows
+        self.mod_dtype = next((t[2] for t in mods.values()), x[2])
+        self.native = native.Rows(rows=self.rows, groups=self.groups, width=self.width, norm=_NORMS[norm],
+                                  post=_NORMS[post_norm], is_bf16=int(x[2] == torch.bfloat16),
+                                  mod_is_fp32=int(self.mod_dtype == torch.float32), eps=float(eps))
+        m = self.mod_strides
+        self.forward_strides = native.strides_array((self.x_stride, self.y_stride, m["gate"], m["scale"], m["shift"]))
+        self.x_layout = x
 
-    def row_stride(self, t):
-        return 0 if t is None else t.stride(0)
+    @lru_cache(maxsize=16)
+    def backward_strides(self, dx_out, dh):
+        steps = [0 if t is None else _row_stride(t, name, self.x_layout) for name, t in (("dx_out", dx_out), ("dh", dh))]
+        return native.strides_array((*steps, self.x_stride, self.y_stride, self.mod_strides["gate"],
+                                     self.mod_strides["scale"]))
+
+    @lru_cache(maxsize=2)
+    def backward_bytes(self, weights):
+        return native.gate_norm_modulate_backward_bytes(self.native, weights)
+
+
+_plan = lru_cache(maxsize=256)(_Plan)
+
+
+def _packed16(t: torch.Tensor | None) -> torch.Tensor | None:
+    """A small tensor as the kernels read it: contiguous, on 16 bytes."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _modulation(plan: _Plan, name: str, t: torch.Tensor | None) -> torch.Tensor | None:
+    """As the plan's strides read it.  (A copy of an unaligned view keeps its strides' meaning only where it is one row, or
+    packed: the rest is packed first.)"""
+    if t is None:
+        return None
+    if name in plan.packs:
+        return t.contiguous() if t.numel() else None
+    if t.data_ptr() % 16 == 0:
+        return t
+    if plan.mod_strides[name] in (0, plan.width):
+        return t.clone(memory_format=torch.contiguous_format)
+    raise ValueError(f"the rows of {name} must start on 16 bytes")
+
+
+def _aligned(**tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.data_ptr() % 16:
+            raise ValueError(f"the rows of {name} must start on 16 bytes")
 
 
 def _forward(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, with_norm=True):
-    c = _Call(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm)
+    plan = _plan(_layout(x), _layout(y), _layout(gate), _layout(scale), _layout(shift), _layout(weight),
+                 _layout(post_weight), eps, norm, post_norm)
     x_out = None if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_norm else None
-    if x.numel():
+    if plan.rows:
+        _aligned(x=x, y=y)
         native.gate_norm_modulate(
-            c.native, c.x, c.y, c.mods.get("gate"), c.mods.get("scale"), c.mods.get("shift"), c.weight, c.post_weight,
-            (c.row_stride(c.x), c.row_stride(c.y), *(c.strides.get(k, 0) for k in ("gate", "scale", "shift"))), x_out, h)
+            plan.native, x, y, _modulation(plan, "gate", gate), _modulation(plan, "scale", scale),
+            _modulation(plan, "shift", shift), _packed16(weight), _packed16(post_weight), plan.forward_strides, x_out, h)
     return x_out, h
 
 
-def _like_modulation(t: torch.Tensor, sums: torch.Tensor, groups: int) -> torch.Tensor:
-    """Sums of ``groups`` groups in the shape of the argument (which may have been one row for all of them)."""
-    if t.numel() // t.shape[-1] == groups:
-        return sums.view(t.shape)
-    return sums.float().sum(0).to(t.dtype).view(t.shape)
-
-
-def _backward(dx_out, dh, x_out, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm) -> GateNormGradients:
-    c = _Call(x_out, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm)
+def _backward(dx_out, dh, x_out, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm,
+              wanted=(True,) * 7) -> GateNormGradients:
+    plan = _plan(_layout(x_out), _layout(y), _layout(gate), _layout(scale), _layout(shift), _layout(weight),
+                 _layout(post_weight), eps, norm, post_norm)
     if dx_out is None and dh is None:
         raise ValueError("one of the outputs' gradients is needed")
-    given = [None if t is None else _rows(t, name, x_out) for name, t in (("dx_out", dx_out), ("dh", dh))]
+    strides = plan.backward_strides(_layout(dx_out), _layout(dh))
     dx = torch.empty(x_out.shape, dtype=x_out.dtype, device=x_out.device)
-    dy = None if y is None else torch.empty_like(dx)
-    rows = x_out.numel() // x_out.shape[-1] if x_out.numel() else 0
-    make = torch.empty if rows else torch.zeros
+    dy = None if y is None else torch.empty(x_out.shape, dtype=x_out.dtype, device=x_out.device)
+    make = torch.empty if plan.rows else torch.zeros
+    normed = dh is not None
 
-    def sums(name, wanted=True):
-        if name not in c.mods or not wanted:
+    def sums(t, name, want):
+        if t is None or not want:
             return None
-        return make((c.groups, x_out.shape[-1]), dtype=c.mods[name].dtype, device=x_out.device)
+        # the argument's own shape, unless one row of it served several groups
+        shape = t.shape if plan.mod_rows[name] == plan.groups else (plan.groups, plan.width)
+        return make(shape, dtype=t.dtype, device=t.device)
 
-    def weight_sums(t, wanted=True):
-        return None if t is None or not wanted else make(t.shape, dtype=t.dtype, device=t.device)
-
-    norm_wanted = dh is not None
-    dgate, dscale, dshift = sums("gate"), sums("scale", norm_wanted), sums("shift", norm_wanted)
-    dweight, dpost = weight_sums(c.weight, norm_wanted), weight_sums(c.post_weight)
-    if rows:
+    dgate, dscale, dshift = (sums(gate, "gate", wanted[2]), sums(scale, "scale", wanted[3] and normed),
+                             sums(shift, "shift", wanted[4] and normed))
+    dweight, dpost = (make(t.shape, dtype=t.dtype, device=t.device) if t is not None and want else None
+                      for t, want in ((weight, wanted[5] and normed), (post_weight, wanted[6])))
+    if plan.rows:
+        _aligned(dx_out=dx_out, dh=dh, x_out=x_out, y=y)
         native.gate_norm_modulate_backward(
-            c.native, *given, c.x, c.y, c.mods.get("gate"), c.mods.get("scale"), c.weight, c.post_weight,
-            (c.row_stride(given[0]), c.row_stride(given[1]), c.row_stride(c.x), c.row_stride(c.y),
-             c.strides.get("gate", 0), c.strides.get("scale", 0)), dx, dy, dgate, dscale, dshift, dweight, dpost)
-    like = {name: t for name, t in (("gate", gate), ("scale", scale), ("shift", shift)) if t is not None}
-    shaped = {name: None if s is None else _like_modulation(like[name], s, c.groups)
-              for name, s in (("gate", dgate), ("scale", dscale), ("shift", dshift))}
-    return GateNormGradients(dx, dy, shaped["gate"], shaped["scale"], shaped["shift"], dweight, dpost)
+            plan.native, dx_out, dh, x_out, y, _modulation(plan, "gate", gate), _modulation(plan, "scale", scale),
+            _packed16(weight), _packed16(post_weight), strides, dx, dy, dgate, dscale, dshift, dweight, dpost,
+            plan.backward_bytes(dweight is not None or dpost is not None))
 
+    def whole(s, t):
+        return s if s is None or s.shape == t.shape else s.float().sum(0).to(t.dtype).view(t.shape)
 
-def _readable(t: torch.Tensor | None) -> torch.Tensor | None:
-    """A gradient as autograd hands it over (expanded, transposed, ...) in a form that the kernels read."""
-    if t is None or t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    return GateNormGradients(dx, dy, whole(dgate, gate), whole(dscale, scale), whole(dshift, shift), dweight, dpost)
 
 
 class _GateNorm(torch.autograd.Function):
@@ -205,11 +270,21 @@ class _GateNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         given = iter(grads)
-        dx_out, dh = (_readable(next(given)) if there else None for there in ctx.outputs)
+        # (autograd hands gradients over in any layout: expanded, transposed)
+        dx_out, dh = (_packed16(next(given)) if there else None for there in ctx.outputs)
         if dx_out is None and dh is None:
             return (None,) * 11
-        out = _backward(dx_out, dh, *ctx.saved_tensors, *ctx.options)
+        out = _backward(dx_out, dh, *ctx.saved_tensors, *ctx.options, wanted=ctx.needs_input_grad[:7])
         return (*(g if need else None for g, need in zip(out, ctx.needs_input_grad)), None, None, None, None)
+
+
+def _call(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, with_norm):
+    """The outputs that there are, recorded by autograd where an argument asks for it."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, y, gate, scale, shift, weight, post_weight)):
+        return _GateNorm.apply(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, with_norm)
+    x_out, h = _forward(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, with_norm)
+    return (h,) if x_out is None else (x_out,) if h is None else (x_out, h)
 
 
 def fused_gate_norm_modulate(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor, scale: torch.Tensor | None = None,
@@ -219,19 +294,19 @@ def fused_gate_norm_modulate(x: torch.Tensor, y: torch.Tensor, gate: torch.Tenso
     """``(x_out, h)``: the residual stream behind a block and the modulated input of the next one.
 
     ``h`` is the norm of the unrounded sum.  ``post_norm`` normalises ``y`` before the gate, ``post_weight`` then weighs it."""
-    return _GateNorm.apply(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, True)
+    return _call(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, True)
 
 
 def fused_norm_modulate(x: torch.Tensor, scale: torch.Tensor | None = None, shift: torch.Tensor | None = None,
                         weight: torch.Tensor | None = None, *, eps: float = 1e-6, norm: str = "rms") -> torch.Tensor:
     """``norm(x) * weight * (1 + scale) + shift``: the input of a stack's first block."""
-    return _GateNorm.apply(x, None, None, scale, shift, weight, None, eps, norm, None, True)[0]
+    return _call(x, None, None, scale, shift, weight, None, eps, norm, None, True)[0]
 
 
 def fused_gate_residual(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor, post_weight: torch.Tensor | None = None, *,
                         eps: float = 1e-6, post_norm: str | None = None) -> torch.Tensor:
     """``x + gate * post(y)``: the residual stream behind a stack's last block."""
-    return _GateNorm.apply(x, y, gate, None, None, None, post_weight, eps, "rms", post_norm, False)[0]
+    return _call(x, y, gate, None, None, None, post_weight, eps, "rms", post_norm, False)[0]
 
 
 def fused_gate_norm_modulate_backward(dx_out: torch.Tensor | None, dh: torch.Tensor | None, x_out: torch.Tensor,

@@ -773,81 +773,112 @@ def _at(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(nbytes: int, device) -> torch.Tensor | None:
-    """Scratch of one call, from torch's allocator (which keeps it for the stream of the call)."""
+class _OnDevice:
+    """The device of a call is the current one inside, and the one before it again behind."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+        return False
+
+
+def workspace_bytes(nbytes: int) -> int:
+    """A workspace query's answer; its negative ones are errors."""
     if nbytes < 0:
         raise RuntimeError(f"workspace query failed: {ERRORS.get(nbytes, nbytes)}")
+    return int(nbytes)
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor | None:
+    """Scratch of one call, from torch's allocator (which keeps it for the stream of the call)."""
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def strides_array(strides):
+    return (C.c_int64 * len(strides))(*strides)
+
+
+# The functions below take shapes and strides as ctypes objects, which their callers keep with the configuration: building
+# them costs more than the call.
 def gate_norm_modulate(rows: Rows, x, y, gate, scale, shift, weight, post_weight, strides, x_out, h_out) -> None:
-    with torch.cuda.device(x.device):
-        _count("gate_norm_modulate", 1 if rows.rows else 0)
+    with _OnDevice(x.device) as stream:
+        _count("gate_norm_modulate", 1)
         _check(library().anemoi_sm100_gate_norm_modulate(
-            C.byref(rows), _at(x), _at(y), _at(gate), _at(scale), _at(shift), _at(weight), _at(post_weight),
-            (C.c_int64 * 5)(*strides), _at(x_out), _at(h_out), torch.cuda.current_stream().cuda_stream),
-            "anemoi_sm100_gate_norm_modulate")
+            rows, _at(x), _at(y), _at(gate), _at(scale), _at(shift), _at(weight), _at(post_weight), strides, _at(x_out),
+            _at(h_out), stream), "anemoi_sm100_gate_norm_modulate")
+
+
+def gate_norm_modulate_backward_bytes(rows: Rows, weights: bool) -> int:
+    return workspace_bytes(library().anemoi_sm100_gate_norm_modulate_backward_workspace(rows, int(weights)))
 
 
 def gate_norm_modulate_backward(rows: Rows, dx_out, dh, x, y, gate, scale, weight, post_weight, strides, dx, dy, dgate,
-                                dscale, dshift, dweight, dpost_weight) -> None:
-    lib = library()
-    with torch.cuda.device(x.device):
-        nbytes = int(lib.anemoi_sm100_gate_norm_modulate_backward_workspace(
-            C.byref(rows), int(dweight is not None or dpost_weight is not None)))
+                                dscale, dshift, dweight, dpost_weight, nbytes: int) -> None:
+    with _OnDevice(x.device) as stream:
         space = _workspace(nbytes, x.device)
         _count("gate_norm_modulate_backward", 2 if nbytes else 1)
-        _check(lib.anemoi_sm100_gate_norm_modulate_backward(
-            C.byref(rows), _at(dx_out), _at(dh), _at(x), _at(y), _at(gate), _at(scale), _at(weight), _at(post_weight),
-            (C.c_int64 * 6)(*strides), _at(dx), _at(dy), _at(dgate), _at(dscale), _at(dshift), _at(dweight),
-            _at(dpost_weight), _at(space), nbytes, torch.cuda.current_stream().cuda_stream),
-            "anemoi_sm100_gate_norm_modulate_backward")
+        _check(library().anemoi_sm100_gate_norm_modulate_backward(
+            rows, _at(dx_out), _at(dh), _at(x), _at(y), _at(gate), _at(scale), _at(weight), _at(post_weight), strides,
+            _at(dx), _at(dy), _at(dgate), _at(dscale), _at(dshift), _at(dweight), _at(dpost_weight), _at(space), nbytes,
+            stream), "anemoi_sm100_gate_norm_modulate_backward")
 
 
 def axial_rope(shape: AxialRopeShape, q, k, q_weight, k_weight, positions, position_batch: int, turns, strides, q_out,
                k_out) -> None:
-    with torch.cuda.device(q.device):
+    with _OnDevice(q.device) as stream:
         _count("axial_rope", 1)
         _check(library().anemoi_sm100_axial_rope(
-            C.byref(shape), _at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions), position_batch, turns,
-            (C.c_int64 * 12)(*strides), _at(q_out), _at(k_out), torch.cuda.current_stream().cuda_stream),
-            "anemoi_sm100_axial_rope")
+            shape, _at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions), position_batch, turns, strides, _at(q_out),
+            _at(k_out), stream), "anemoi_sm100_axial_rope")
+
+
+def axial_rope_backward_bytes(shape: AxialRopeShape) -> int:
+    return workspace_bytes(library().anemoi_sm100_axial_rope_backward_workspace(shape))
 
 
 def axial_rope_backward(shape: AxialRopeShape, dq_out, dk_out, q, k, q_weight, k_weight, positions, position_batch: int,
-                        turns, strides, dq, dk, dq_weight, dk_weight) -> None:
-    lib = library()
-    weights = dq_weight is not None or dk_weight is not None
-    with torch.cuda.device(dq_out.device):
-        nbytes = int(lib.anemoi_sm100_axial_rope_backward_workspace(C.byref(shape))) if weights else 0
+                        turns, strides, dq, dk, dq_weight, dk_weight, nbytes: int) -> None:
+    with _OnDevice(dq_out.device) as stream:
         space = _workspace(nbytes, dq_out.device)
-        _count("axial_rope_backward", 2 if weights else 1)
-        _check(lib.anemoi_sm100_axial_rope_backward(
-            C.byref(shape), _at(dq_out), _at(dk_out), _at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions),
-            position_batch, turns, (C.c_int64 * 18)(*strides), _at(dq), _at(dk), _at(dq_weight), _at(dk_weight),
-            _at(space), nbytes, torch.cuda.current_stream().cuda_stream), "anemoi_sm100_axial_rope_backward")
+        _count("axial_rope_backward", 2 if nbytes else 1)
+        _check(library().anemoi_sm100_axial_rope_backward(
+            shape, _at(dq_out), _at(dk_out), _at(q), _at(k), _at(q_weight), _at(k_weight), _at(positions), position_batch,
+            turns, strides, _at(dq), _at(dk), _at(dq_weight), _at(dk_weight), _at(space), nbytes, stream),
+            "anemoi_sm100_axial_rope_backward")
 
 
-def dense_attention(shape: DenseShape, q, k, v, q_lengths, k_lengths, strides, out, lse, status) -> None:
+def dense_attention_bytes(shape: DenseShape) -> tuple[int, int]:
+    """Workspace of the forward and of the backward pass."""
     lib = library()
-    with torch.cuda.device(q.device):
-        nbytes = int(lib.anemoi_sm100_dense_attention_workspace(C.byref(shape)))
+    return (workspace_bytes(lib.anemoi_sm100_dense_attention_workspace(shape)),
+            workspace_bytes(lib.anemoi_sm100_dense_attention_backward_workspace(shape)))
+
+
+def dense_attention(shape: DenseShape, q, k, v, q_lengths, k_lengths, strides, out, lse, nbytes: int, status) -> None:
+    with _OnDevice(q.device) as stream:
         space = _workspace(nbytes, q.device)
         _count("dense_attention", 2 if nbytes else 1)
-        _check(lib.anemoi_sm100_dense_attention(
-            C.byref(shape), _at(q), _at(k), _at(v), _at(q_lengths), _at(k_lengths), (C.c_int64 * 12)(*strides), _at(out),
-            _at(lse), _at(space), nbytes, _at(status), torch.cuda.current_stream().cuda_stream),
-            "anemoi_sm100_dense_attention")
+        _check(library().anemoi_sm100_dense_attention(
+            shape, _at(q), _at(k), _at(v), _at(q_lengths), _at(k_lengths), strides, _at(out), _at(lse), _at(space), nbytes,
+            _at(status), stream), "anemoi_sm100_dense_attention")
 
 
 def dense_attention_backward(shape: DenseShape, dout, q, k, v, out, lse, q_lengths, k_lengths, strides, dq, dk, dv,
-                             status) -> None:
-    lib = library()
-    with torch.cuda.device(q.device):
-        nbytes = int(lib.anemoi_sm100_dense_attention_backward_workspace(C.byref(shape)))
+                             nbytes: int, status) -> None:
+    with _OnDevice(q.device) as stream:
         space = _workspace(nbytes, q.device)
         _count("dense_attention_backward", 2)
-        _check(lib.anemoi_sm100_dense_attention_backward(
-            C.byref(shape), _at(dout), _at(q), _at(k), _at(v), _at(out), _at(lse), _at(q_lengths), _at(k_lengths),
-            (C.c_int64 * 24)(*strides), _at(dq), _at(dk), _at(dv), _at(space), nbytes, _at(status),
-            torch.cuda.current_stream().cuda_stream), "anemoi_sm100_dense_attention_backward")
+        _check(library().anemoi_sm100_dense_attention_backward(
+            shape, _at(dout), _at(q), _at(k), _at(v), _at(out), _at(lse), _at(q_lengths), _at(k_lengths), strides, _at(dq),
+            _at(dk), _at(dv), _at(space), nbytes, _at(status), stream), "anemoi_sm100_dense_attention_backward")

@@ -17,7 +17,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 from dataclasses import dataclass
-from functools import cached_property
+from functools import cached_property, lru_cache
 
 import torch
 
@@ -90,91 +90,116 @@ class AxialRotary:
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
-def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
-    if t.ndim != 4 or t.dtype not in (torch.float16, torch.bfloat16) or t.shape[-1] not in (64, 128):
+def _layout(t: torch.Tensor | None):
+    """What of a tensor decides how a call runs."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _check_heads(layout, name: str, like=None) -> None:
+    shape, stride, dtype, device = layout
+    if len(shape) != 4 or dtype not in (torch.float16, torch.bfloat16) or shape[-1] not in (64, 128):
         raise ValueError(f"{name} must be (B, seq, heads, 64 or 128) in fp16 or bf16")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape[:2] != like.shape[:2]
-                             or t.shape[-1] != like.shape[-1]):
+    if device.type != "cuda":
+        raise ValueError(f"{name} must be on a CUDA device")
+    if like is not None and (dtype != like[2] or device != like[3] or shape[:2] != like[0][:2] or shape[-1] != like[0][-1]):
         raise ValueError(f"{name} must have q's dtype, device, batch, sequence and head dimension")
-    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16
-                      or any(t.stride(i) % 8 for i in range(3) if t.size(i) > 1)):
+    if 0 not in shape and (stride[-1] != 1 or any(shape[i] > 1 and stride[i] % 8 for i in range(3))):
         raise ValueError(f"the heads of {name} must be contiguous and start on 16 bytes")
-    return t
 
 
-def _head_strides(t: torch.Tensor | None):
-    return (0, 0, 0) if t is None else tuple(t.stride(i) if t.size(i) > 1 else 0 for i in range(3))
+def _head_strides(layout):
+    return (0, 0, 0) if layout is None else tuple(n if size > 1 else 0 for n, size in zip(layout[1][:3], layout[0][:3]))
 
 
-class _AxialCall:
-    """One call's arguments, checked and laid out as the kernels read them."""
+class _AxialPlan:
+    """What calls on tensors of the same layout share; found by these layouts."""
 
     def __init__(self, q, k, q_weight, k_weight, positions, rotary, eps):
         if not isinstance(rotary, AxialRotary):
             raise TypeError("rotary must be an AxialRotary")
-        _heads(q, "q")
+        _check_heads(q, "q")
         if k is not None:
-            _heads(k, "k", q)
-        if not q.is_cuda:
-            raise ValueError("q must be on a CUDA device")
-        dim = q.shape[-1]
+            _check_heads(k, "k", q)
+        (batch, tokens, q_heads, dim), dtype, device = q[0], q[2], q[3]
         if 2 * rotary.pairs > dim:
             raise ValueError(f"{rotary.pairs} pairs of channels do not fit a head of {dim}")
-        if k is not None and (q_weight is None) != (k_weight is None) or k is None and k_weight is not None:
+        if q_heads == 0 or (k is not None and k[0][2] == 0):
+            raise ValueError("q and k need at least one head")
+        if (k is not None and (q_weight is None) != (k_weight is None)) or (k is None and k_weight is not None):
             raise ValueError("q_weight and k_weight go together")
-        weights = []
         for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None and (w.shape != (dim,) or w.dtype != q.dtype or w.device != q.device):
+            if w is not None and (w[0] != (dim,) or w[2] != dtype or w[3] != device):
                 raise ValueError(f"{name} must be (head_dim,) of q's dtype, on its device")
-            w = None if w is None else w.contiguous()
-            weights.append(w.clone() if w is not None and w.data_ptr() % 16 else w)
-        self.q_weight, self.k_weight = weights
-        batch, tokens = q.shape[:2]
         axes = len(rotary.sections)
-        if (positions.dtype not in _POSITION_TYPES or positions.device != q.device
-                or positions.shape not in ((tokens, axes), (batch, tokens, axes))):
+        if positions[2] not in _POSITION_TYPES or positions[3] != device or positions[0] not in ((tokens, axes),
+                                                                                                 (batch, tokens, axes)):
             raise ValueError("positions must be (seq, axes) or (B, seq, axes), int32, int64 or float32, on q's device")
         if not (eps >= 0.0):
             raise ValueError("eps must not be negative")
-        self.positions = positions.contiguous()
-        self.position_batch = tokens * axes if positions.ndim == 3 else 0
-        self.turns = rotary._turns
+        self.position_batch = tokens * axes if len(positions[0]) == 3 else 0
         self.empty = batch == 0 or tokens == 0
         self.shape = native.AxialRopeShape(
-            batch=batch, tokens=tokens, q_heads=q.size(2), k_heads=0 if k is None else k.size(2), head_dim=dim, axes=axes,
+            batch=batch, tokens=tokens, q_heads=q_heads, k_heads=0 if k is None else k[0][2], head_dim=dim, axes=axes,
             sections=(C.c_int32 * 4)(*rotary.sections), interleaved=int(rotary.interleaved),
-            positions_type=_POSITION_TYPES[positions.dtype], is_bf16=int(q.dtype == torch.bfloat16), eps=float(eps))
-        if q.size(2) == 0 or (k is not None and k.size(2) == 0):
-            raise ValueError("q and k need at least one head")
+            positions_type=_POSITION_TYPES[positions[2]], is_bf16=int(dtype == torch.bfloat16), eps=float(eps))
+        self.of_inputs = _head_strides(q) + _head_strides(k)
+        self.of_packed = tuple(n for heads in (q_heads, self.shape.k_heads)
+                               for n in (tokens * heads * dim, heads * dim, dim))
+        self.forward_strides = {place: native.strides_array(self.of_inputs + out)
+                                for place, out in ((True, self.of_inputs), (False, self.of_packed))}
+        self.backward_bytes = 0 if self.empty else native.axial_rope_backward_bytes(self.shape)
+        self.q_layout, self.k_layout = q, k
+
+    @lru_cache(maxsize=16)
+    def backward_strides(self, dq_out, dk_out):
+        for name, t, like in (("dq_out", dq_out, self.q_layout), ("dk_out", dk_out, self.k_layout)):
+            if (t is None) != (like is None) or (t is not None and t[0] != like[0]):
+                raise ValueError(f"{name} must have the shape of the output")
+            if t is not None:
+                _check_heads(t, name, self.q_layout)
+        return native.strides_array(_head_strides(dq_out) + _head_strides(dk_out) + self.of_inputs + self.of_packed)
+
+
+_axial_plan = lru_cache(maxsize=256)(_AxialPlan)
+
+
+def _aligned(**tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.data_ptr() % 16:
+            raise ValueError(f"the heads of {name} must be contiguous and start on 16 bytes")
+
+
+def _packed16(t: torch.Tensor | None) -> torch.Tensor | None:
+    """A small tensor as the kernels read it: contiguous, on 16 bytes."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, inplace):
-    c = _AxialCall(q, k, q_weight, k_weight, positions, rotary, eps)
+    plan = _axial_plan(_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(positions), rotary, eps)
     q_out = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     k_out = k if inplace or k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if not c.empty:
-        strides = [s for t in (q, k, q_out, k_out) for s in _head_strides(t)]
-        native.axial_rope(c.shape, q, k, c.q_weight, c.k_weight, c.positions, c.position_batch, c.turns, strides, q_out,
-                          k_out)
+    if not plan.empty:
+        _aligned(q=q, k=k)
+        native.axial_rope(plan.shape, q, k, _packed16(q_weight), _packed16(k_weight), positions.contiguous(),
+                          plan.position_batch, rotary._turns, plan.forward_strides[inplace], q_out, k_out)
     return q_out, k_out
 
 
 def _axial_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, rotary, eps, wanted=(True, True)):
-    c = _AxialCall(q, k, q_weight, k_weight, positions, rotary, eps)
-    for name, t, like in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
-        if (t is None) != (like is None) or t is not None and t.shape != like.shape:
-            raise ValueError(f"{name} must have the shape of the output")
-        if t is not None:
-            _heads(t, name, q)
+    plan = _axial_plan(_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(positions), rotary, eps)
+    strides = plan.backward_strides(_layout(dq_out), _layout(dk_out))
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    make = torch.zeros if c.empty else torch.empty
+    make = torch.zeros if plan.empty else torch.empty
     dq_weight, dk_weight = (None if w is None or not want else make(w.shape, dtype=w.dtype, device=w.device)
-                            for w, want in zip((c.q_weight, c.k_weight), wanted))
-    if not c.empty:
-        strides = [s for t in (dq_out, dk_out, q, k, dq, dk) for s in _head_strides(t)]
-        native.axial_rope_backward(c.shape, dq_out, dk_out, q, k, c.q_weight, c.k_weight, c.positions, c.position_batch,
-                                   c.turns, strides, dq, dk, dq_weight, dk_weight)
+                            for w, want in zip((q_weight, k_weight), wanted))
+    if not plan.empty:
+        _aligned(dq_out=dq_out, dk_out=dk_out, q=q, k=k)
+        native.axial_rope_backward(plan.shape, dq_out, dk_out, q, k, _packed16(q_weight), _packed16(k_weight),
+                                   positions.contiguous(), plan.position_batch, rotary._turns, strides, dq, dk, dq_weight,
+                                   dk_weight, 0 if dq_weight is None and dk_weight is None else plan.backward_bytes)
     return dq, dk, dq_weight, dk_weight
 
 
@@ -189,8 +214,8 @@ class _AxialRope(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
-        grads = [None if t is None else t.contiguous() for t in (dq_out, dk_out)]
-        grads = [t.clone() if t is not None and t.data_ptr() % 16 else t for t in grads]
+        # autograd hands gradients over in any layout (expanded, transposed)
+        grads = [_packed16(dq_out), _packed16(dk_out)]
         q, k, *_ = ctx.saved_tensors
         if k is None:
             grads[1] = None
@@ -206,10 +231,11 @@ def fused_qknorm_axial_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: t
 
     ``positions``: ``(seq, axes)`` or ``(B, seq, axes)``, whole or fractional.  New tensors, recorded by autograd; with
     ``inplace`` q and k are overwritten, as ``fused_qknorm_rope`` does, which autograd cannot go through."""
-    if inplace:
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-            raise ValueError("inplace=True overwrites what the gradient needs")
-        return _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, True)
+    recorded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    if inplace and recorded:
+        raise ValueError("inplace=True overwrites what the gradient needs")
+    if not recorded:
+        return _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, bool(inplace))
     return _AxialRope.apply(q, k, q_weight, k_weight, positions, rotary, eps)
 
 
