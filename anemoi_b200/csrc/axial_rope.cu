@@ -10,9 +10,11 @@
 // sines).  Gradient: g = the output's, turned back (angle -a); w's is sum g_j x_j r; with b = g w the input's is
 // r (b - x r mean(b x r)).
 //
-// The angle is formed in double precision and reduced to a fraction of a turn there: position * turns has 2^-53 relative,
-// so that positions of 2^31 still have angles good to 2^-22 of a turn, where a product in fp32 has none beyond 2^24.  Cosine
-// and sine of the fraction are fp32 (sincospif).
+// The angle is reduced to a fraction of a turn before it is rounded to fp32, where a product in fp32 has no bits left beyond
+// positions of 2^24.  Whole positions: the frequency is a 64-bit fraction of a turn, and the low 64 bits of its product with
+// the position are the angle's fraction (a position of 2^31 is 2^-22 of a turn off, as the frequency is a double's 53 bits).
+// Fractional positions: the same in double precision.  Of the fraction, within half
+// a turn, the fast cosine and sine are good to 2^-20.
 #include <math.h>
 #include <stdint.h>
 
@@ -31,317 +33,387 @@ struct RopeParams {
   const void *q, *k, *dq_out, *dk_out, *q_weight, *k_weight, *positions;
   void *q_out, *k_out;
   float* weight_partial;  // [blocks of queries, then of keys][D]
-  int64_t position_batch, batch, tokens;
+  int64_t position_batch;
+  uint32_t batch, tokens;
   int64_t strides[6][3];  // forward: q, k, q_out, k_out; gradient: dq_out, dk_out, q, k, dq, dk
-  int q_heads, k_heads, axes, pairs, interleaved, positions_type, block_tokens, q_blocks;
+  int q_heads, k_heads, axes, pairs, interleaved, positions_type, q_blocks;
   float eps;
   int ends[4];       // of the axes' pairs
-  double turns[64];
+  double rates[64];    // frequencies in turns
+  uint64_t turns[64];  // the frequencies' fractions of a turn times 2^64
 };
 
-// Cosines and sines of `count` tokens from `first` on: [token][cosines of all pairs, then sines].
-__device__ __forceinline__ void angles(const RopeParams& p, int64_t first, int count, float* table) {
-  for (int i = threadIdx.x; i < count * p.pairs; i += kThreads) {
-    const int t = i / p.pairs, pair = i - t * p.pairs;
-    int axis = 0;
-    while (axis < p.axes - 1 && pair >= p.ends[axis]) ++axis;
-    const int64_t token = first + t, b = quotient(token, p.tokens);
-    const int64_t at = b * p.position_batch + (token - b * p.tokens) * p.axes + axis;
-    const double position = p.positions_type == 0   ? (double)static_cast<const int32_t*>(p.positions)[at]
-                            : p.positions_type == 1 ? (double)static_cast<const int64_t*>(p.positions)[at]
-                                                    : (double)static_cast<const float*>(p.positions)[at];
-    const double turn = position * p.turns[pair];
-    float s, c;
-    sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
-    table[2 * t * p.pairs + pair] = c;
-    table[(2 * t + 1) * p.pairs + pair] = s;
+// The position of a sample's token on the axis of a pair, as it lies in memory (32 bits of whatever type, or 64).
+__device__ __forceinline__ int64_t position_of(const RopeParams& p, uint32_t token, int pair) {
+  int axis = 0;
+#pragma unroll
+  for (int a = 0; a < 3; ++a) axis += pair >= p.ends[a];
+  const int64_t at = blockIdx.y * p.position_batch + (int64_t)token * p.axes + axis;
+  if (p.positions_type == 1) return static_cast<const int64_t*>(p.positions)[at];
+  return static_cast<const int32_t*>(p.positions)[at];
+}
+// Cosine and sine of the pair's angle.
+__device__ __forceinline__ float2 angle_of(const RopeParams& p, int64_t position, int pair) {
+  float turn;
+  if (p.positions_type == 2) {
+    const double exact = (double)__int_as_float((int)position) * p.rates[pair];
+    turn = (float)(exact - rint(exact));
+  } else {
+    const uint64_t fraction = (uint64_t)position * p.turns[pair];
+    turn = (float)(int32_t)(uint32_t)(fraction >> 32) * 0x1p-32f;
   }
+  const float radians = 6.283185307f * turn;
+  return make_float2(__cosf(radians), __sinf(radians));
 }
 
-// What a lane has of a head: 8 consecutive channels.
+// What a lane has of a head: two pieces of 4 channels, which are 4 whole pairs where they turn.  Halves: channels 4 l ... and
+// their partners P channels on; neighbours: 8 channels in a row.  No pair crosses lanes, so that turning needs no shuffles
+// (with 8 channels in a row for both, 8 shuffles per row and half the arithmetic idle: 430 us for 33,272 tokens of 112 heads
+// of 128).
 struct Span {
-  bool in, first;
-  int partner, pair;
-  __device__ __forceinline__ Span(int lane, int pairs, int interleaved) {
-    const int c0 = lane * 8;
-    in = c0 < 2 * pairs;
-    first = c0 < pairs;
-    partner = in && !interleaved ? (first ? lane + pairs / 8 : lane - pairs / 8) : lane;
-    pair = interleaved ? c0 / 2 : first ? c0 : c0 - pairs;
+  int first, second;  // channels
+  bool in;
+  __device__ __forceinline__ Span(int lane, int pairs, bool interleaved) {
+    in = 4 * lane < pairs;
+    first = interleaved ? 8 * lane : in ? 4 * lane : 2 * pairs + 8 * (lane - pairs / 4);
+    second = interleaved || !in ? first + 4 : first + pairs;
   }
 };
 
-// A lane's cosines and sines (of its 8 channels' pairs, or of its 4 pairs of neighbours).  Halves: the sines of the first
-// one's channels change sign here.  kBack: of the opposite angles.
-template <bool kBack>
-__device__ __forceinline__ void load_angles(const float* row, const Span& span, int pairs, bool interleaved, float (&c)[8],
-                                            float (&s)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    c[i] = 1.0f;
-    s[i] = 0.0f;
+// The lane's 4 pairs' cosines and sines; 1 and 0 where its channels do not turn.
+__device__ __forceinline__ void load_angles(const float* row, int lane, const Span& span, int pairs, float4& c, float4& s) {
+  c = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+  s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (span.in) {
+    c = *reinterpret_cast<const float4*>(row + 4 * lane);
+    s = *reinterpret_cast<const float4*>(row + pairs + 4 * lane);
   }
-  if (!span.in) return;
-  *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(row + span.pair);
-  *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(row + pairs + span.pair);
-  if (!interleaved) {
-    *reinterpret_cast<float4*>(c + 4) = *reinterpret_cast<const float4*>(row + span.pair + 4);
-    *reinterpret_cast<float4*>(s + 4) = *reinterpret_cast<const float4*>(row + pairs + span.pair + 4);
-  }
-  const bool minus = interleaved ? kBack : span.first != kBack;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = minus ? -s[i] : s[i];
 }
 
-// Turns a lane's 8 channels.  All lanes of the warp take part.
-template <int kLanes>
-__device__ __forceinline__ void turn8(float (&n)[8], const Span& span, bool interleaved, const float (&c)[8],
-                                      const float (&s)[8]) {
+// A lane's 8 channels as the first and the second of each of its 4 pairs: u[0] = (u_0, u_1), u[1] = (u_2, u_3), v alike.
+template <typename T>
+__device__ __forceinline__ void open_pairs(uint2 a, uint2 b, bool interleaved, float2 (&u)[2], float2 (&v)[2]) {
+  const float2 a0 = Pair<T>::open(a.x), a1 = Pair<T>::open(a.y), b0 = Pair<T>::open(b.x), b1 = Pair<T>::open(b.y);
+  u[0] = interleaved ? make_float2(a0.x, a1.x) : a0;
+  v[0] = interleaved ? make_float2(a0.y, a1.y) : b0;
+  u[1] = interleaved ? make_float2(b0.x, b1.x) : a1;
+  v[1] = interleaved ? make_float2(b0.y, b1.y) : b1;
+}
+template <typename T>
+__device__ __forceinline__ void store_pairs(T* a, T* b, bool interleaved, const float2 (&u)[2], const float2 (&v)[2]) {
   if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float u = n[2 * i], v = n[2 * i + 1];
-      n[2 * i] = fmaf(-v, s[i], u * c[i]);
-      n[2 * i + 1] = fmaf(u, s[i], v * c[i]);
-    }
-    return;
+    *reinterpret_cast<uint2*>(a) = make_uint2(Pair<T>::round(u[0].x, v[0].x), Pair<T>::round(u[0].y, v[0].y));
+    *reinterpret_cast<uint2*>(b) = make_uint2(Pair<T>::round(u[1].x, v[1].x), Pair<T>::round(u[1].y, v[1].y));
+  } else {
+    *reinterpret_cast<uint2*>(a) = make_uint2(Pair<T>::round(u[0].x, u[0].y), Pair<T>::round(u[1].x, u[1].y));
+    *reinterpret_cast<uint2*>(b) = make_uint2(Pair<T>::round(v[0].x, v[0].y), Pair<T>::round(v[1].x, v[1].y));
   }
-  float other[8];
+}
+__device__ __forceinline__ float2 negative(float2 a) { return make_float2(-a.x, -a.y); }
+
+// Sums of N rows over kLanes lanes, each in the lanes that shuffle `row * (kLanes / N)` names; the lanes first share the rows
+// out, half of them per step.
+template <int kLanes, int N>
+__device__ __forceinline__ float shared_out_sum(const float (&v)[N]) {
+  static_assert(N == 1 || N == 2 || N == 4, "shared out by halves");
+  const int lane = threadIdx.x;
+  float mine = v[0];
+  int off = kLanes / 2;
+  if constexpr (N == 4) {
+    const bool high = lane & (kLanes / 2), next = lane & (kLanes / 4);
+    const float a = (high ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, high ? v[0] : v[2], kLanes / 2);
+    const float b = (high ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, high ? v[1] : v[3], kLanes / 2);
+    mine = (next ? b : a) + __shfl_xor_sync(0xffffffffu, next ? a : b, kLanes / 4);
+    off = kLanes / 8;
+  } else if constexpr (N == 2) {
+    const bool high = lane & (kLanes / 2);
+    mine = (high ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, high ? v[0] : v[1], kLanes / 2);
+    off = kLanes / 4;
+  }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, n[i], span.partner, kLanes);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = fmaf(other[i], s[i], n[i] * c[i]);
+  for (int o = kLanes / 2; o > 0; o >>= 1)
+    if (o <= off) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  return mine;
 }
 
-template <int kLanes>
-__device__ __forceinline__ float row_sum(float v) {
-#pragma unroll
-  for (int off = kLanes / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  return v;
+// Groups of D/8 lanes take kRows heads of one token of sample blockIdx.y: a unit.  A warp's units are of one token or of
+// neighbours.
+struct Unit {
+  uint32_t first, into;   // the warp's first token, its first unit's place there
+  uint32_t t, token;      // the group's token, from the first one and from the sample's
+  uint32_t place;         // of the unit among its token's
+};
+template <int kUnits>
+__device__ __forceinline__ uint32_t token_in_warp(uint32_t local, uint32_t per_token) {
+  return per_token >= kUnits ? (uint32_t)(local >= per_token) : local / per_token;
+}
+template <int kUnits>
+__device__ __forceinline__ Unit unit_at(uint32_t warp_unit, int group, uint32_t per_token) {
+  Unit u;
+  u.first = warp_unit / per_token;
+  u.into = warp_unit - u.first * per_token;
+  const uint32_t local = u.into + group;
+  u.t = token_in_warp<kUnits>(local, per_token);
+  u.token = u.first + u.t;
+  u.place = local - u.t * per_token;
+  return u;
+}
+// The angles of the warp's tokens, each once: [token][cosines of all pairs, then sines], in shared memory of the warp's own.
+template <int kUnits>
+__device__ __forceinline__ void warp_angles(const RopeParams& p, const Unit& u, uint32_t per_token, float* table) {
+  const uint32_t last = token_in_warp<kUnits>(u.into + kUnits - 1, per_token);
+  for (uint32_t n = 0; n <= last; ++n)
+    if (u.first + n < p.tokens)
+      for (int pair = threadIdx.x % 32; pair < p.pairs; pair += 32) {
+        const float2 cs = angle_of(p, position_of(p, u.first + n, pair), pair);
+        table[2 * n * p.pairs + pair] = cs.x;
+        table[(2 * n + 1) * p.pairs + pair] = cs.y;
+      }
 }
 
-// Groups of D/8 lanes take kRows heads of one token: a unit.  A block has as many units as groups, of one token or of
-// neighbours, whose angles it forms once in shared memory while the heads' loads are in flight.  HBM bound: two bytes in and
-// two out per channel.  One unit per group: several in turn, whose loads only start when the one before is done, took 430 us
-// for 33,272 tokens of 112 heads of 128.
-template <typename T, int D, int kRows>
-__global__ void __launch_bounds__(kThreads, 4) forward_kernel(const __grid_constant__ RopeParams p) {
-  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes;
-  __shared__ __align__(16) float table[(kGroups + 1) * D];
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  const uint32_t all = (uint32_t)(p.batch * p.tokens);
+// HBM bound: two bytes in and two out per channel; what comes next is issue slots, hence packed arithmetic, with the weights
+// multiplied into the cosines and sines once for all rows: out = r (u w_u c - v w_v s), r (v w_v c + u w_u s).  The angles are
+// formed while the heads' loads are in flight.  (One table per block, behind a barrier: 377 us for 33,272 tokens of 112 heads
+// of 128.)
+__host__ __device__ constexpr int forward_blocks(int rows) { return rows == 8 ? 3 : 4; }
+template <typename T, int D, int kRows, bool interleaved>
+__global__ void __launch_bounds__(kThreads, forward_blocks(kRows)) forward_kernel(const __grid_constant__ RopeParams p) {
+  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes, kUnits = 32 / kLanes;
+  __shared__ __align__(16) float tables[kThreads / 32][kUnits * D];
+  float* table = tables[threadIdx.x / 32];
+  const int lane = threadIdx.x % kLanes;
   const uint32_t q_units = (p.q_heads + kRows - 1) / kRows, per_token = q_units + (p.k_heads + kRows - 1) / kRows;
-  const uint64_t unit0 = (uint64_t)blockIdx.x * kGroups;
-  const uint32_t first = (uint32_t)quotient(unit0, per_token);
-  const uint32_t local = (uint32_t)(unit0 - (uint64_t)first * per_token) + group, t = local / per_token;
-  const uint32_t token = first + t, u = local - t * per_token;
-  const bool is_q = u < q_units;
-  const int head = (int)(is_q ? u : u - q_units) * kRows;
-  const int heads = token < all ? min(kRows, (is_q ? p.q_heads : p.k_heads) - head) : 0;
-  const uint32_t b = token / (uint32_t)p.tokens, at = token - b * (uint32_t)p.tokens;
+  const Unit u = unit_at<kUnits>(blockIdx.x * kGroups + threadIdx.x / 32 * kUnits, threadIdx.x % 32 / kLanes, per_token);
+  const bool is_q = u.place < q_units;
+  const int head = (int)(is_q ? u.place : u.place - q_units) * kRows;
+  const int heads = u.token < p.tokens ? min(kRows, (is_q ? p.q_heads : p.k_heads) - head) : 0;
   const int64_t *in = p.strides[is_q ? 0 : 1], *out = p.strides[is_q ? 2 : 3];
-  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + b * in[0] + at * in[1] + head * in[2] + lane * 8;
-  uint4 raw[kRows];
+  const Span span(lane, p.pairs, interleaved);
+  const T* src = static_cast<const T*>(is_q ? p.q : p.k) + blockIdx.y * in[0] + u.token * in[1] + head * in[2];
+  uint2 raw[kRows][2];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (i < heads) raw[i] = load_stream(src + i * in[2]);
-  }
-  const uint32_t last = (uint32_t)(unit0 - (uint64_t)first * per_token + kGroups - 1) / per_token;
-  angles(p, first, (int)(min(all, first + last + 1) - first), table);
-  const T* weight = static_cast<const T*>(is_q ? p.q_weight : p.k_weight);
-  const bool normed = p.q_weight != nullptr;
-  float w[8];
-  if (normed) shared8(weight + lane * 8, w);
-  __syncthreads();
-  const Span span(lane, p.pairs, p.interleaved);
-  float cs[8], sn[8];
-  load_angles<false>(table + 2 * t * p.pairs, span, p.pairs, p.interleaved, cs, sn);
-  T* dst = static_cast<T*>(is_q ? p.q_out : p.k_out) + b * out[0] + at * out[1] + head * out[2] + lane * 8;
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    float n[8];
-    open8<T>(raw[i], n);
-    if (normed) {
-      float s = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s = fmaf(n[j], n[j], s);
-      const float r = rsqrtf(fmaf(row_sum<kLanes>(s), 1.0f / D, p.eps));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) n[j] = n[j] * r * w[j];
+    raw[i][0] = raw[i][1] = make_uint2(0, 0);
+    if (i < heads) {
+      raw[i][0] = load_stream8(src + span.first);
+      raw[i][1] = load_stream8(src + span.second);
     }
-    turn8<kLanes>(n, span, p.interleaved, cs, sn);
-    if (i < heads) *reinterpret_cast<uint4*>(dst + i * out[2]) = round8<T>(n);
+    src += in[2];
+  }
+  warp_angles<kUnits>(p, u, per_token, table);
+  const bool normed = p.q_weight != nullptr;
+  float2 wu[2] = {both(1.0f), both(1.0f)}, wv[2] = {both(1.0f), both(1.0f)};
+  if (normed) {
+    const T* weight = static_cast<const T*>(is_q ? p.q_weight : p.k_weight);
+    open_pairs<T>(__ldg(reinterpret_cast<const uint2*>(weight + span.first)),
+                  __ldg(reinterpret_cast<const uint2*>(weight + span.second)), interleaved, wu, wv);
+  }
+  __syncwarp();
+  float4 c4, s4;
+  load_angles(table + 2 * u.t * p.pairs, lane, span, p.pairs, c4, s4);
+  const float2 c[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
+  const float2 s[2] = {make_float2(s4.x, s4.y), make_float2(s4.z, s4.w)};
+  float2 uc[2], us[2], vc[2], vs[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uc[j] = fmul2(wu[j], c[j]);
+    us[j] = fmul2(wu[j], s[j]);
+    vc[j] = fmul2(wv[j], c[j]);
+    vs[j] = negative(fmul2(wv[j], s[j]));
+  }
+  T* dst = static_cast<T*>(is_q ? p.q_out : p.k_out) + blockIdx.y * out[0] + u.token * out[1] + head * out[2];
+  constexpr int kShared = kRows < 4 ? kRows : 4;  // rows that share a sum over the lanes
+#pragma unroll
+  for (int i0 = 0; i0 < kRows; i0 += kShared) {
+    float r_mine = 1.0f;
+    if (normed) {
+      float squares[kShared];
+#pragma unroll
+      for (int i = 0; i < kShared; ++i) {
+        float2 x[2], y[2];
+        open_pairs<T>(raw[i0 + i][0], raw[i0 + i][1], false, x, y);
+        float2 sum = fmul2(x[0], x[0]);
+        sum = ffma2(x[1], x[1], sum);
+        sum = ffma2(y[0], y[0], sum);
+        sum = ffma2(y[1], y[1], sum);
+        squares[i] = sum.x + sum.y;
+      }
+      r_mine = rsqrtf(fmaf(shared_out_sum<kLanes, kShared>(squares), 1.0f / D, p.eps));
+    }
+#pragma unroll
+    for (int i = 0; i < kShared; ++i) {
+      float2 x[2], y[2];
+      open_pairs<T>(raw[i0 + i][0], raw[i0 + i][1], interleaved, x, y);
+      const float2 r = both(normed ? __shfl_sync(0xffffffffu, r_mine, i * (kLanes / kShared), kLanes) : 1.0f);
+      float2 a[2], e[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        a[j] = fmul2(ffma2(y[j], vs[j], fmul2(x[j], uc[j])), r);
+        e[j] = fmul2(ffma2(x[j], us[j], fmul2(y[j], vc[j])), r);
+      }
+      if (i0 + i < heads) store_pairs<T>(dst + span.first, dst + span.second, interleaved, a, e);
+      dst += out[2];
+    }
   }
 }
 
-// The gradient.  A block has queries or keys, and walks sets of block_tokens tokens a grid apart, so that a thread's 8 sums
-// of the weight stay in registers; they are added over its groups at the end, and the blocks' by sums_kernel.  The next
-// units are copied into a ring of shared memory meanwhile (a thread's own channels).
-constexpr int kBackwardRows = 2, kRing = 4;
-template <typename T, int D>
+// The gradient, the same way.  A block has queries or keys and walks units a grid apart, so that a thread's 8 sums of the
+// weight stay in registers; they are added over its groups at the end, and the blocks' by sums_kernel.  Blocks are many more
+// than fit at once: loads of one are in flight under the arithmetic of others (a ring of copies ahead, in blocks that stay,
+// cost more instructions than it hid: 150 us for 32,256 tokens of 32 heads of 64).
+constexpr int kBackwardRows = 4;
+template <typename T, int D, bool interleaved>
 __global__ void __launch_bounds__(kThreads, 3) backward_kernel(const __grid_constant__ RopeParams p) {
-  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes, kRows = kBackwardRows;
-  extern __shared__ __align__(16) uint4 ring_all[];  // [kRing][d, x][kRows][thread]
-  __shared__ __align__(16) float table[16 * 128];
+  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes, kUnits = 32 / kLanes, kRows = kBackwardRows;
+  __shared__ __align__(16) float tables[kThreads / 32][kUnits * D];
+  __shared__ float sums[kGroups][D];
+  float* table = tables[threadIdx.x / 32];
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  const bool keys = (int)blockIdx.x >= p.q_blocks;
+  const bool keys = (int)blockIdx.x >= p.q_blocks, normed = p.q_weight != nullptr;
   const int block = keys ? blockIdx.x - p.q_blocks : blockIdx.x, blocks = keys ? gridDim.x - p.q_blocks : p.q_blocks;
   const int all_heads = keys ? p.k_heads : p.q_heads, which = keys ? 1 : 0;
-  const uint32_t all = (uint32_t)(p.batch * p.tokens), per_token = (all_heads + kRows - 1) / kRows;
-  const uint32_t sets = (all + p.block_tokens - 1) / p.block_tokens, units = p.block_tokens * per_token;
-  const uint32_t steps = (units + kGroups - 1) / kGroups;
-  const Span span(lane, p.pairs, p.interleaved);
-  const bool normed = p.q_weight != nullptr;
+  const uint32_t per_token = (all_heads + kRows - 1) / kRows, units = p.tokens * per_token;
+  const Span span(lane, p.pairs, interleaved);
   const T* weight = static_cast<const T*>(keys ? p.k_weight : p.q_weight);
   const int64_t *ds = p.strides[which], *xs = p.strides[2 + which], *os = p.strides[4 + which];
-  const T* d_all = static_cast<const T*>(keys ? p.dk_out : p.dq_out) + lane * 8;
-  const T* x_all = static_cast<const T*>(keys ? p.k : p.q) + lane * 8;
-  T* out_all = static_cast<T*>(keys ? p.k_out : p.q_out) + lane * 8;
-  float w[8];
-  if (normed) shared8(weight + lane * 8, w);
-  float weight_sum[8] = {};
-  struct Unit {
-    uint32_t b, at, t;
-    int head, heads;
-  };
-  auto unit_of = [&](uint32_t set, uint32_t step) {
-    const uint32_t unit = step * kGroups + group;
-    Unit u;
-    u.t = unit / per_token;
-    const uint32_t token = set * p.block_tokens + u.t;
-    u.head = (int)(unit - u.t * per_token) * kRows;
-    u.heads = unit < units && token < all ? min(kRows, all_heads - u.head) : 0;
-    u.b = token / (uint32_t)p.tokens;
-    u.at = token - u.b * (uint32_t)p.tokens;
-    if (u.heads == 0) u.t = 0;
-    return u;
-  };
-  uint4* ring = ring_all + threadIdx.x;
-  uint32_t ahead_set = block, ahead_step = 0;
-  int ahead_place = 0;
-  auto copy_next = [&]() {
-    if (ahead_set < sets) {
-      const Unit u = unit_of(ahead_set, ahead_step);
-      uint4* to = ring + ahead_place * (2 * kRows * kThreads);
+  float2 wu[2] = {both(1.0f), both(1.0f)}, wv[2] = {both(1.0f), both(1.0f)};
+  if (normed)
+    open_pairs<T>(__ldg(reinterpret_cast<const uint2*>(weight + span.first)),
+                  __ldg(reinterpret_cast<const uint2*>(weight + span.second)), interleaved, wu, wv);
+  float2 sum_u[2] = {both(0.0f), both(0.0f)}, sum_v[2] = {both(0.0f), both(0.0f)};
+#pragma unroll 1
+  for (uint32_t unit = block * kGroups; unit < units; unit += blocks * kGroups) {
+    const Unit u = unit_at<kUnits>(unit + threadIdx.x / 32 * kUnits, threadIdx.x % 32 / kLanes, per_token);
+    const int head = (int)u.place * kRows, heads = u.token < p.tokens ? min(kRows, all_heads - head) : 0;
+    const T* d = static_cast<const T*>(keys ? p.dk_out : p.dq_out) + blockIdx.y * ds[0] + u.token * ds[1] + head * ds[2];
+    const T* x = static_cast<const T*>(keys ? p.k : p.q) + blockIdx.y * xs[0] + u.token * xs[1] + head * xs[2];
+    uint2 d_raw[kRows][2], x_raw[kRows][2];
 #pragma unroll
-      for (int i = 0; i < kRows; ++i)
-        if (i < u.heads) {
-          copy_async16(to + i * kThreads, d_all + u.b * ds[0] + u.at * ds[1] + (u.head + i) * ds[2]);
-          if (normed) copy_async16(to + (kRows + i) * kThreads, x_all + u.b * xs[0] + u.at * xs[1] + (u.head + i) * xs[2]);
-        }
-    }
-    copy_commit();
-    ahead_place = ahead_place + 1 == kRing ? 0 : ahead_place + 1;
-    if (++ahead_step == steps) {
-      ahead_step = 0;
-      ahead_set += blocks;
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kRing - 1; ++i) copy_next();
-  int place = 0;
-  for (uint32_t set = block; set < sets; set += blocks) {
-    const uint32_t first = set * p.block_tokens;
-    __syncthreads();
-    angles(p, first, (int)min((uint32_t)p.block_tokens, all - first), table);
-    __syncthreads();
-    for (uint32_t step = 0; step < steps; ++step) {
-      const Unit u = unit_of(set, step);
-      // (into the place that was read in the step before, by this thread alone)
-      copy_next();
-      copy_wait<kRing - 1>();
-      const uint4* from = ring + place * (2 * kRows * kThreads);
-      place = place + 1 == kRing ? 0 : place + 1;
-      float cs[8], sn[8];
-      load_angles<true>(table + 2 * u.t * p.pairs, span, p.pairs, p.interleaved, cs, sn);
-      T* out = out_all + u.b * os[0] + u.at * os[1] + u.head * os[2];
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        float g[8];
-        open8<T>(i < u.heads ? from[i * kThreads] : make_uint4(0, 0, 0, 0), g);
-        turn8<kLanes>(g, span, p.interleaved, cs, sn);
+    for (int i = 0; i < kRows; ++i) {
+      d_raw[i][0] = d_raw[i][1] = x_raw[i][0] = x_raw[i][1] = make_uint2(0, 0);
+      if (i < heads) {
+        d_raw[i][0] = load_stream8(d + span.first);
+        d_raw[i][1] = load_stream8(d + span.second);
         if (normed) {
-          float v[8];
-          float2 s = make_float2(0.0f, 0.0f);
-          open8<T>(i < u.heads ? from[(kRows + i) * kThreads] : make_uint4(0, 0, 0, 0), v);
+          x_raw[i][0] = load_stream8(x + span.first);
+          x_raw[i][1] = load_stream8(x + span.second);
+        }
+      }
+      d += ds[2];
+      x += xs[2];
+    }
+    // (everybody in the warp has read the angles of the units before)
+    __syncwarp();
+    warp_angles<kUnits>(p, u, per_token, table);
+    __syncwarp();
+    float4 c4, s4;
+    load_angles(table + 2 * u.t * p.pairs, lane, span, p.pairs, c4, s4);
+    const float2 c[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
+    const float2 s[2] = {make_float2(s4.x, s4.y), make_float2(s4.z, s4.w)};
+    const float2 minus_s[2] = {negative(s[0]), negative(s[1])};
+    T* out = static_cast<T*>(keys ? p.k_out : p.q_out) + blockIdx.y * os[0] + u.token * os[1] + head * os[2];
+    // two rows at a time
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            s.x = fmaf(v[j], v[j], s.x);
-            s.y = fmaf(g[j] * w[j], v[j], s.y);
-          }
-          s = make_float2(row_sum<kLanes>(s.x), row_sum<kLanes>(s.y));
-          const float r = rsqrtf(fmaf(s.x, 1.0f / D, p.eps)), along = s.y * r * (1.0f / D);
+    for (int i0 = 0; i0 < kRows; i0 += 2) {
+      float2 gu[2][2], gv[2][2], xu[2][2], xv[2][2];
+      float row_sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[j] *= r;
-            weight_sum[j] = fmaf(g[j], v[j], weight_sum[j]);
-            g[j] = r * fmaf(-v[j], along, g[j] * w[j]);
+      for (int i = 0; i < 2; ++i) {
+        float2 a[2], e[2];
+        open_pairs<T>(d_raw[i0 + i][0], d_raw[i0 + i][1], interleaved, a, e);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          // turned back
+          gu[i][j] = ffma2(e[j], s[j], fmul2(a[j], c[j]));
+          gv[i][j] = ffma2(a[j], minus_s[j], fmul2(e[j], c[j]));
+        }
+        if (!normed) continue;
+        open_pairs<T>(x_raw[i0 + i][0], x_raw[i0 + i][1], interleaved, xu[i], xv[i]);
+        float2 square = both(0.0f), along = both(0.0f);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          square = ffma2(xu[i][j], xu[i][j], square);
+          square = ffma2(xv[i][j], xv[i][j], square);
+          along = ffma2(fmul2(gu[i][j], wu[j]), xu[i][j], along);
+          along = ffma2(fmul2(gv[i][j], wv[j]), xv[i][j], along);
+        }
+        row_sums[2 * i] = square.x + square.y;
+        row_sums[2 * i + 1] = along.x + along.y;
+      }
+      const float mine = normed ? shared_out_sum<kLanes, 4>(row_sums) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (normed) {
+          const float square = __shfl_sync(0xffffffffu, mine, 2 * i * (kLanes / 4), kLanes);
+          const float with_x = __shfl_sync(0xffffffffu, mine, (2 * i + 1) * (kLanes / 4), kLanes);
+          // (a head that does not exist is zeros, and stays so with eps = 0)
+          const float r = i0 + i < heads ? rsqrtf(fmaf(square, 1.0f / D, p.eps)) : 0.0f;
+          const float2 r2 = both(r), back = both(-with_x * r * r * (1.0f / D));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            sum_u[j] = ffma2(gu[i][j], fmul2(xu[i][j], r2), sum_u[j]);
+            sum_v[j] = ffma2(gv[i][j], fmul2(xv[i][j], r2), sum_v[j]);
+            gu[i][j] = fmul2(ffma2(xu[i][j], back, fmul2(gu[i][j], wu[j])), r2);
+            gv[i][j] = fmul2(ffma2(xv[i][j], back, fmul2(gv[i][j], wv[j])), r2);
           }
         }
-        if (i < u.heads) *reinterpret_cast<uint4*>(out + i * os[2]) = round8<T>(g);
+        if (i0 + i < heads) store_pairs<T>(out + span.first, out + span.second, interleaved, gu[i], gv[i]);
+        out += os[2];
       }
     }
   }
-  copy_wait<0>();
   if (p.weight_partial == nullptr) return;
-  // [group][D] over the ring, which nobody reads any more
-  float* sums = reinterpret_cast<float*>(ring_all);
-  __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sums[group * D + lane * 8 + j] = weight_sum[j];
+  for (int i = 0; i < 4; ++i) {
+    const float a = i & 1 ? sum_u[i / 2].y : sum_u[i / 2].x, e = i & 1 ? sum_v[i / 2].y : sum_v[i / 2].x;
+    const int at = interleaved ? (i < 2 ? span.first + 2 * i : span.second + 2 * (i - 2)) : span.first + i;
+    const int partner = interleaved ? at + 1 : span.second + i;
+    sums[group][at] = a;
+    sums[group][partner] = e;
+  }
   __syncthreads();
   if (threadIdx.x < D) {
     float total = 0.0f;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) total += sums[g * D + threadIdx.x];
-    p.weight_partial[(int64_t)blockIdx.x * D + threadIdx.x] = total;
+    for (int g = 0; g < kGroups; ++g) total += sums[g][threadIdx.x];
+    // (all samples' parts of queries first)
+    const int64_t part = keys ? (int64_t)gridDim.y * p.q_blocks + blockIdx.y * blocks + block : blockIdx.y * blocks + block;
+    p.weight_partial[part * D + threadIdx.x] = total;
   }
 }
 
+constexpr int kSumThreads = 1024;  // (few columns, many parts)
+// blockIdx.y: queries', keys' weight; its blocks' parts.
 template <typename T>
-__global__ void sums_kernel(const float* partial, int q_blocks, int k_blocks, int d, void* dq_weight, void* dk_weight) {
-  const int column = blockIdx.x * 32 + threadIdx.x;
+__global__ void __launch_bounds__(kSumThreads) sums_kernel(const float* partial, int q_parts, int k_parts, int d,
+                                                           void* dq_weight, void* dk_weight) {
   void* out = blockIdx.y ? dk_weight : dq_weight;
-  if (out == nullptr) return;
-  const float v = column_sum(partial + (blockIdx.y ? (int64_t)q_blocks * d : 0), d, blockIdx.y ? k_blocks : q_blocks, column,
-                             true);
-  if (threadIdx.y == 0) store1(static_cast<T*>(out) + column, v);
+  const int parts = blockIdx.y ? k_parts : q_parts, across = sum_columns(parts), first = blockIdx.x * across;
+  if (out == nullptr || first >= d) return;
+  const float v = column_sum<kSumThreads>(partial + (blockIdx.y ? (int64_t)q_parts * d : 0), d, parts, first, d);
+  if (threadIdx.x < across) store1(static_cast<T*>(out) + first + threadIdx.x, v);
 }
 
-// Four heads per group of lanes (four loads in flight, one read of weights for them) where heads fill them and the groups
-// fill the SMs, one else.
+// Heads per group of lanes: eight (that many loads in flight, one read of weights and angles for them) where heads fill them
+// and the groups fill the SMs, four where one of the two is half so, else one.
 int rows_of(const anemoi_sm100_axial_rope_shape* s) {
-  const int64_t groups = (int64_t)kSms * kThreads / (s->head_dim / 8);
-  return std::max(s->q_heads, s->k_heads) > 2 && s->batch * s->tokens * (s->q_heads + s->k_heads) > groups ? 4 : 1;
+  const int64_t groups = (int64_t)kSms * 2 * kThreads / (s->head_dim / 8);
+  const int heads = std::max(s->q_heads, s->k_heads);
+  const int64_t rows = s->batch * s->tokens * (s->q_heads + s->k_heads);
+  return heads > 4 && rows >= 8 * groups ? 8 : heads > 2 && rows >= 2 * groups ? 4 : 1;
 }
 
-// The gradient's blocks: three per SM, shared by queries and keys as their heads are; tokens of a set: up to 16, whose units
-// leave the fewest groups of lanes without one in the last step.
+// The gradient's blocks of a sample: as many as its units fill, or as few as leave every SM 32 of them in all (a sum of the
+// weights has that many parts), each of as many turns.
 struct BackwardPlan {
-  int q_blocks, k_blocks, block_tokens;
+  int q_blocks, k_blocks;
 };
 BackwardPlan plan_of(const anemoi_sm100_axial_rope_shape* s) {
-  const int64_t tokens = s->batch * s->tokens;
-  const int groups = kThreads / (s->head_dim / 8), blocks = kSms * 3;
-  const int heads = s->q_heads + s->k_heads, per_token = (s->q_heads + kBackwardRows - 1) / kBackwardRows;
-  BackwardPlan p{1, 0, 1};
-  if (s->k_heads > 0) p.k_blocks = std::max(1, (int)((int64_t)blocks * s->k_heads / heads));
-  p.q_blocks = blocks - p.k_blocks;
-  double best = 0.0;
-  for (int t = 1; t <= 16; ++t) {
-    if (t > 1 && tokens / t < 4 * p.q_blocks) break;  // (few tokens: a set for every block first)
-    const int steps = (t * per_token + groups - 1) / groups;
-    const double share = (double)t * per_token / ((double)steps * groups);
-    if (share > best + 0.02) {
-      best = share;
-      p.block_tokens = t;
-    }
-  }
-  const int64_t sets = (tokens + p.block_tokens - 1) / p.block_tokens;
-  p.q_blocks = (int)std::min<int64_t>(p.q_blocks, sets);
-  p.k_blocks = (int)std::min<int64_t>(p.k_blocks, sets);
-  return p;
+  const int64_t groups = kThreads / (s->head_dim / 8);
+  const int64_t q = (s->tokens * ((s->q_heads + kBackwardRows - 1) / kBackwardRows) + groups - 1) / groups;
+  const int64_t k = (s->tokens * ((s->k_heads + kBackwardRows - 1) / kBackwardRows) + groups - 1) / groups;
+  const int64_t turns = ((q + k) * s->batch + kSms * 32 - 1) / (kSms * 32);
+  return {(int)((q + turns - 1) / turns), (int)((k + turns - 1) / turns)};
 }
 
 int check(const anemoi_sm100_axial_rope_shape* s) {
@@ -356,14 +428,15 @@ int check(const anemoi_sm100_axial_rope_shape* s) {
     pairs += s->sections[a];
   }
   if (2 * pairs > s->head_dim || pairs % (s->interleaved ? 4 : 8)) return ANEMOI_SM100_EINVAL;
-  if (s->q_heads > 65536 || s->k_heads > 65536 || (s->batch > 0 && s->tokens > 0x7fffffffLL / s->batch))
+  // (a sample's heads are counted in 32 bits, samples by the grid)
+  if (s->q_heads > 4096 || s->k_heads > 4096 || s->batch > 65535 || s->tokens > 0x7fffffffLL / (s->q_heads + s->k_heads))
     return ANEMOI_SM100_ELIMIT;
   return ANEMOI_SM100_OK;
 }
 
 void fill(RopeParams& p, const anemoi_sm100_axial_rope_shape* s, const double* turns, const int64_t* strides, int tensors) {
-  p.batch = s->batch;
-  p.tokens = s->tokens;
+  p.batch = (uint32_t)s->batch;
+  p.tokens = (uint32_t)s->tokens;
   p.q_heads = s->q_heads;
   p.k_heads = s->k_heads;
   p.axes = s->axes;
@@ -371,8 +444,12 @@ void fill(RopeParams& p, const anemoi_sm100_axial_rope_shape* s, const double* t
   p.positions_type = s->positions_type;
   p.eps = s->eps;
   p.pairs = 0;
-  for (int a = 0; a < s->axes; ++a) p.ends[a] = p.pairs += s->sections[a];
-  for (int i = 0; i < p.pairs; ++i) p.turns[i] = turns[i];
+  for (int a = 0; a < 4; ++a) p.ends[a] = p.pairs += a < s->axes ? s->sections[a] : 0;
+  for (int i = 0; i < p.pairs; ++i) {
+    p.rates[i] = turns[i];
+    // (a double below 1 times 2^64 is whole from 2^-11 on, and rounds by less than one below)
+    p.turns[i] = (uint64_t)((turns[i] - floor(turns[i])) * 0x1p64);
+  }
   for (int i = 0; i < tensors; ++i)
     for (int j = 0; j < 3; ++j) p.strides[i][j] = strides[3 * i + j];
 }
@@ -380,26 +457,27 @@ void fill(RopeParams& p, const anemoi_sm100_axial_rope_shape* s, const double* t
 template <typename T, int D, int kRows>
 int forward_launch(const RopeParams& p, cudaStream_t st) {
   constexpr int64_t kGroups = kThreads / (D / 8);
-  const int64_t units = p.batch * p.tokens * ((p.q_heads + kRows - 1) / kRows + (p.k_heads + kRows - 1) / kRows);
-  const int64_t blocks = (units + kGroups - 1) / kGroups;
-  if (blocks > 0x7fffffffLL) return ANEMOI_SM100_ELIMIT;
-  forward_kernel<T, D, kRows><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+  const int64_t units = (int64_t)p.tokens * ((p.q_heads + kRows - 1) / kRows + (p.k_heads + kRows - 1) / kRows);
+  const dim3 grid((unsigned)((units + kGroups - 1) / kGroups), p.batch);
+  auto kernel = p.interleaved ? forward_kernel<T, D, kRows, true> : forward_kernel<T, D, kRows, false>;
+  kernel<<<grid, kThreads, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
 }
 
 template <typename T, int D>
+int forward_rows(const RopeParams& p, int rows, cudaStream_t st) {
+  return rows == 8 ? forward_launch<T, D, 8>(p, st) : rows == 4 ? forward_launch<T, D, 4>(p, st) : forward_launch<T, D, 1>(p, st);
+}
+
+template <typename T, int D>
 int backward_launch(RopeParams& p, const BackwardPlan& plan, void* dq_weight, void* dk_weight, cudaStream_t st) {
-  p.block_tokens = plan.block_tokens;
   p.q_blocks = plan.q_blocks;
-  auto kernel = backward_kernel<T, D>;
-  constexpr int kSmem = kRing * 2 * kBackwardRows * kThreads * 16;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-    return ANEMOI_SM100_ELAUNCH;
-  kernel<<<plan.q_blocks + plan.k_blocks, kThreads, kSmem, st>>>(p);
+  auto kernel = p.interleaved ? backward_kernel<T, D, true> : backward_kernel<T, D, false>;
+  kernel<<<dim3(plan.q_blocks + plan.k_blocks, p.batch), kThreads, 0, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
   if (p.weight_partial == nullptr) return ANEMOI_SM100_OK;
-  sums_kernel<T><<<dim3(D / 32, 2), dim3(32, kSlices), 0, st>>>(p.weight_partial, plan.q_blocks, plan.k_blocks, D, dq_weight,
-                                                                dk_weight);
+  sums_kernel<T><<<dim3(D / 8, 2), kSumThreads, 0, st>>>(p.weight_partial, plan.q_blocks * (int)p.batch,
+                                                         plan.k_blocks * (int)p.batch, D, dq_weight, dk_weight);
   return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
 }
 
@@ -432,15 +510,10 @@ extern "C" int anemoi_sm100_axial_rope(const anemoi_sm100_axial_rope_shape* s, c
   p.k_out = k_out;
   fill(p, s, turns, strides, 4);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool four = rows_of(s) == 4;
-  if (s->is_bf16) {
-    using T = __nv_bfloat16;
-    if (s->head_dim == 64) return four ? forward_launch<T, 64, 4>(p, st) : forward_launch<T, 64, 1>(p, st);
-    return four ? forward_launch<T, 128, 4>(p, st) : forward_launch<T, 128, 1>(p, st);
-  }
-  using T = __half;
-  if (s->head_dim == 64) return four ? forward_launch<T, 64, 4>(p, st) : forward_launch<T, 64, 1>(p, st);
-  return four ? forward_launch<T, 128, 4>(p, st) : forward_launch<T, 128, 1>(p, st);
+  if (s->is_bf16)
+    return s->head_dim == 64 ? forward_rows<__nv_bfloat16, 64>(p, rows_of(s), st)
+                             : forward_rows<__nv_bfloat16, 128>(p, rows_of(s), st);
+  return s->head_dim == 64 ? forward_rows<__half, 64>(p, rows_of(s), st) : forward_rows<__half, 128>(p, rows_of(s), st);
 }
 
 extern "C" int64_t anemoi_sm100_axial_rope_backward_workspace(const anemoi_sm100_axial_rope_shape* s) {
@@ -448,7 +521,7 @@ extern "C" int64_t anemoi_sm100_axial_rope_backward_workspace(const anemoi_sm100
   if (bad != ANEMOI_SM100_OK) return bad;
   if (s->batch == 0 || s->tokens == 0) return 0;
   const BackwardPlan plan = plan_of(s);
-  return (int64_t)(plan.q_blocks + plan.k_blocks) * s->head_dim * (int64_t)sizeof(float);
+  return (int64_t)(plan.q_blocks + plan.k_blocks) * s->batch * s->head_dim * (int64_t)sizeof(float);
 }
 
 extern "C" int anemoi_sm100_axial_rope_backward(const anemoi_sm100_axial_rope_shape* s, const void* dq_out,

@@ -56,15 +56,17 @@ struct BackwardParams {
 // of a thread leave.
 __host__ __device__ constexpr int forward_threads(int vectors, bool wide) { return !wide ? 128 : vectors == 1 ? 1024 : 352; }
 // The gradient holds three column sums per channel in registers, and takes kR rows at a time, so that the chain of a row's
-// sums through the block's barriers is paid once for them.  Wide rows: one piece per thread up to 352 threads, two above; two
-// rows where a thread may have 168 registers (12 warps), one above 352 threads of two pieces.  33,272 rows of 5,376 channels:
+// sums through the block's barriers is paid once for them.  Wide rows: one piece per thread up to 256 threads, of
+// which several blocks share an SM, two above; two rows up to 352 threads (128 and 168 registers), one above.  33,272 rows of 5,376 channels:
 // 672 threads of one piece, one row at a time, spilled at the 80 registers that are left for them, 784 us; 336 threads, one
 // row, copies ahead, 565.
-constexpr int kOnePiece = 352;
-__host__ __device__ constexpr int backward_threads(int rows, bool wide) { return !wide ? 128 : rows == 2 ? kOnePiece : 512; }
+constexpr int kOnePiece = 256, kTwoRows = 352;
+__host__ __device__ constexpr int backward_threads(int vectors, int rows, bool wide) {
+  return !wide ? 128 : vectors == 1 ? kOnePiece : rows == 2 ? kTwoRows : 512;
+}
 // (and blocks per SM that its registers are to leave room for)
 __host__ __device__ constexpr int backward_blocks(int vectors, bool wide) {
-  return wide ? 1 : vectors == 1 ? 5 : vectors == 2 ? 3 : 2;
+  return wide ? (vectors == 1 ? 2 : 1) : vectors == 1 ? 5 : vectors == 2 ? 3 : 2;
 }
 
 // Sums of N values over the threads of a row, in each of them.  Narrow rows: `lanes` lanes of a warp.  Wide rows: the block;
@@ -127,38 +129,41 @@ struct RowSum {
   }
 };
 
-// Normalises v in place; returns the reciprocal root.  Channels that the thread does not have are zeros and stay so.
+__device__ __forceinline__ float sum4(const float2 (&v)[4]) {
+  const float2 s = fadd2(fadd2(v[0], v[1]), fadd2(v[2], v[3]));
+  return s.x + s.y;
+}
+__device__ __forceinline__ float dot4(const float2 (&a)[4], const float2 (&b)[4]) {
+  const float2 s = ffma2(a[0], b[0], fmul2(a[1], b[1])), t = ffma2(a[2], b[2], fmul2(a[3], b[3]));
+  return (s.x + s.y) + (t.x + t.y);
+}
+
+// Normalises v in place.  Channels that the thread does not have are zeros and stay so.
 template <int V, bool kWide>
-__device__ __forceinline__ float normalise(float (&v)[V][8], const bool (&has)[V], int kind, int width, float eps,
-                                           RowSum<kWide>& sum) {
+__device__ __forceinline__ void normalise(float2 (&v)[V][4], const bool (&has)[V], int kind, int width, float eps,
+                                          RowSum<kWide>& sum) {
   const float inv = 1.0f / (float)width;
+  float all[1];
   if (kind == kLayer) {
-    float s = 0.0f;
+    all[0] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[j][i];
-    float all[1] = {s};
+    for (int j = 0; j < V; ++j) all[0] += sum4(v[j]);
     sum(all);
-    const float mean = all[0] * inv;
+    const float2 mean = both(-all[0] * inv);
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = has[j] ? v[j][i] - mean : 0.0f;
+      for (int i = 0; i < 4; ++i) v[j][i] = has[j] ? fadd2(v[j][i], mean) : both(0.0f);
   }
-  float s = 0.0f;
+  all[0] = 0.0f;
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s = fmaf(v[j][i], v[j][i], s);
-  float all[1] = {s};
+  for (int j = 0; j < V; ++j) all[0] += dot4(v[j], v[j]);
   sum(all);
-  const float r = rsqrtf(fmaf(all[0], inv, eps));
+  const float2 r = both(rsqrtf(fmaf(all[0], inv, eps)));
 #pragma unroll
   for (int j = 0; j < V; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[j][i] *= r;
-  return r;
+    for (int i = 0; i < 4; ++i) v[j][i] = fmul2(v[j][i], r);
 }
 
 // One row per `lanes` threads.  HBM bound: 2 C bytes of each of x, y in, x', h out.
@@ -183,29 +188,28 @@ __global__ void __launch_bounds__(forward_threads(V, kWide)) forward_kernel(cons
       if (p.y != nullptr) yr[j] = load_stream(static_cast<const T*>(p.y) + row * p.y_stride + at[j]);
     }
   }
-  const int64_t group = quotient(row, p.per_group);
-  float x[V][8];
+  const int64_t group = p.per_group == p.rows ? 0 : quotient(row, p.per_group);
+  float2 x[V][4];
 #pragma unroll
   for (int j = 0; j < V; ++j) open8<T>(xr[j], x[j]);
   if (p.y != nullptr) {
-    float y[V][8];
+    float2 y[V][4];
 #pragma unroll
     for (int j = 0; j < V; ++j) open8<T>(yr[j], y[j]);
     if (p.post != kNone) normalise<V, kWide>(y, has, p.post, p.width, p.eps, sum);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       if (!has[j]) continue;
+      float2 f[4];
       if (p.post_weight != nullptr) {
-        float w[8];
-        shared8(static_cast<const T*>(p.post_weight) + at[j], w);
+        shared8(static_cast<const T*>(p.post_weight) + at[j], f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[j][i] *= w[i];
+        for (int i = 0; i < 4; ++i) y[j][i] = fmul2(y[j][i], f[i]);
       }
-      float g[8];
-      shared8(static_cast<const M*>(p.gate) + group * p.gate_stride + at[j], g);
+      shared8(static_cast<const M*>(p.gate) + group * p.gate_stride + at[j], f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = fmaf(g[i], y[j][i], x[j][i]);
-      if (live) *reinterpret_cast<uint4*>(static_cast<T*>(p.x_out) + row * p.width + at[j]) = round8<T>(x[j]);
+      for (int i = 0; i < 4; ++i) x[j][i] = ffma2(f[i], y[j][i], x[j][i]);
+      if (live) store8(static_cast<T*>(p.x_out) + row * p.width + at[j], x[j]);
     }
   }
   if (p.h_out == nullptr) return;
@@ -213,23 +217,23 @@ __global__ void __launch_bounds__(forward_threads(V, kWide)) forward_kernel(cons
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     if (!has[j]) continue;
-    float f[8];
+    float2 f[4];
     if (p.weight != nullptr) {
       shared8(static_cast<const T*>(p.weight) + at[j], f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] *= f[i];
+      for (int i = 0; i < 4; ++i) x[j][i] = fmul2(x[j][i], f[i]);
     }
     if (p.scale != nullptr) {
       shared8(static_cast<const M*>(p.scale) + group * p.scale_stride + at[j], f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = fmaf(x[j][i], f[i], x[j][i]);
+      for (int i = 0; i < 4; ++i) x[j][i] = ffma2(x[j][i], f[i], x[j][i]);
     }
     if (p.shift != nullptr) {
       shared8(static_cast<const M*>(p.shift) + group * p.shift_stride + at[j], f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] += f[i];
+      for (int i = 0; i < 4; ++i) x[j][i] = fadd2(x[j][i], f[i]);
     }
-    if (live) *reinterpret_cast<uint4*>(static_cast<T*>(p.h_out) + row * p.width + at[j]) = round8<T>(x[j]);
+    if (live) store8(static_cast<T*>(p.h_out) + row * p.width + at[j], x[j]);
   }
 }
 
@@ -240,8 +244,9 @@ struct NormGradient {
   float r, along, mean;
 };
 template <int V, int kR, bool kWide>
-__device__ __forceinline__ void gradient_of_norm(float (&v)[kR][V][8], const float (&g)[kR][V][8], const bool (&has)[V],
-                                                 int kind, int width, float eps, RowSum<kWide>& sum, NormGradient (&n)[kR]) {
+__device__ __forceinline__ void gradient_of_norm(float2 (&v)[kR][V][4], const float2 (&g)[kR][V][4], const bool (&has)[V],
+                                                 int kind, int width, float eps, int rows_in, RowSum<kWide>& sum,
+                                                 NormGradient (&n)[kR]) {
   const float inv = 1.0f / (float)width;
   float s[2 * kR];
   if (kind == kLayer) {
@@ -249,21 +254,20 @@ __device__ __forceinline__ void gradient_of_norm(float (&v)[kR][V][8], const flo
     for (int k = 0; k < kR; ++k) {
       s[2 * k] = s[2 * k + 1] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          s[2 * k] += v[k][j][i];
-          s[2 * k + 1] += g[k][j][i];
-        }
+      for (int j = 0; j < V; ++j) {
+        s[2 * k] += sum4(v[k][j]);
+        s[2 * k + 1] += sum4(g[k][j]);
+      }
     }
     sum(s);
 #pragma unroll
     for (int k = 0; k < kR; ++k) {
       n[k].mean = s[2 * k + 1] * inv;
+      const float2 mean = both(-s[2 * k] * inv);
 #pragma unroll
       for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][j][i] = has[j] ? v[k][j][i] - s[2 * k] * inv : 0.0f;
+        for (int i = 0; i < 4; ++i) v[k][j][i] = has[j] ? fadd2(v[k][j][i], mean) : both(0.0f);
     }
   } else {
 #pragma unroll
@@ -273,22 +277,22 @@ __device__ __forceinline__ void gradient_of_norm(float (&v)[kR][V][8], const flo
   for (int k = 0; k < kR; ++k) {
     s[2 * k] = s[2 * k + 1] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s[2 * k] = fmaf(v[k][j][i], v[k][j][i], s[2 * k]);
-        s[2 * k + 1] = fmaf(g[k][j][i], v[k][j][i], s[2 * k + 1]);
-      }
+    for (int j = 0; j < V; ++j) {
+      s[2 * k] += dot4(v[k][j], v[k][j]);
+      s[2 * k + 1] += dot4(g[k][j], v[k][j]);
+    }
   }
   sum(s);
 #pragma unroll
   for (int k = 0; k < kR; ++k) {
-    n[k].r = rsqrtf(fmaf(s[2 * k], inv, eps));
+    // (rows that do not exist are zeros, and stay so with eps = 0)
+    n[k].r = k < rows_in ? rsqrtf(fmaf(s[2 * k], inv, eps)) : 0.0f;
     n[k].along = s[2 * k + 1] * n[k].r * inv;
+    const float2 r = both(n[k].r);
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][j][i] *= n[k].r;
+      for (int i = 0; i < 4; ++i) v[k][j][i] = fmul2(v[k][j][i], r);
   }
 }
 
@@ -301,7 +305,7 @@ __device__ __forceinline__ void gradient_of_norm(float (&v)[kR][V][8], const flo
 // steps of kR rows of each array, a thread's own channels, no registers held): at 5,376 channels two rows, 86 KB per SM, are on
 // their way, where HBM's latency asks for 45.
 template <typename T, typename M, int V, int kR, bool kWide, int kStages>
-__global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V, kWide)) backward_kernel(
+__global__ void __launch_bounds__(backward_threads(V, kR, kWide), backward_blocks(V, kWide)) backward_kernel(
     const __grid_constant__ BackwardParams p, int lanes) {
   extern __shared__ __align__(16) uint8_t shared[];
   __shared__ __align__(16) float buffer[kBuffer];
@@ -360,32 +364,43 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
     }
     return s;
   };
-  // the copies run kStages - 1 steps ahead, into the next segments, too
-  Segment ahead = segment_of(0);
+  // the copies run kStages - 1 steps ahead, into the next segments, too; rows that a segment does not have come as zeros
   int64_t ahead_turn = 0;
-  int ahead_step = 0, ahead_stage = 0;
+  int ahead_step = 0, ahead_stage = 0, ahead_count = 0;
+  const T *x_at, *dh_at, *dx_at, *y_at;
+  auto copies_from = [&](const Segment& s) {
+    ahead_count = s.count;
+    x_at = static_cast<const T*>(p.x) + s.first * p.x_stride + lane * 8;
+    dh_at = static_cast<const T*>(p.dh) + s.first * p.dh_stride + lane * 8;
+    dx_at = static_cast<const T*>(p.dx_out) + s.first * p.dx_out_stride + lane * 8;
+    y_at = static_cast<const T*>(p.y) + s.first * p.y_stride + lane * 8;
+  };
+  copies_from(segment_of(0));
+  const int step_of_at = lanes * 8;
   auto copy_next = [&]() {
+    uint4* to = ring + ahead_stage * step_of_stage;
 #pragma unroll
     for (int k = 0; k < kR; ++k) {
-      const int n = ahead_step * kR + k;
-      if (ahead_turn >= turns || n >= ahead.count) continue;
-      const int64_t row = ahead.first + n;
-      uint4* to = ring + ahead_stage * step_of_stage;
+      const uint32_t bytes = ahead_step * kR + k < ahead_count ? 16u : 0u;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if (!has[j]) continue;
-        copy_async16(to + place(kX, k, j), static_cast<const T*>(p.x) + row * p.x_stride + at[j]);
-        if (p.dh != nullptr) copy_async16(to + place(kDh, k, j), static_cast<const T*>(p.dh) + row * p.dh_stride + at[j]);
-        if (p.dx_out != nullptr)
-          copy_async16(to + place(kDx, k, j), static_cast<const T*>(p.dx_out) + row * p.dx_out_stride + at[j]);
-        if (p.y != nullptr) copy_async16(to + place(kY, k, j), static_cast<const T*>(p.y) + row * p.y_stride + at[j]);
+        copy_async16(to + place(kX, k, j), x_at + j * step_of_at, bytes);
+        if (p.dh != nullptr) copy_async16(to + place(kDh, k, j), dh_at + j * step_of_at, bytes);
+        if (p.dx_out != nullptr) copy_async16(to + place(kDx, k, j), dx_at + j * step_of_at, bytes);
+        if (p.y != nullptr) copy_async16(to + place(kY, k, j), y_at + j * step_of_at, bytes);
       }
+      x_at += p.x_stride;
+      dh_at += p.dh_stride;
+      dx_at += p.dx_out_stride;
+      y_at += p.y_stride;
     }
     copy_commit();
     ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
     if (++ahead_step == steps) {
       ahead_step = 0;
-      if (++ahead_turn < turns) ahead = segment_of(ahead_turn);
+      // (behind the last segment: an empty one)
+      copies_from(segment_of(++ahead_turn));
     }
   };
 #pragma unroll
@@ -396,7 +411,11 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
     const int64_t group = seg.group;
     const M* gates = static_cast<const M*>(p.gate) + group * p.gate_stride;
     const M* scales = static_cast<const M*>(p.scale) + group * p.scale_stride;
-    float a_sum[V][8] = {}, s_sum[V][8] = {}, b_sum[V][8] = {};
+    float2 a_sum[V][4], s_sum[V][4], b_sum[V][4];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a_sum[j][i] = s_sum[j][i] = b_sum[j][i] = both(0.0f);
 #pragma unroll 1
     for (int step = 0; step < steps; ++step) {
       // (into the place that was read in the step before, by this thread alone)
@@ -405,28 +424,26 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
       const uint4* from = ring + stage * step_of_stage;
       stage = stage + 1 == kStages ? 0 : stage + 1;
       const int rows_in = seg.count - step * kR;  // rows k < rows_in exist
-      auto read = [&](int array, int k, int j, float(&f)[8]) {
-        open8<T>(k < rows_in ? from[place(array, k, j)] : make_uint4(0, 0, 0, 0), f);
+      auto read = [&](int array, int k, int j, float2(&f)[4]) {
+        open8<T>(from[place(array, k, j)], f);
       };
-      float dx[kR][V][8];
+      float2 dx[kR][V][4];
       if (p.dh != nullptr) {
-        float x[kR][V][8], g[kR][V][8];
+        float2 x[kR][V][4], g[kR][V][4];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = 1.0f;
+          float2 f[4] = {both(1.0f), both(1.0f), both(1.0f), both(1.0f)};
           if (has[j]) {
             if (p.scale != nullptr) {
               shared8(scales + at[j], f);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] += 1.0f;
+              for (int i = 0; i < 4; ++i) f[i] = fadd2(f[i], both(1.0f));
             }
             if (p.weight != nullptr) {
-              float w[8];
+              float2 w[4];
               shared8(static_cast<const T*>(p.weight) + at[j], w);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] *= w[i];
+              for (int i = 0; i < 4; ++i) f[i] = fmul2(f[i], w[i]);
             }
           }
 #pragma unroll
@@ -434,27 +451,29 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
             read(kX, k, j, x[k][j]);
             read(kDh, k, j, g[k][j]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              s_sum[j][i] += g[k][j][i];
-              g[k][j][i] *= f[i];
+            for (int i = 0; i < 4; ++i) {
+              s_sum[j][i] = fadd2(s_sum[j][i], g[k][j][i]);
+              g[k][j][i] = fmul2(g[k][j][i], f[i]);
             }
           }
         }
         NormGradient n[kR];
-        gradient_of_norm<V, kR, kWide>(x, g, has, p.norm, p.width, p.eps, sum, n);
+        gradient_of_norm<V, kR, kWide>(x, g, has, p.norm, p.width, p.eps, rows_in, sum, n);
 #pragma unroll
-        for (int k = 0; k < kR; ++k)
+        for (int k = 0; k < kR; ++k) {
+          const float2 r = both(n[k].r), along = both(-n[k].along), mean = both(-n[k].mean);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            float d[8];
+            float2 d[4];
             read(kDh, k, j, d);
             read(kDx, k, j, dx[k][j]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              a_sum[j][i] = fmaf(d[i], x[k][j][i], a_sum[j][i]);
-              dx[k][j][i] = fmaf(n[k].r, g[k][j][i] - fmaf(x[k][j][i], n[k].along, n[k].mean), dx[k][j][i]);
+            for (int i = 0; i < 4; ++i) {
+              a_sum[j][i] = ffma2(d[i], x[k][j][i], a_sum[j][i]);
+              dx[k][j][i] = ffma2(r, fadd2(ffma2(x[k][j][i], along, g[k][j][i]), mean), dx[k][j][i]);
             }
           }
+        }
       } else {
 #pragma unroll
         for (int k = 0; k < kR; ++k)
@@ -466,15 +485,11 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
       for (int k = 0; k < kR; ++k)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          if (k < rows_in && has[j]) {
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.dx) + (row + k) * p.width + at[j]) = round8<T>(dx[k][j]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dx[k][j][i] = 0.0f;
-          }
+          if (k < rows_in && has[j]) store8(static_cast<T*>(p.dx) + (row + k) * p.width + at[j], dx[k][j]);
         }
       if (p.y == nullptr) continue;
-      float y[kR][V][8];
+      // (B takes dx as it stands, dy takes it times gate and weight)
+      float2 y[kR][V][4];
 #pragma unroll
       for (int k = 0; k < kR; ++k)
 #pragma unroll
@@ -482,71 +497,70 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
       if (p.post == kNone) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          float f[8] = {};
+          float2 f[4] = {};
           if (has[j]) shared8(gates + at[j], f);
 #pragma unroll
           for (int k = 0; k < kR; ++k) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              b_sum[j][i] = fmaf(dx[k][j][i], y[k][j][i], b_sum[j][i]);
-              dx[k][j][i] *= f[i];
+            for (int i = 0; i < 4; ++i) {
+              b_sum[j][i] = ffma2(dx[k][j][i], y[k][j][i], b_sum[j][i]);
+              dx[k][j][i] = fmul2(dx[k][j][i], f[i]);
             }
-            if (k < rows_in && has[j])
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.dy) + (row + k) * p.width + at[j]) = round8<T>(dx[k][j]);
+            if (k < rows_in && has[j]) store8(static_cast<T*>(p.dy) + (row + k) * p.width + at[j], dx[k][j]);
           }
         }
         continue;
       }
-      // B takes dx before the gate: its sums over this step are formed with the normalised y, from dx = u / (gate * weight),
-      // which may be a division by zero, so both are kept
-      float u[kR][V][8];
+      float2 u[kR][V][4];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float f[8] = {};
+        float2 f[4] = {};
         if (has[j]) {
           shared8(gates + at[j], f);
           if (p.post_weight != nullptr) {
-            float w[8];
+            float2 w[4];
             shared8(static_cast<const T*>(p.post_weight) + at[j], w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] *= w[i];
+            for (int i = 0; i < 4; ++i) f[i] = fmul2(f[i], w[i]);
           }
         }
 #pragma unroll
         for (int k = 0; k < kR; ++k)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) u[k][j][i] = dx[k][j][i] * f[i];
+          for (int i = 0; i < 4; ++i) u[k][j][i] = fmul2(dx[k][j][i], f[i]);
       }
       NormGradient n[kR];
-      gradient_of_norm<V, kR, kWide>(y, u, has, p.post, p.width, p.eps, sum, n);
+      gradient_of_norm<V, kR, kWide>(y, u, has, p.post, p.width, p.eps, rows_in, sum, n);
 #pragma unroll
-      for (int k = 0; k < kR; ++k)
+      for (int k = 0; k < kR; ++k) {
+        const float2 r = both(n[k].r), along = both(-n[k].along), mean = both(-n[k].mean);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            b_sum[j][i] = fmaf(dx[k][j][i], y[k][j][i], b_sum[j][i]);
-            u[k][j][i] = n[k].r * (u[k][j][i] - fmaf(y[k][j][i], n[k].along, n[k].mean));
+          for (int i = 0; i < 4; ++i) {
+            b_sum[j][i] = ffma2(dx[k][j][i], y[k][j][i], b_sum[j][i]);
+            u[k][j][i] = fmul2(r, fadd2(ffma2(y[k][j][i], along, u[k][j][i]), mean));
           }
-          if (k < rows_in && has[j])
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.dy) + (row + k) * p.width + at[j]) = round8<T>(u[k][j]);
+          if (k < rows_in && has[j]) store8(static_cast<T*>(p.dy) + (row + k) * p.width + at[j], u[k][j]);
         }
+      }
     }
     if (seg.count == 0) continue;
     const int64_t segment = turn * p.workers + worker;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       if (!has[j]) continue;
-      float f[8];
+      float2 f[4] = {};
       if (weights) {
-        float* mine = own + at[j];
+        float2* mine = reinterpret_cast<float2*>(own + at[j]);
         if (p.scale != nullptr) shared8(scales + at[j], f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mine[i] += p.scale != nullptr ? fmaf(a_sum[j][i], f[i], a_sum[j][i]) : a_sum[j][i];
+        for (int i = 0; i < 4; ++i) mine[i] = fadd2(mine[i], ffma2(a_sum[j][i], f[i], a_sum[j][i]));
         if (p.y != nullptr) {
           shared8(gates + at[j], f);
+          mine += V * lanes * 4;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mine[V * lanes * 8 + i] = fmaf(b_sum[j][i], f[i], mine[V * lanes * 8 + i]);
+          for (int i = 0; i < 4; ++i) mine[i] = ffma2(b_sum[j][i], f[i], mine[i]);
         }
       }
       if (p.per_group_segments > 1) {
@@ -562,7 +576,7 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
         if (p.weight != nullptr) {
           shared8(static_cast<const T*>(p.weight) + at[j], f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) a_sum[j][i] *= f[i];
+          for (int i = 0; i < 4; ++i) a_sum[j][i] = fmul2(a_sum[j][i], f[i]);
         }
         store8(static_cast<M*>(p.dscale) + out, a_sum[j]);
       }
@@ -570,7 +584,7 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
         if (p.post_weight != nullptr) {
           shared8(static_cast<const T*>(p.post_weight) + at[j], f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) b_sum[j][i] *= f[i];
+          for (int i = 0; i < 4; ++i) b_sum[j][i] = fmul2(b_sum[j][i], f[i]);
         }
         store8(static_cast<M*>(p.dgate) + out, b_sum[j]);
       }
@@ -591,6 +605,7 @@ __global__ void __launch_bounds__(backward_threads(kR, kWide), backward_blocks(V
       }
 }
 
+constexpr int kSumThreads = 256;
 struct SumsParams {
   const float *partial, *weight_partial;
   const void *weight, *post_weight;
@@ -599,31 +614,32 @@ struct SumsParams {
   int per_group_segments, workers, width;
 };
 
-// blockIdx.y: the groups' A, S, B sums (where groups have several segments), then the two weights' sums.
+// First the groups' A, S, B sums (where groups have several segments), then the two weights' sums.
 template <typename T, typename M>
-__global__ void sums_kernel(const __grid_constant__ SumsParams p) {
-  const int column = blockIdx.x * 32 + threadIdx.x;
-  const bool in = column < p.width;
-  const int64_t job = blockIdx.y + (int64_t)blockIdx.z * 32768;
-  const int64_t group_jobs = p.per_group_segments > 1 ? p.groups * 3 : 0;
-  if (job < group_jobs) {
-    const int64_t group = job / 3;
-    const int which = (int)(job - group * 3);
+__global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant__ SumsParams p) {
+  const int group_across = sum_columns(p.per_group_segments), weight_across = sum_columns(p.workers);
+  const uint32_t each = ((uint32_t)p.width + group_across - 1) / group_across;
+  const uint32_t group_blocks = p.per_group_segments > 1 ? (uint32_t)p.groups * 3 * each : 0;
+  if (blockIdx.x < group_blocks) {
+    const uint32_t job = blockIdx.x / each, group = job / 3, which = job - group * 3, first = (blockIdx.x - job * each) * group_across;
     void* out = which == 0 ? p.dscale : which == 1 ? p.dshift : p.dgate;
     if (out == nullptr) return;
-    float v = column_sum(p.partial + (group * p.per_group_segments * 3 + which) * p.width, 3 * (int64_t)p.width,
-                         p.per_group_segments, column, in);
-    if (threadIdx.y != 0 || !in) return;
+    float v = column_sum<kSumThreads>(p.partial + ((int64_t)group * p.per_group_segments * 3 + which) * p.width, 3 * (int64_t)p.width,
+                         p.per_group_segments, first, p.width);
+    const int column = first + threadIdx.x;
+    if (threadIdx.x >= group_across || column >= p.width) return;
     const void* w = which == 0 ? p.weight : which == 2 ? p.post_weight : nullptr;
     if (w != nullptr) v *= load1(static_cast<const T*>(w) + column);
-    store1(static_cast<M*>(out) + group * p.width + column, v);
+    store1(static_cast<M*>(out) + (int64_t)group * p.width + column, v);
     return;
   }
-  const int which = (int)(job - group_jobs);
-  void* out = which == 0 ? p.dweight : which == 1 ? p.dpost_weight : nullptr;
+  const uint32_t narrow = ((uint32_t)p.width + weight_across - 1) / weight_across, at = blockIdx.x - group_blocks;
+  const uint32_t which = at / narrow, first = (at - which * narrow) * weight_across;
+  void* out = which == 0 ? p.dweight : p.dpost_weight;
   if (out == nullptr) return;
-  const float v = column_sum(p.weight_partial + (int64_t)which * p.width, 2 * (int64_t)p.width, p.workers, column, in);
-  if (threadIdx.y == 0 && in) store1(static_cast<T*>(out) + column, v);
+  const float v = column_sum<kSumThreads>(p.weight_partial + (int64_t)which * p.width, 2 * (int64_t)p.width, p.workers, first, p.width);
+  const int column = first + threadIdx.x;
+  if (threadIdx.x < weight_across && column < p.width) store1(static_cast<T*>(out) + column, v);
 }
 
 // How a row lies on threads: `lanes` threads of `vectors` pieces of 8 channels each.
@@ -685,10 +701,10 @@ Split split_of(const RowShape& s, int64_t rows, int64_t groups, int blocks_per_s
   return out;
 }
 
-// Blocks per SM: 12 warps at 168 registers, 16 at 128.
+// Blocks per SM: 16 warps at 128 registers, 12 at 168.
 int backward_blocks_per_sm(const RowShape& s) {
   if (!s.wide) return backward_blocks(s.vectors, false);
-  return std::max(1, (s.threads > kOnePiece ? 16 : 12) / ((s.threads + 31) / 32));
+  return std::max(1, (s.vectors == 1 || s.threads > kTwoRows ? 16 : 12) / ((s.threads + 31) / 32));
 }
 
 template <typename T, typename M, int V, bool kWide>
@@ -735,14 +751,15 @@ int backward_typed(const BackwardParams& p, const SumsParams& q, const RowShape&
   else if (s.vectors == 1)
     code = backward_launch<T, M, 1, 2, true, 2>(p, s, split, st);
   else
-    code = s.threads <= kOnePiece ? backward_launch<T, M, 2, 2, true, 2>(p, s, split, st)
+    code = s.threads <= kTwoRows ? backward_launch<T, M, 2, 2, true, 2>(p, s, split, st)
                                   : backward_launch<T, M, 2, 1, true, 2>(p, s, split, st);
   if (code != ANEMOI_SM100_OK) return code;
-  const int64_t jobs = (split.per_group_segments > 1 ? 3 * q.groups : 0) + (q.weight_partial != nullptr ? 2 : 0);
-  if (jobs == 0) return ANEMOI_SM100_OK;
-  const dim3 grid((unsigned)((q.width + 31) / 32), (unsigned)std::min<int64_t>(jobs, 32768),
-                  (unsigned)((jobs + 32767) / 32768));
-  sums_kernel<T, M><<<grid, dim3(32, kSlices), 0, st>>>(q);
+  const int64_t each = (q.width + sum_columns(split.per_group_segments) - 1) / sum_columns(split.per_group_segments);
+  const int64_t narrow = (q.width + sum_columns(split.workers) - 1) / sum_columns(split.workers);
+  const int64_t grid = (split.per_group_segments > 1 ? 3 * q.groups * each : 0) + (q.weight_partial != nullptr ? 2 * narrow : 0);
+  if (grid == 0) return ANEMOI_SM100_OK;
+  if (grid > 0x7fffffffLL) return ANEMOI_SM100_ELIMIT;
+  sums_kernel<T, M><<<(unsigned)grid, kSumThreads, 0, st>>>(q);
   return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
 }
 

@@ -6,7 +6,15 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "packed.cuh"
+
 namespace rows {
+
+using sm100::fadd2;
+using sm100::ffma2;
+using sm100::fmul2;
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 constexpr int kSms = 148;
 
@@ -19,11 +27,34 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {
   return v;
 }
 
+__device__ __forceinline__ uint2 load_stream8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
 // The same into shared memory, without registers: per thread, in groups that complete in order.  (A thread reads back what
 // it copied itself, so that no barrier is needed.)
 __device__ __forceinline__ void copy_async16(void* smem, const void* p) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
                "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async8(void* smem, const void* p) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(smem))), "l"(p)
+               : "memory");
+}
+// `bytes` = 0: zeros, and nothing is read.
+__device__ __forceinline__ void copy_async16(void* smem, const void* p, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
+               "l"(p), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async8(void* smem, const void* p, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
+               "l"(p), "r"(bytes)
                : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -74,6 +105,20 @@ __device__ __forceinline__ uint4 round8(const float (&f)[8]) {
                     Pair<T>::round(f[6], f[7]));
 }
 
+// The same as four packed pairs (packed.cuh).
+template <typename T>
+__device__ __forceinline__ void open8(const uint4& raw, float2 (&f)[4]) {
+  f[0] = Pair<T>::open(raw.x);
+  f[1] = Pair<T>::open(raw.y);
+  f[2] = Pair<T>::open(raw.z);
+  f[3] = Pair<T>::open(raw.w);
+}
+template <typename T>
+__device__ __forceinline__ uint4 round8(const float2 (&f)[4]) {
+  return make_uint4(Pair<T>::round(f[0].x, f[0].y), Pair<T>::round(f[1].x, f[1].y), Pair<T>::round(f[2].x, f[2].y),
+                    Pair<T>::round(f[3].x, f[3].y));
+}
+
 // 8 values that many rows share, in 16 or 32 bits.
 template <typename M>
 __device__ __forceinline__ void shared8(const M* p, float (&f)[8]) {
@@ -83,6 +128,27 @@ template <>
 __device__ __forceinline__ void shared8<float>(const float* p, float (&f)[8]) {
   *reinterpret_cast<float4*>(f) = __ldg(reinterpret_cast<const float4*>(p));
   *reinterpret_cast<float4*>(f + 4) = __ldg(reinterpret_cast<const float4*>(p) + 1);
+}
+template <typename M>
+__device__ __forceinline__ void shared8(const M* p, float2 (&f)[4]) {
+  open8<M>(__ldg(reinterpret_cast<const uint4*>(p)), f);
+}
+template <>
+__device__ __forceinline__ void shared8<float>(const float* p, float2 (&f)[4]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  f[0] = make_float2(a.x, a.y);
+  f[1] = make_float2(a.z, a.w);
+  f[2] = make_float2(b.x, b.y);
+  f[3] = make_float2(b.z, b.w);
+}
+template <typename M>
+__device__ __forceinline__ void store8(M* p, const float2 (&f)[4]) {
+  *reinterpret_cast<uint4*>(p) = round8<M>(f);
+}
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float2 (&f)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
 }
 template <typename M>
 __device__ __forceinline__ void store8(M* p, const float (&f)[8]) {
@@ -122,23 +188,28 @@ __device__ __forceinline__ float load1<__nv_bfloat16>(const __nv_bfloat16* p) {
   return __bfloat162float(*p);
 }
 
-// Sum of `parts` rows of `columns` fp32 partial sums, `stride` values apart, by a block of 32 x kSlices threads: slice y
-// takes the parts y, y + kSlices, ..., the slices are added in order.  The order depends on `parts` alone, so that equal
-// calls give equal bits.  Thread (x, 0) returns the sum of column `column`.
-constexpr int kSlices = 16;
-__device__ __forceinline__ float column_sum(const float* partial, int64_t stride, int parts, int column, bool in) {
-  __shared__ float part[kSlices][33];
+// Sum of a column of `parts` fp32 partial sums, `stride` values apart, by a block of kThreads threads: `across` neighbouring
+// columns (32, or 8 where parts are many: a 32-byte sector), kThreads / across slices of the parts, added in order.  The
+// order depends on `parts` alone, so that equal calls give equal bits.  Threads below `across` return the sum of column
+// `first + threadIdx.x`, others nothing of use.
+__host__ __device__ constexpr int sum_columns(int parts) { return parts > 256 ? 8 : 32; }
+template <int kThreads>
+__device__ __forceinline__ float column_sum(const float* partial, int64_t stride, int parts, int first, int columns) {
+  __shared__ float part[kThreads];
+  const int across = sum_columns(parts), slices = kThreads / across;
+  const int x = threadIdx.x % across, y = threadIdx.x / across;
   float sum = 0.0f;
-  if (in) {
-#pragma unroll 4
-    for (int i = threadIdx.y; i < parts; i += kSlices) sum += partial[(int64_t)i * stride + column];
+  if (first + x < columns) {
+    const float* at = partial + first + x + (int64_t)y * stride;
+#pragma unroll 8
+    for (int i = y; i < parts; i += slices, at += slices * stride) sum += *at;
   }
-  part[threadIdx.y][threadIdx.x] = sum;
+  part[threadIdx.x] = sum;
   __syncthreads();
   float total = 0.0f;
-  if (threadIdx.y == 0)
-#pragma unroll
-    for (int y = 0; y < kSlices; ++y) total += part[y][threadIdx.x];
+  if (y == 0)
+#pragma unroll 8
+    for (int i = 0; i < slices; ++i) total += part[i * across + x];
   return total;
 }
 
