@@ -80,11 +80,13 @@ struct Span {
   }
 };
 
-// The lane's 4 pairs' cosines and sines; 1 and 0 where its channels do not turn.
-__device__ __forceinline__ void load_angles(const float* row, int lane, const Span& span, int pairs, float4& c, float4& s) {
+// The lane's 4 pairs' cosines and sines; 1 and 0 where its channels do not turn, or for a token that does not exist (whose
+// place in the table nobody has written).
+__device__ __forceinline__ void load_angles(const float* row, int lane, const Span& span, bool exists, int pairs, float4& c,
+                                            float4& s) {
   c = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
   s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (span.in) {
+  if (span.in && exists) {
     c = *reinterpret_cast<const float4*>(row + 4 * lane);
     s = *reinterpret_cast<const float4*>(row + pairs + 4 * lane);
   }
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, forward_blocks(kRows)) forward_kerne
   }
   __syncwarp();
   float4 c4, s4;
-  load_angles(table + 2 * u.t * p.pairs, lane, span, p.pairs, c4, s4);
+  load_angles(table + 2 * u.t * p.pairs, lane, span, heads > 0, p.pairs, c4, s4);
   const float2 c[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
   const float2 s[2] = {make_float2(s4.x, s4.y), make_float2(s4.z, s4.w)};
   float2 uc[2], us[2], vc[2], vs[2];
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 3) backward_kernel(const __grid_cons
     warp_angles<kUnits>(p, u, per_token, table);
     __syncwarp();
     float4 c4, s4;
-    load_angles(table + 2 * u.t * p.pairs, lane, span, p.pairs, c4, s4);
+    load_angles(table + 2 * u.t * p.pairs, lane, span, heads > 0, p.pairs, c4, s4);
     const float2 c[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
     const float2 s[2] = {make_float2(s4.x, s4.y), make_float2(s4.z, s4.w)};
     const float2 minus_s[2] = {negative(s[0]), negative(s[1])};
