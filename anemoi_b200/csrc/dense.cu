@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/anemoi_sm100.h"
 #include "bounded_wait.cuh"
@@ -62,12 +63,13 @@ struct BackwardParams {
   CUtensorMap q, k, v, dout;
   Geometry g;                  // (splits: of the key tiles' queries)
   const void *q_rows, *do_rows;
-  const float *lse2, *delta;   // [B][H][q_tokens]
+  const float *lse, *delta;    // [B][H][q_tokens]
+  float* few_parts;            // [few key tiles][B][H][q_tokens], where query tiles may see few keys (few_kernel)
   const uint32_t* norms;       // fp16: largest |dO_i|^2 and |v_j|^2 per (sample, key head)
   void *dq, *dk, *dv;
   float *q_partial, *k_partial;  // with splits: [splits][B][H][q_tokens][D]; [splits][dV, dK][B][Hk][k_tokens][D]
   Strides sq, sdo, sdq, sdk, sdv;
-  int q_splits, key_tiles, query_tiles, key_ctas;
+  int q_splits, key_tiles, query_tiles, key_ctas, few_splits;
 };
 
 __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int tokens) {
@@ -78,6 +80,29 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^x for two values without the special-function unit, for x > -126 (below: 2^-126): the nearest whole number by adding
+// 1.5 * 2^23, and a minimax polynomial of degree 4 of the rest, 2^-18.5 relative (fitted for |f| <= 1/2 by exchange).  Some of
+// the exponentials go this way, as that unit (16 per cycle and SM) is what the softmax steps wait for.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);
+  const float2 n = fadd2(x, magic), whole = fadd2(n, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = ffma2(whole, make_float2(-1.0f, -1.0f), x);
+  float2 p = ffma2(make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f), f, make_float2(0x1.ca144p-5f, 0x1.ca144p-5f));
+  p = ffma2(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = ffma2(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = ffma2(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(n.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(n.y) << 23)));
+}
+// Two of 2^x; pair `j` of a row goes to the polynomial once in kPolyEvery (a constant once the loop is unrolled).
+template <int kPolyEvery>
+__device__ __forceinline__ float2 exp2_pair(float2 x, int j) {
+  if (kPolyEvery > 0 && j % (kPolyEvery > 0 ? kPolyEvery : 1) == kPolyEvery - 1) return exp2_poly(x);
+  return make_float2(exp2_approx(x.x), exp2_approx(x.y));
 }
 
 __device__ __forceinline__ bool elect_one() {
@@ -106,6 +131,16 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
   mbar_arrive_expect_tx(bar, kTileBytes<D>);
 #pragma unroll
   for (int c = 0; c < D; c += 64) tensor_g2s(dst + c * (kTile * 2), map, c, head, token, batch, bar);
+}
+
+// One thread: the same tile into L2 only.
+template <int D>
+__device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int head, int token, int batch) {
+#pragma unroll
+  for (int c = 0; c < D; c += 64)
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c), "r"(head),
+                 "r"(token), "r"(batch)
+                 : "memory");
 }
 
 // A warp: a tile of which only the first `valid` rows count.  The copy lands on `side`; then the other rows are cleared and
@@ -200,6 +235,27 @@ __device__ __forceinline__ void store32_fp32(const uint32_t (&r)[32], float fact
                     __uint_as_float(r[i + 3]) * factor);
 }
 
+// The thread's row of a tensor (zeros where there is none) to its lane of tensor memory, as the A operand of an MMA.
+template <int D>
+__device__ __forceinline__ void move_rows(const void* rows, const Strides& st, int b, int row, int h, bool in, uint32_t dst) {
+  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(rows) + b * st.batch +
+                                                    (int64_t)row * st.token + h * st.head);
+#pragma unroll
+  for (int c0 = 0; c0 < D; c0 += 32) {
+    uint32_t r[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 v = in ? __ldg(src + c0 / 8 + j) : make_uint4(0, 0, 0, 0);
+      r[4 * j] = v.x;
+      r[4 * j + 1] = v.y;
+      r[4 * j + 2] = v.z;
+      r[4 * j + 3] = v.w;
+    }
+    tmem_st16(dst + c0 / 2, r);
+  }
+  tmem_wait_st();
+}
+
 struct SharedHead {
   WaitContext wc;
   uint32_t tmem_base;
@@ -252,14 +308,22 @@ __device__ __forceinline__ int key_end(const Geometry& g, int q0, int q_len, int
 // ------------------------------------------------------------------------------------------
 // A CTA has two tiles of 128 queries, a softmax warpgroup each; keys and values come in stages of 128.  While one tile's
 // probabilities are formed, the tensor core runs the other tile's products.  Tensor memory: scores of the tiles at columns
-// 0 and 128 (their probabilities replace them, 64 columns), outputs at 256 and 256 + D.
+// 0 and 128, outputs at 256 and 256 + D, and the probabilities in place of the scores (64 columns), or, where D = 64 leaves
+// columns, at 384 and 448: the next scores are then computed as soon as these have been read, not after PV.
 template <int D>
 struct ForwardShared {
   static constexpr int kStages = D == 64 ? 3 : 2;
   SharedHead head;
-  uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_ready[2], o_done[2],
-      side;
+  uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], s_read[2], p_ready[2],
+      o_done[2], side;
 };
+// Every which pair of exponentials takes the polynomial.
+constexpr int kForwardPoly = 4, kBackwardPoly = 4;
+// Roles of the waits: warpgroups of different register counts cannot share a function.
+enum { kFeedRole = 0, kSoftmaxRole = 1 };
+// Registers per thread: 168 at launch, of which the feeding warps leave most to the softmax warps (a row of 128 scores each).
+constexpr int kSoftmaxRegs = 208, kFeedRegs = 72;
+static_assert(256 * kSoftmaxRegs + 128 * kFeedRegs <= kThreads * 168, "what the launch has");
 template <int D>
 constexpr int kForwardTiles = 2 + 2 * ForwardShared<D>::kStages;
 
@@ -268,6 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
   extern __shared__ __align__(1024) uint8_t smem[];
   static_assert(256 + 2 * D <= 512, "scores and outputs of two tiles");
   constexpr int kStages = ForwardShared<D>::kStages, kBytes = kTileBytes<D>;
+  constexpr bool kApart = D == 64;
+  constexpr uint32_t kP = kApart ? 384 : 0, kPStep = kApart ? 64 : 128;  // columns of the probabilities
   auto* s = reinterpret_cast<ForwardShared<D>*>(smem + kForwardTiles<D> * kBytes);
   const Geometry& g = p.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -292,6 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s->s_full[t], 1);
+      mbar_init(&s->s_read[t], 4);
       mbar_init(&s->p_ready[t], 4);
       mbar_init(&s->o_done[t], 1);
     }
@@ -301,91 +368,111 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
   WaitContext* wc = &s->head.wc;
   uint8_t *k_tiles = smem + 2 * kBytes, *v_tiles = k_tiles + kStages * kBytes;
 
-  if (warp == kLoadWarp) {
-    if (n > 0) {
-      uint32_t side_uses = 0;
-      if (lane == 0)
-        for (int t = 0; t < 2; ++t) load_tile<D>(smem + t * kBytes, &p.q, h, min(q0 + t * kTile, g.q_tokens), b, &s->q_full);
-      __syncwarp();
-#pragma unroll 1
-      for (int i = 0; i < n; ++i) {
-        const int st = i % kStages, use = i / kStages, token = (first + i) * kTile;
-        if (use > 0) wait(wc, &s->k_empty[st], (use - 1) & 1, 41);
-        if (lane == 0) load_tile<D>(k_tiles + st * kBytes, &p.k, hk, token, b, &s->k_full[st]);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFeedRegs));
+    if (warp == kLoadWarp) {
+      if (n > 0) {
+        uint32_t side_uses = 0;
+        if (lane == 0)
+          for (int t = 0; t < 2; ++t) load_tile<D>(smem + t * kBytes, &p.q, h, min(q0 + t * kTile, g.q_tokens), b, &s->q_full);
         __syncwarp();
-        if (use > 0) wait(wc, &s->v_empty[st], (use - 1) & 1, 42);
-        if (token + kTile > k_len && k_len < g.k_tokens) {
-          load_cut_tile<D>(v_tiles + st * kBytes, &p.v, hk, token, b, k_len - token, &s->side, side_uses, &s->v_full[st], wc);
-        } else if (lane == 0) {
-          load_tile<D>(v_tiles + st * kBytes, &p.v, hk, token, b, &s->v_full[st]);
-        }
-        __syncwarp();
-      }
-      if (wc->abort) {
-        // unwinding: the copies in flight have to land before the CTA gives its shared memory back
-        drain_wait(&s->q_full, 0, kDrainNs);
-        for (int i = max(0, n - kStages); i < n; ++i) {
-          drain_wait(&s->k_full[i % kStages], (i / kStages) & 1, kDrainNs);
-          drain_wait(&s->v_full[i % kStages], (i / kStages) & 1, kDrainNs);
-        }
-      }
-    }
-  } else if (warp == kMmaWarp) {
-    if (n > 0) {
-      const bool leader = elect_one();
-      const uint32_t qa = smem_u32(smem), ka = smem_u32(k_tiles), va = smem_u32(v_tiles);
-      wait(wc, &s->q_full, 0, 43);
-      wait(wc, &s->k_full[0], 0, 44);
-      tc_fence_after_sync();
-      if (leader) {
-        for (int t = 0; t < tiles; ++t) {
-          scores_ss<D, kBf16>(tmem + t * 128, qa + t * kBytes, ka);
-          mma_commit(&s->s_full[t]);
-        }
-        mma_commit(&s->k_empty[0]);
-      }
-      __syncwarp();
 #pragma unroll 1
-      for (int i = 0; i < n; ++i) {
-        const int st = i % kStages, next = (i + 1) % kStages;
-        wait(wc, &s->v_full[st], (i / kStages) & 1, 45);
-#pragma unroll 1
-        for (int t = 0; t < tiles; ++t) {
-          wait(wc, &s->p_ready[t], i & 1, 46);
-          tc_fence_after_sync();
-          if (leader) {
-            gather_ts<D, kBf16>(tmem + 256 + t * D, tmem + t * 128, 32, va + st * kBytes, i > 0);
-            mma_commit(&s->o_done[t]);
+        for (int i = 0; i < n; ++i) {
+          const int st = i % kStages, use = i / kStages, token = (first + i) * kTile;
+          if (use > 0) wait(wc, &s->k_empty[st], (use - 1) & 1, 41);
+          if (lane == 0) load_tile<D>(k_tiles + st * kBytes, &p.k, hk, token, b, &s->k_full[st]);
+          __syncwarp();
+          if (use > 0) wait(wc, &s->v_empty[st], (use - 1) & 1, 42);
+          if (token + kTile > k_len && k_len < g.k_tokens) {
+            load_cut_tile<D>(v_tiles + st * kBytes, &p.v, hk, token, b, k_len - token, &s->side, side_uses, &s->v_full[st], wc);
+          } else if (lane == 0) {
+            load_tile<D>(v_tiles + st * kBytes, &p.v, hk, token, b, &s->v_full[st]);
           }
           __syncwarp();
-          if (i + 1 < n) {
-            if (t == 0) {
-              wait(wc, &s->k_full[next], ((i + 1) / kStages) & 1, 47);
-              tc_fence_after_sync();
-            }
-            // (the probabilities in this place: read by the products issued just before, which run first)
-            if (leader) {
-              scores_ss<D, kBf16>(tmem + t * 128, qa + t * kBytes, ka + next * kBytes);
-              mma_commit(&s->s_full[t]);
-            }
-            __syncwarp();
+        }
+        if (wc->abort) {
+          // unwinding: the copies in flight have to land before the CTA gives its shared memory back
+          drain_wait(&s->q_full, 0, kDrainNs);
+          for (int i = max(0, n - kStages); i < n; ++i) {
+            drain_wait(&s->k_full[i % kStages], (i / kStages) & 1, kDrainNs);
+            drain_wait(&s->v_full[i % kStages], (i / kStages) & 1, kDrainNs);
           }
         }
+      }
+    } else if (warp == kMmaWarp) {
+      if (n > 0) {
+        const bool leader = elect_one();
+        const uint32_t qa = smem_u32(smem), ka = smem_u32(k_tiles), va = smem_u32(v_tiles);
+        wait(wc, &s->q_full, 0, 43);
+        wait(wc, &s->k_full[0], 0, 44);
+        tc_fence_after_sync();
         if (leader) {
-          mma_commit(&s->v_empty[st]);
-          if (i + 1 < n) mma_commit(&s->k_empty[next]);
+          for (int t = 0; t < tiles; ++t) {
+            scores_ss<D, kBf16>(tmem + t * 128, qa + t * kBytes, ka);
+            mma_commit(&s->s_full[t]);
+          }
+          mma_commit(&s->k_empty[0]);
         }
         __syncwarp();
-      }
-      if (wc->abort) {
-        // the last v_empty follows everything issued
-        drain_wait(&s->v_empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, kDrainNs);
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+          const int st = i % kStages, next = (i + 1) % kStages;
+          if (kApart && i + 1 < n) {
+            wait(wc, &s->k_full[next], ((i + 1) / kStages) & 1, 47);
+#pragma unroll 1
+            for (int t = 0; t < tiles; ++t) {
+              wait(wc, &s->s_read[t], i & 1, 47);
+              tc_fence_after_sync();
+              if (leader) {
+                scores_ss<D, kBf16>(tmem + t * 128, qa + t * kBytes, ka + next * kBytes);
+                mma_commit(&s->s_full[t]);
+              }
+              __syncwarp();
+            }
+            if (leader) mma_commit(&s->k_empty[next]);
+            __syncwarp();
+          }
+          wait(wc, &s->v_full[st], (i / kStages) & 1, 45);
+#pragma unroll 1
+          for (int t = 0; t < tiles; ++t) {
+            wait(wc, &s->p_ready[t], i & 1, 46);
+            tc_fence_after_sync();
+            if (leader) {
+              gather_ts<D, kBf16>(tmem + 256 + t * D, tmem + kP + t * kPStep, 32, va + st * kBytes, i > 0);
+              mma_commit(&s->o_done[t]);
+            }
+            __syncwarp();
+            if (!kApart && i + 1 < n) {
+              if (t == 0) {
+                wait(wc, &s->k_full[next], ((i + 1) / kStages) & 1, 47);
+                tc_fence_after_sync();
+              }
+              // (the probabilities in this place: read by the products issued just before, which run first)
+              if (leader) {
+                scores_ss<D, kBf16>(tmem + t * 128, qa + t * kBytes, ka + next * kBytes);
+                mma_commit(&s->s_full[t]);
+              }
+              __syncwarp();
+            }
+          }
+          if (leader) {
+            mma_commit(&s->v_empty[st]);
+            if (!kApart && i + 1 < n) mma_commit(&s->k_empty[next]);
+          }
+          __syncwarp();
+        }
+        if (wc->abort) {
+          // the last v_empty follows everything issued
+          drain_wait(&s->v_empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, kDrainNs);
+        }
       }
     }
-  } else if (warp < 8) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int t = warp >> 2, row = q0 + t * kTile + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t scores = tmem + lanes + t * 128, acc = tmem + lanes + 256 + t * D;
+    const uint32_t probabilities = tmem + lanes + kP + t * kPStep;
     const float c = g.scale * kLog2e;
     const int seen = g.causal ? min(k_len, row + 1 + k_len - q_len) : k_len;  // keys that this row sees
     // (a warp masks a stage that one of its rows does not see whole)
@@ -395,14 +482,16 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     if (live) {
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
-        wait(wc, &s->s_full[t], i & 1, 48);
+        wait<kSoftmaxRole>(wc, &s->s_full[t], i & 1, 48);
         tc_fence_after_sync();
         float v[128];
 #pragma unroll
         for (int c0 = 0; c0 < 128; c0 += 32) tmem_ld32(scores + c0, *reinterpret_cast<uint32_t(*)[32]>(v + c0));
         tmem_wait_ld();
+        if (kApart) warp_arrive(&s->s_read[t]);
         const int key0 = (first + i) * kTile;
-        if (key0 + kTile > least) {
+        const bool masked = key0 + kTile > least;
+        if (masked) {
           const int valid = seen - key0;
 #pragma unroll
           for (int j = 0; j < 128; ++j) v[j] = j < valid ? v[j] : -INFINITY;
@@ -420,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
           m = m_new;
         } else if (__any_sync(0xffffffffu, move)) {
           const float alpha = move ? exp2_approx((m - m_new) * c) : 1.0f;
-          wait(wc, &s->o_done[t], (i - 1) & 1, 49);
+          wait<kSoftmaxRole>(wc, &s->o_done[t], (i - 1) & 1, 49);
           tc_fence_after_sync();
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 16) {
@@ -442,24 +531,36 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
         const float base = m == -INFINITY ? 0.0f : -m * c;
         const float2 c2 = make_float2(c, c), base2 = make_float2(base, base);
         float2 sum2 = make_float2(0.0f, 0.0f);
+        // (with keys hidden every probability is the unit's: the polynomial has no zero)
+        auto form = [&](auto every) {
 #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          uint32_t packed[16];
+          for (int c0 = 0; c0 < 128; c0 += 32) {
+            uint32_t packed[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float2 e = ffma2(make_float2(v[c0 + j], v[c0 + j + 1]), c2, base2);
-            e.x = exp2_approx(e.x);
-            e.y = exp2_approx(e.y);
-            sum2 = fadd2(sum2, e);
-            packed[j / 2] = pack2<kBf16>(e.x, e.y);
+            for (int j = 0; j < 32; j += 2) {
+              const float2 e =
+                  exp2_pair<decltype(every)::value>(ffma2(make_float2(v[c0 + j], v[c0 + j + 1]), c2, base2), (c0 + j) / 2);
+              sum2 = fadd2(sum2, e);
+              packed[j / 2] = pack2<kBf16>(e.x, e.y);
+            }
+            if (kApart && c0 == 0 && i > 0) {
+              // (PV of the stage before has read these columns)
+              wait<kSoftmaxRole>(wc, &s->o_done[t], (i - 1) & 1, 49);
+              tc_fence_after_sync();
+            }
+            tmem_st16(probabilities + c0 / 2, packed);
           }
-          tmem_st16(scores + c0 / 2, packed);
+        };
+        if (masked) {
+          form(std::integral_constant<int, 0>{});
+        } else {
+          form(std::integral_constant<int, kForwardPoly>{});
         }
         sum += sum2.x + sum2.y;
         tmem_wait_st();
         warp_arrive(&s->p_ready[t]);
       }
-      wait(wc, &s->o_done[t], (n - 1) & 1, 50);
+      wait<kSoftmaxRole>(wc, &s->o_done[t], (n - 1) & 1, 50);
       tc_fence_after_sync();
     }
     // all lanes read (the loads are the warp's), rows that exist are written
@@ -534,16 +635,14 @@ __global__ void __launch_bounds__(128) join_forward_kernel(const float* partial,
 // ------------------------------------------------------------------------------------------
 struct RowParams {
   const void *out, *dout, *v;
-  const float* lse;
-  float *lse2, *delta;
+  float* delta;
   uint32_t* norms;
   Strides so, sd, sv;
   const int32_t *q_lengths, *k_lengths;
   int batch, q_heads, k_heads, q_tokens, k_tokens, q_blocks;
 };
 
-// delta_i and the log-sum-exp in units of log 2 (+inf where the row has no gradient: its probabilities then come out as
-// zeros).  fp16: the largest |dO_i|^2 and |v_j|^2 of each key head, too (a maximum does not depend on the order of atomics).
+// delta_i.  fp16: the largest |dO_i|^2 and |v_j|^2 of each key head, too (a maximum does not depend on the order of atomics).
 // Rows in memory order (heads of a token, tokens, samples), kRowsEach at once per group of D/8 lanes: that many loads in flight.
 constexpr int kRowsEach = 4;
 template <int D, bool kBf16>
@@ -594,10 +693,7 @@ __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowPar
     }
     if (!in[n] || lane != 0) continue;
     if (!values) {
-      const int64_t flat = ((int64_t)b[n] * p.q_heads + h[n]) * p.q_tokens + i[n];
-      const float lse = live[n] ? p.lse[flat] : -INFINITY;
-      p.lse2[flat] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-      p.delta[flat] = live[n] && lse != -INFINITY ? dot : 0.0f;
+      p.delta[((int64_t)b[n] * p.q_heads + h[n]) * p.q_tokens + i[n]] = dot;
     }
     if (!kBf16 && live[n])
       atomicMax(p.norms + 2 * (b[n] * p.k_heads + (values ? h[n] : h[n] / (p.q_heads / p.k_heads))) + (values ? 1 : 0),
@@ -630,6 +726,14 @@ __device__ __forceinline__ Scaling scaling(const BackwardParams& p, int b, int h
   return s;
 }
 
+// Query tiles that see at most kFewStages stages of keys have their delta from few_kernel.
+constexpr int kFewStages = 8;
+
+// A row's log-sum-exp in units of log 2: +inf where it has no gradient, so that its probabilities come out as zeros.
+__device__ __forceinline__ float lse2_of(const BackwardParams& p, int64_t flat, int row, int q_len) {
+  const float lse = row < q_len ? p.lse[flat + row] : -INFINITY;
+  return lse == -INFINITY ? INFINITY : lse * kLog2e;
+}
 // ------------------------------------------------------------------------------------------
 // backward: dK and dV of a key tile
 // ------------------------------------------------------------------------------------------
@@ -731,8 +835,8 @@ __device__ __forceinline__ void key_tile(const BackwardParams& p, uint8_t* smem,
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = token + j * 32 + lane;
-        l[j] = row < g.q_tokens ? p.lse2[flat + row] - f.p_shift : INFINITY;
-        d[j] = row < g.q_tokens ? p.delta[flat + row] * f.ds : 0.0f;
+        l[j] = lse2_of(p, flat, row, q_len) - f.p_shift;
+        d[j] = row < q_len ? p.delta[flat + row] * f.ds : 0.0f;
       }
       if (use > 0) wait(wc, &s->stat_empty[st], (use - 1) & 1, 53);
 #pragma unroll
@@ -825,10 +929,11 @@ __device__ __forceinline__ void key_tile(const BackwardParams& p, uint8_t* smem,
         const float4 l = l4[j / 4];
         const float2 a = ffma2(make_float2(v[j], v[j + 1]), c2, make_float2(l.x, l.y));
         const float2 e = ffma2(make_float2(v[j + 2], v[j + 3]), c2, make_float2(l.z, l.w));
-        v[j] = exp2_approx(a.x);
-        v[j + 1] = exp2_approx(a.y);
-        v[j + 2] = exp2_approx(e.x);
-        v[j + 3] = exp2_approx(e.y);
+        const float2 pa = exp2_pair<kBackwardPoly>(a, j / 2), pe = exp2_pair<kBackwardPoly>(e, j / 2 + 1);
+        v[j] = pa.x;
+        v[j + 1] = pa.y;
+        v[j + 2] = pe.x;
+        v[j + 3] = pe.y;
       }
       if (g.causal) {
         // query token + j sees key `row` from j >= hidden on
@@ -1035,29 +1140,13 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t scores = tmem + lanes + half * 64, grads = scores + 128;
     const float c = g.scale * kLog2e;
-    const int64_t flat = ((int64_t)b * g.q_heads + h) * g.q_tokens + row;
+    const int64_t first_row = ((int64_t)b * g.q_heads + h) * g.q_tokens, flat = first_row + row;
     const bool in = row < q_len;
-    const float lse2 = in ? f.p_shift - p.lse2[flat] : -INFINITY, delta = in ? -p.delta[flat] * f.ds : 0.0f;
+    const float lse2 = f.p_shift - lse2_of(p, first_row, row, q_len);
+    const float delta = in ? -p.delta[flat] * f.ds : 0.0f;
     if (n > 0) {
-      // the first warpgroup's threads read their row of Q, the second's of dO, and move it to tensor memory
-      const Strides& st = half == 0 ? p.sq : p.sdo;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(half == 0 ? p.q_rows : p.do_rows) +
-                                                        b * st.batch + (int64_t)row * st.token + h * st.head);
-      const uint32_t dst = (half == 0 ? q_at : do_at) + lanes;
-#pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t r[16];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 v = in ? __ldg(src + c0 / 8 + j) : make_uint4(0, 0, 0, 0);
-          r[4 * j] = v.x;
-          r[4 * j + 1] = v.y;
-          r[4 * j + 2] = v.z;
-          r[4 * j + 3] = v.w;
-        }
-        tmem_st16(dst + c0 / 2, r);
-      }
-      tmem_wait_st();
+      // the first warpgroup's threads read their row of Q, the second's of dO
+      move_rows<D>(half == 0 ? p.q_rows : p.do_rows, half == 0 ? p.sq : p.sdo, b, row, h, in, (half == 0 ? q_at : do_at) + lanes);
       warp_arrive(&s->moved);
     }
     const int seen = g.causal ? min(k_len, row + 1 + k_len - q_len) : k_len;
@@ -1075,9 +1164,9 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
       warp_arrive(&s->s_read);
 #pragma unroll
       for (int j = 0; j < 64; j += 2) {
-        const float2 a = ffma2(make_float2(v[j], v[j + 1]), c2, l2);
-        v[j] = exp2_approx(a.x);
-        v[j + 1] = exp2_approx(a.y);
+        const float2 e = exp2_pair<kBackwardPoly>(ffma2(make_float2(v[j], v[j + 1]), c2, l2), j / 2);
+        v[j] = e.x;
+        v[j + 1] = e.y;
       }
       const int key0 = (first + i) * kTile + half * 64;
       const bool masked = key0 + 64 > least;
@@ -1131,6 +1220,216 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
     }
   }
   tmem_end(tmem);
+}
+
+// ------------------------------------------------------------------------------------------
+// backward: delta where keys are few
+// ------------------------------------------------------------------------------------------
+// delta_i = dO_i . o_i takes o's rounding to 16 bits along: an error of 2^-9 |dO| |o| that every dS of the row has in common.
+// With many keys o is small and the rounding of dS itself is all that is seen; with few, where o is as large as a value, it
+// is not (bf16, two keys: dQ 0.0052 off relative, 0.0023 with the sum below; 512: 0.0026 and 0.0024; 2,048: 0.0025 and 0.0024).
+// Query tiles that see at most kFewStages stages of keys therefore take delta_i = sum_j P_ij dP_ij in fp32.  A CTA keeps two key
+// tiles, one per warpgroup, and streams query tiles: S at columns 0 and 128, dP at 256 and 384.  Each query tile is read once
+// per two key tiles, as L2 is the bound (5.8 TB/s): for 2 x 16 heads of 7,800 queries on 512 keys one key tile per CTA took
+// 97 us, and a CTA per query tile, most of whose time was its start, 123.  few_sums_kernel adds the key tiles' parts up.
+template <int D>
+struct FewShared {
+  static constexpr int kStages = D == 64 ? 2 : 1;  // of query tiles
+  SharedHead head;
+  uint64_t kv_full, q_full[kStages], q_empty[kStages], do_full[kStages], do_empty[kStages], s_full[2], s_read[2], dp_full[2],
+      dp_read[2];
+};
+template <int D>
+constexpr int kFewTiles = 4 + 2 * FewShared<D>::kStages;
+
+// Query tiles [first, last) of a sample that see key tile `tile` and few in all.
+struct TileRange {
+  int first, last;
+};
+__device__ __forceinline__ TileRange few_tiles(const Geometry& g, int tile, int q_len, int k_len) {
+  const int k0 = tile * kTile, q_tiles = k0 < k_len ? (q_len + kTile - 1) / kTile : 0;
+  TileRange r{0, k_len <= kFewStages * kTile ? q_tiles : 0};
+  if (g.causal) {
+    r.first = min(q_tiles, max(0, k0 - (k_len - q_len)) / kTile);
+    if (k_len > kFewStages * kTile) r.last = min(q_tiles, max(0, kFewStages * kTile - (k_len - q_len)) / kTile);
+  }
+  return r;
+}
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant__ BackwardParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  layer::grid_dependency_wait();
+  constexpr int kBytes = kTileBytes<D>, kStages = FewShared<D>::kStages;
+  auto* s = reinterpret_cast<FewShared<D>*>(smem + kFewTiles<D> * kBytes);
+  const Geometry& g = p.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z / p.few_splits, split = blockIdx.z % p.few_splits, h = blockIdx.y, hk = h / (g.q_heads / g.k_heads);
+  const int q_len = length_of(g.q_lengths, b, g.q_tokens), k_len = length_of(g.k_lengths, b, g.k_tokens);
+  // (what the first of the two sees, the second one's query tiles are among: of the others its part is not asked for)
+  const TileRange range = few_tiles(g, 2 * blockIdx.x, q_len, k_len);
+  const int all = max(0, range.last - range.first);
+  const int first = range.first + (int)((int64_t)all * split / p.few_splits);
+  const int n = range.first + (int)((int64_t)all * (split + 1) / p.few_splits) - first;
+  const int tiles = (2 * blockIdx.x + 1) * kTile < k_len ? 2 : 1;
+  if (n == 0 || given_up(g)) return;
+  if (threadIdx.x == 0) {
+    begin_waits(&s->head, g);
+    mbar_init(&s->kv_full, 2 * tiles);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s->q_full[i], 1);
+      mbar_init(&s->q_empty[i], 1);
+      mbar_init(&s->do_full[i], 1);
+      mbar_init(&s->do_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s->s_full[t], 1);
+      mbar_init(&s->s_read[t], 4);
+      mbar_init(&s->dp_full[t], 1);
+      mbar_init(&s->dp_read[t], 4);
+    }
+    mbar_init_fence();
+  }
+  const uint32_t tmem = tmem_begin(&s->head);
+  WaitContext* wc = &s->head.wc;
+  uint8_t *q_tiles_at = smem + 4 * kBytes, *do_tiles_at = q_tiles_at + kStages * kBytes;
+  if (warp == kLoadWarp) {
+    if (lane == 0)
+      for (int t = 0; t < tiles; ++t) {
+        load_tile<D>(smem + 2 * t * kBytes, &p.k, hk, (2 * blockIdx.x + t) * kTile, b, &s->kv_full);
+        load_tile<D>(smem + (2 * t + 1) * kBytes, &p.v, hk, (2 * blockIdx.x + t) * kTile, b, &s->kv_full);
+      }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int st = i % kStages, use = i / kStages, token = (first + i) * kTile;
+      // (the tiles are read from HBM for the first time here: L2 fetches two steps ahead of the copies)
+      for (int j = i == 0 ? 1 : 2; j <= 2; ++j)
+        if (lane == 0 && i + j < n) {
+          prefetch_tile<D>(&p.q, h, token + j * kTile, b);
+          prefetch_tile<D>(&p.dout, h, token + j * kTile, b);
+        }
+      if (use > 0) wait(wc, &s->q_empty[st], (use - 1) & 1, 91);
+      if (lane == 0) load_tile<D>(q_tiles_at + st * kBytes, &p.q, h, token, b, &s->q_full[st]);
+      __syncwarp();
+      if (use > 0) wait(wc, &s->do_empty[st], (use - 1) & 1, 92);
+      if (lane == 0) load_tile<D>(do_tiles_at + st * kBytes, &p.dout, h, token, b, &s->do_full[st]);
+      __syncwarp();
+    }
+    if (wc->abort) {
+      drain_wait(&s->kv_full, 0, kDrainNs);
+      for (int i = max(0, n - kStages); i < n; ++i) {
+        drain_wait(&s->q_full[i % kStages], (i / kStages) & 1, kDrainNs);
+        drain_wait(&s->do_full[i % kStages], (i / kStages) & 1, kDrainNs);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    const bool leader = elect_one();
+    const uint32_t ka = smem_u32(smem), va = ka + kBytes, qa = smem_u32(q_tiles_at), da = smem_u32(do_tiles_at);
+    wait(wc, &s->kv_full, 0, 93);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int st = i % kStages, parity = (i / kStages) & 1;
+      wait(wc, &s->q_full[st], parity, 95);
+      for (int t = 0; t < tiles; ++t) {
+        if (i > 0) wait(wc, &s->s_read[t], (i - 1) & 1, 94);
+        tc_fence_after_sync();
+        if (leader) {
+          scores_ss<D, kBf16>(tmem + t * 128, qa + st * kBytes, ka + 2 * t * kBytes);
+          mma_commit(&s->s_full[t]);
+        }
+        __syncwarp();
+      }
+      if (leader) mma_commit(&s->q_empty[st]);
+      __syncwarp();
+      wait(wc, &s->do_full[st], parity, 97);
+      for (int t = 0; t < tiles; ++t) {
+        if (i > 0) wait(wc, &s->dp_read[t], (i - 1) & 1, 96);
+        tc_fence_after_sync();
+        if (leader) {
+          scores_ss<D, kBf16>(tmem + 256 + t * 128, da + st * kBytes, va + 2 * t * kBytes);
+          mma_commit(&s->dp_full[t]);
+        }
+        __syncwarp();
+      }
+      if (leader) mma_commit(&s->do_empty[st]);
+      __syncwarp();
+    }
+    // (the last of them follows everything issued)
+    if (wc->abort) drain_wait(&s->do_empty[(n - 1) % kStages], ((n - 1) / kStages) & 1, kDrainNs);
+  } else if (warp < 8 && warp >> 2 < tiles) {
+    const int t = warp >> 2, local = (warp & 3) * 32 + lane, key0 = (2 * blockIdx.x + t) * kTile;
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * 128;
+    const float c = g.scale * kLog2e;
+    const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens;
+    const int64_t flat = ((int64_t)b * g.q_heads + h) * g.q_tokens;
+    float* part = p.few_parts + (2 * blockIdx.x + t) * rows_all + flat;
+    float lse2 = lse2_of(p, flat, first * kTile + local, q_len);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int row = (first + i) * kTile + local;
+      const float next = i + 1 < n ? lse2_of(p, flat, row + kTile, q_len) : 0.0f;
+      const int seen = (g.causal ? min(k_len, row + 1 + k_len - q_len) : k_len) - key0;
+      const float2 c2 = make_float2(c, c), l2 = make_float2(-lse2, -lse2);
+      wait(wc, &s->s_full[t], i & 1, 98);
+      tc_fence_after_sync();
+      float v[128];
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) tmem_ld32(at + c0, *reinterpret_cast<uint32_t(*)[32]>(v + c0));
+      tmem_wait_ld();
+      warp_arrive(&s->s_read[t]);
+#pragma unroll
+      for (int j = 0; j < 128; j += 2) {
+        const float2 a = ffma2(make_float2(v[j], v[j + 1]), c2, l2);
+        v[j] = exp2_approx(a.x);
+        v[j + 1] = exp2_approx(a.y);
+      }
+      wait(wc, &s->dp_full[t], i & 1, 99);
+      tc_fence_after_sync();
+      float sum = 0.0f;
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld32(at + 256 + c0, r);
+        tmem_wait_ld();
+        // (what stands behind the keys may be NaN)
+        if (seen < 128) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < seen) sum = fmaf(v[c0 + j], __uint_as_float(r[j]), sum);
+        } else {
+          float2 sum2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2)
+            sum2 = ffma2(make_float2(v[c0 + j], v[c0 + j + 1]),
+                         make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), sum2);
+          sum += sum2.x + sum2.y;
+        }
+      }
+      warp_arrive(&s->dp_read[t]);
+      if (row < q_len) part[row] = lse2 == INFINITY ? 0.0f : sum;
+      lse2 = next;
+    }
+  }
+  tmem_end(tmem);
+}
+
+// Adds a row's parts up, in order, into its delta.
+__global__ void __launch_bounds__(256) few_sums_kernel(const float* parts, float* delta, const __grid_constant__ Geometry g) {
+  layer::grid_dependency_wait();
+  const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x * 256 + threadIdx.x;
+  const int q_len = length_of(g.q_lengths, b, g.q_tokens), k_len = length_of(g.k_lengths, b, g.k_tokens);
+  if (row >= q_len) return;
+  const int stages = (key_end(g, row / kTile * kTile + kTile, q_len, k_len) + kTile - 1) / kTile;
+  if (stages > kFewStages) return;
+  const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens, flat = ((int64_t)b * g.q_heads + h) * g.q_tokens + row;
+  float part[kFewStages];
+#pragma unroll
+  for (int i = 0; i < kFewStages; ++i) part[i] = i < stages ? parts[i * rows_all + flat] : 0.0f;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kFewStages; ++i) sum += part[i];
+  delta[flat] = sum;
 }
 
 // Both kinds of tiles in one launch: the query tiles fill the SMs that the last key tiles leave.
@@ -1254,15 +1553,20 @@ int parts_of(int64_t ctas, int steps) {
 }
 
 struct Plan {
-  int forward_splits, key_splits, query_splits;
+  int forward_splits, key_splits, query_splits, few_splits;
+  bool few;  // whether a query tile may see few keys (a sample may be shorter than its tensor)
 };
-Plan plan_of(const anemoi_sm100_dense_shape* s) {
+Plan plan_of(const anemoi_sm100_dense_shape* s, bool key_lengths = false) {
   const int64_t qt = tiles_of(s->q_tokens), kt = tiles_of(s->k_tokens), b = s->batch;
   const int group = s->q_heads / s->k_heads;
   Plan p;
   p.forward_splits = parts_of((qt + 1) / 2 * s->q_heads * b, (int)kt);
   p.key_splits = parts_of(kt * s->k_heads * b, (int)std::min<int64_t>(1 << 20, qt * group));
   p.query_splits = parts_of(qt * s->q_heads * b, (int)kt);
+  p.few = kt <= kFewStages || s->causal || key_lengths;
+  // one walk for every SM
+  const int64_t ctas = (std::min<int64_t>(kt, kFewStages) + 1) / 2 * s->q_heads * b;
+  p.few_splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(qt, 65535 / b), rows::kSms / ctas));
   return p;
 }
 
@@ -1309,8 +1613,22 @@ int backward_launch(const BackwardParams& p, const RowParams& r, cudaStream_t st
   rp.q_blocks = (int)q_blocks;
   if (!kBf16 && cudaMemsetAsync(rp.norms, 0, (size_t)g.batch * g.k_heads * 2 * sizeof(uint32_t), st) != cudaSuccess)
     return ANEMOI_SM100_ELAUNCH;
-  row_kernel<D, kBf16><<<(unsigned)(q_blocks + v_blocks), 256, 0, st>>>(rp);
-  if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+  // (bf16 with few keys everywhere needs nothing of it)
+  if (!kBf16 || p.few_parts == nullptr || g.k_tokens > kFewStages * kTile) {
+    row_kernel<D, kBf16><<<(unsigned)(q_blocks + v_blocks), 256, 0, st>>>(rp);
+    if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+  }
+  if (p.few_parts != nullptr) {
+    auto few = few_kernel<D, kBf16>;
+    const size_t smem = kFewTiles<D> * (size_t)kTileBytes<D> + sizeof(FewShared<D>);
+    if (cudaFuncSetAttribute(few, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return ANEMOI_SM100_ELAUNCH;
+    const dim3 grid((std::min(p.key_tiles, kFewStages) + 1) / 2, g.q_heads, g.batch * p.few_splits);
+    if (layer::launch(few, grid, dim3(kThreads), smem, st, p) != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+    if (layer::launch(few_sums_kernel, dim3((g.q_tokens + 255) / 256, g.q_heads, g.batch), dim3(256), 0, st,
+                      (const float*)p.few_parts, rp.delta, g) != cudaSuccess)
+      return ANEMOI_SM100_ELAUNCH;
+  }
   auto kernel = backward_kernel<D, kBf16>;
   const size_t smem = 6 * (size_t)kTileBytes<D> + std::max(sizeof(KeyShared<D>), sizeof(QueryShared<D>));
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
@@ -1384,12 +1702,13 @@ extern "C" int anemoi_sm100_dense_attention(const anemoi_sm100_dense_shape* s, c
   return bf16 ? forward_launch<128, true>(p, st) : forward_launch<128, false>(p, st);
 }
 
-extern "C" int64_t anemoi_sm100_dense_attention_backward_workspace(const anemoi_sm100_dense_shape* s) {
+extern "C" int64_t anemoi_sm100_dense_attention_backward_workspace(const anemoi_sm100_dense_shape* s, int key_lengths) {
   const int bad = check(s);
   if (bad != ANEMOI_SM100_OK) return bad;
-  const Plan plan = plan_of(s);
+  const Plan plan = plan_of(s, key_lengths != 0);
   const int64_t q_rows = (int64_t)s->batch * s->q_heads * s->q_tokens, k_rows = (int64_t)s->batch * s->k_heads * s->k_tokens;
-  int64_t bytes = 2 * round16(q_rows * 4) + round16((int64_t)s->batch * s->k_heads * 8);
+  int64_t bytes = round16(q_rows * 4) + round16((int64_t)s->batch * s->k_heads * 8);
+  if (plan.few) bytes += round16(std::min(tiles_of(s->k_tokens), kFewStages) * q_rows * 4);
   if (plan.query_splits > 1) bytes += plan.query_splits * q_rows * s->head_dim * 4;
   if (plan.key_splits > 1) bytes += plan.key_splits * 2 * k_rows * s->head_dim * 4;
   return bytes;
@@ -1404,7 +1723,7 @@ extern "C" int anemoi_sm100_dense_attention_backward(const anemoi_sm100_dense_sh
   if (bad != ANEMOI_SM100_OK) return bad;
   if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv || !strides || !status || !workspace)
     return ANEMOI_SM100_EINVAL;
-  if (workspace_bytes < anemoi_sm100_dense_attention_backward_workspace(s) || reinterpret_cast<uintptr_t>(workspace) % 16)
+  if (workspace_bytes < anemoi_sm100_dense_attention_backward_workspace(s, k_lengths != nullptr) || reinterpret_cast<uintptr_t>(workspace) % 16)
     return ANEMOI_SM100_EINVAL;
   const int d = s->head_dim;
   Tensor t[8];
@@ -1422,7 +1741,8 @@ extern "C" int anemoi_sm100_dense_attention_backward(const anemoi_sm100_dense_sh
       !encode(&p.k, t[2], bf16, d, s->batch) || !encode(&p.v, t[3], bf16, d, s->batch))
     return ANEMOI_SM100_EINVAL;
   geometry(p.g, s, q_lengths, k_lengths, status);
-  const Plan plan = plan_of(s);
+  const Plan plan = plan_of(s, k_lengths != nullptr);
+  p.few_splits = plan.few_splits;
   p.g.splits = plan.key_splits;
   p.q_splits = plan.query_splits;
   p.key_tiles = tiles_of(s->k_tokens);
@@ -1430,17 +1750,19 @@ extern "C" int anemoi_sm100_dense_attention_backward(const anemoi_sm100_dense_sh
   p.key_ctas = p.key_tiles * s->k_heads * s->batch * plan.key_splits;
   const int64_t q_rows = (int64_t)s->batch * s->q_heads * s->q_tokens;
   char* w = static_cast<char*>(workspace);
-  float* lse2 = reinterpret_cast<float*>(w);
-  w += round16(q_rows * 4);
   float* delta = reinterpret_cast<float*>(w);
   w += round16(q_rows * 4);
   uint32_t* norms = reinterpret_cast<uint32_t*>(w);
   w += round16((int64_t)s->batch * s->k_heads * 8);
+  if (plan.few) {
+    p.few_parts = reinterpret_cast<float*>(w);
+    w += round16(std::min(p.key_tiles, kFewStages) * q_rows * 4);
+  }
   p.q_partial = reinterpret_cast<float*>(w);
   p.k_partial = p.q_partial + (plan.query_splits > 1 ? plan.query_splits * q_rows * d : 0);
   p.q_rows = q;
   p.do_rows = dout;
-  p.lse2 = lse2;
+  p.lse = lse;
   p.delta = delta;
   p.norms = norms;
   p.dq = dq;
@@ -1455,8 +1777,6 @@ extern "C" int anemoi_sm100_dense_attention_backward(const anemoi_sm100_dense_sh
   r.out = out;
   r.dout = dout;
   r.v = v;
-  r.lse = lse;
-  r.lse2 = lse2;
   r.delta = delta;
   r.norms = bf16 ? nullptr : norms;
   r.so = t[4].s;

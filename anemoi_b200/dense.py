@@ -62,7 +62,7 @@ class _Plan:
         self.shape = native.DenseShape(batch=batch, q_heads=q_heads, k_heads=k_heads, q_tokens=q_tokens, k_tokens=k_tokens,
                                        head_dim=dim, causal=int(bool(causal)), is_bf16=int(dtype == torch.bfloat16),
                                        scale=scale)
-        self.forward_bytes, self.backward_bytes = (0, 0) if self.empty else native.dense_attention_bytes(self.shape)
+        self.forward_bytes, self.backward_bytes = (0, (0, 0)) if self.empty else native.dense_attention_bytes(self.shape)
         packed = ((q_tokens * q_heads * dim, q_heads * dim, dim), (k_tokens * k_heads * dim, k_heads * dim, dim))
         self.packed = packed
         self.forward_strides = native.strides_array([n for t in (*self.strides, packed[0]) for n in t])
@@ -126,7 +126,7 @@ def dense_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
     _aligned(grad_out=grad_out, q=q, k=k, v=v, out=out)
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     native.dense_attention_backward(plan.shape, grad_out, q, k, v, out, lse, q_lengths, k_lengths, strides, dq, dk, dv,
-                                    plan.backward_bytes, _status_word(q.device))
+                                    plan.backward_bytes[k_lengths is not None], _status_word(q.device))
     return dq, dk, dv
 
 

@@ -180,7 +180,7 @@ def library() -> C.CDLL:
                                                        P, P, P, P, P, I64, P]),
         "anemoi_sm100_dense_attention_workspace": (I64, [DP]),
         "anemoi_sm100_dense_attention": (C.c_int, [DP, P, P, P, P, P, C.POINTER(I64), P, P, P, I64, P, P]),
-        "anemoi_sm100_dense_attention_backward_workspace": (I64, [DP]),
+        "anemoi_sm100_dense_attention_backward_workspace": (I64, [DP, C.c_int]),
         "anemoi_sm100_dense_attention_backward": (C.c_int, [DP, P, P, P, P, P, P, P, P, C.POINTER(I64), P, P, P, P, I64, P,
                                                             P]),
     }
@@ -858,11 +858,11 @@ def axial_rope_backward(shape: AxialRopeShape, dq_out, dk_out, q, k, q_weight, k
             "anemoi_sm100_axial_rope_backward")
 
 
-def dense_attention_bytes(shape: DenseShape) -> tuple[int, int]:
-    """Workspace of the forward and of the backward pass."""
+def dense_attention_bytes(shape: DenseShape) -> tuple[int, tuple[int, int]]:
+    """Workspace of the forward pass, and of the backward pass without and with key lengths."""
     lib = library()
     return (workspace_bytes(lib.anemoi_sm100_dense_attention_workspace(shape)),
-            workspace_bytes(lib.anemoi_sm100_dense_attention_backward_workspace(shape)))
+            tuple(workspace_bytes(lib.anemoi_sm100_dense_attention_backward_workspace(shape, n)) for n in (0, 1)))
 
 
 def dense_attention(shape: DenseShape, q, k, v, q_lengths, k_lengths, strides, out, lse, nbytes: int, status) -> None:

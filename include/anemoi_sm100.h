@@ -539,7 +539,8 @@ int anemoi_sm100_dense_attention(const anemoi_sm100_dense_shape* s, const void* 
                                  const int32_t* q_lengths, const int32_t* k_lengths, const int64_t* strides, void* out,
                                  float* lse, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
-int64_t anemoi_sm100_dense_attention_backward_workspace(const anemoi_sm100_dense_shape* s);
+/* Bytes of workspace of the backward pass; `key_lengths`: whether they are given. */
+int64_t anemoi_sm100_dense_attention_backward_workspace(const anemoi_sm100_dense_shape* s, int key_lengths);
 
 /* Gradients of q, k, v from that of out; `out` and `lse` are the forward pass's.  strides: of dout, q, k, v, out, dq, dk, dv.
  * Rows behind a length get zeros.  No atomic additions: equal calls give equal bits. */

@@ -307,7 +307,7 @@ def test_the_library_refuses(native_library):
     from anemoi_b200 import native
 
     good = dict(batch=1, q_heads=4, k_heads=2, q_tokens=8, k_tokens=8, head_dim=64, causal=0, is_bf16=1, scale=0.125)
-    assert native_library.anemoi_sm100_dense_attention_backward_workspace(C.byref(native.DenseShape(**good))) > 0
+    assert native_library.anemoi_sm100_dense_attention_backward_workspace(C.byref(native.DenseShape(**good)), 0) > 0
     for change in (dict(batch=0), dict(k_heads=3), dict(k_heads=0), dict(head_dim=96), dict(scale=0.0), dict(scale=-1.0),
                    dict(scale=float("nan")), dict(scale=float("inf")), dict(q_tokens=0), dict(k_tokens=-1)):
         shape = native.DenseShape(**{**good, **change})
