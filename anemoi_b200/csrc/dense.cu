@@ -46,6 +46,11 @@ struct Geometry {
   float scale;
 };
 
+// Pairs of query tiles of a forward pass: the first `whole` walk all their keys in one CTA, the others in `splits`.
+struct TailSplit {
+  int pairs, whole, splits;
+};
+
 struct Strides {
   int64_t batch, token, head;
 };
@@ -53,22 +58,22 @@ struct Strides {
 struct ForwardParams {
   CUtensorMap q, k, v;
   Geometry g;
+  TailSplit tail;
   void* out;
   float* lse;
-  float* partial;  // with splits: [splits][B][H][q_tokens][D], then their lse [splits][B][H][q_tokens]
+  float* partial;  // of the pairs that are split: [splits][pairs][2 * kTile][D], then the rows' lse [splits][pairs][2 * kTile]
   Strides o;
 };
 
 struct BackwardParams {
   CUtensorMap q, k, v, dout;
   Geometry g;                  // (splits: of the key tiles' queries)
-  const void *q_rows, *do_rows;
   const float *lse, *delta;    // [B][H][q_tokens]
   float* few_parts;            // [few key tiles][B][H][q_tokens], where query tiles may see few keys (few_kernel)
   const uint32_t* norms;       // fp16: largest |dO_i|^2 and |v_j|^2 per (sample, key head)
   void *dq, *dk, *dv;
   float *q_partial, *k_partial;  // with splits: [splits][B][H][q_tokens][D]; [splits][dV, dK][B][Hk][k_tokens][D]
-  Strides sq, sdo, sdq, sdk, sdv;
+  Strides sdq, sdk, sdv;
   int q_splits, key_tiles, query_tiles, key_ctas, few_splits;
 };
 
@@ -235,17 +240,19 @@ __device__ __forceinline__ void store32_fp32(const uint32_t (&r)[32], float fact
                     __uint_as_float(r[i + 3]) * factor);
 }
 
-// The thread's row of a tensor (zeros where there is none) to its lane of tensor memory, as the A operand of an MMA.
+// The thread's row of a tile in shared memory (zeros where there is none) to its lane of tensor memory, as the A operand of
+// an MMA.  (Straight from global memory, a row per thread: 4,000 cycles of L1 for the 64 KB.)
 template <int D>
-__device__ __forceinline__ void move_rows(const void* rows, const Strides& st, int b, int row, int h, bool in, uint32_t dst) {
-  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(rows) + b * st.batch +
-                                                    (int64_t)row * st.token + h * st.head);
+__device__ __forceinline__ void move_row(const uint8_t* tile, int row, bool in, uint32_t dst) {
 #pragma unroll
   for (int c0 = 0; c0 < D; c0 += 32) {
     uint32_t r[16];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint4 v = in ? __ldg(src + c0 / 8 + j) : make_uint4(0, 0, 0, 0);
+      const int piece = c0 / 8 + j;
+      const uint4 v = in ? *reinterpret_cast<const uint4*>(tile + piece / 8 * (kTile * 128) + row * 128 +
+                                                           (piece % 8 ^ row % 8) * 16)
+                         : make_uint4(0, 0, 0, 0);
       r[4 * j] = v.x;
       r[4 * j + 1] = v.y;
       r[4 * j + 2] = v.z;
@@ -337,13 +344,17 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
   auto* s = reinterpret_cast<ForwardShared<D>*>(smem + kForwardTiles<D> * kBytes);
   const Geometry& g = p.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.z / g.splits, split = blockIdx.z % g.splits, h = blockIdx.y, hk = h / (g.q_heads / g.k_heads);
+  const bool parted = (int)blockIdx.x >= p.tail.whole;
+  const int splits = parted ? p.tail.splits : 1, split = parted ? (blockIdx.x - p.tail.whole) % splits : 0;
+  const int pair = parted ? p.tail.whole + (blockIdx.x - p.tail.whole) / splits : blockIdx.x;
+  const int each = (g.q_tokens + 2 * kTile - 1) / (2 * kTile), place = pair % each, bh = pair / each;
+  const int h = bh % g.q_heads, b = bh / g.q_heads, hk = h / (g.q_heads / g.k_heads);
   // (the longest walks first)
-  const int q0 = (g.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * 2 * kTile;
+  const int q0 = (g.causal ? each - 1 - place : place) * 2 * kTile;
   const int q_len = length_of(g.q_lengths, b, g.q_tokens), k_len = length_of(g.k_lengths, b, g.k_tokens);
   const int keys = q0 < q_len ? key_end(g, q0 + 2 * kTile, q_len, k_len) : 0;
   const int all = (keys + kTile - 1) / kTile;
-  const int first = (int)((int64_t)all * split / g.splits), n = (int)((int64_t)all * (split + 1) / g.splits) - first;
+  const int first = (int)((int64_t)all * split / splits), n = (int)((int64_t)all * (split + 1) / splits) - first;
   const int tiles = q0 + kTile < q_len ? 2 : 1;
   if (given_up(g)) return;
   if (threadIdx.x == 0) {
@@ -567,6 +578,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     const bool given = live && row < q_len && sum != 0.0f;  // (NaN is an answer, too)
     const float factor = given ? 1.0f / sum : 0.0f, lse = given ? (m * c + log2f(sum)) * kLn2 : -INFINITY;
     const int64_t flat = ((int64_t)b * g.q_heads + h) * g.q_tokens + row;
+    const int64_t parted_pairs = p.tail.pairs - p.tail.whole;
+    const int64_t part_row = (split * parted_pairs + pair - p.tail.whole) * 2 * kTile + row - q0;
 #pragma unroll 1
     for (int c0 = 0; c0 < D; c0 += 32) {
       uint32_t r[32];
@@ -578,9 +591,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
       for (int j = 0; j < 32; ++j)
         if (!given) r[j] = 0u;
       if (row < g.q_tokens) {
-        if (g.splits > 1) {
-          const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens;
-          store32_fp32(r, factor, p.partial + ((int64_t)split * rows_all + flat) * D + c0);
+        if (parted) {
+          store32_fp32(r, factor, p.partial + part_row * D + c0);
         } else {
           store32<kBf16>(r, factor,
                          static_cast<uint16_t*>(p.out) + b * p.o.batch + (int64_t)row * p.o.token + h * p.o.head + c0);
@@ -588,9 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
       }
     }
     if (row < g.q_tokens) {
-      if (g.splits > 1) {
-        const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens;
-        p.partial[(int64_t)g.splits * rows_all * D + (int64_t)split * rows_all + flat] = lse;
+      if (parted) {
+        p.partial[(int64_t)splits * parted_pairs * 2 * kTile * D + part_row] = lse;
       } else if (p.lse != nullptr) {
         p.lse[flat] = lse;
       }
@@ -601,21 +612,26 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
 
 // Joins a row's parts, in order: weights exp(lse_s - lse).  D / 4 threads per row.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(128) join_forward_kernel(const float* partial, int splits, int64_t rows_all, int q_heads,
-                                                           int q_tokens, Strides o, void* out, float* lse_out) {
+__global__ void __launch_bounds__(128) join_forward_kernel(const __grid_constant__ ForwardParams p) {
   layer::grid_dependency_wait();
   constexpr int kLanes = D / 4;
-  const int64_t flat = (int64_t)blockIdx.x * (128 / kLanes) + threadIdx.x / kLanes;
-  if (flat >= rows_all) return;
-  const int c = threadIdx.x % kLanes * 4;
-  const float* lses = partial + (int64_t)splits * rows_all * D + flat;
+  const Geometry& g = p.g;
+  const int64_t parted_rows = (int64_t)(p.tail.pairs - p.tail.whole) * 2 * kTile;
+  const int64_t at = (int64_t)blockIdx.x * (128 / kLanes) + threadIdx.x / kLanes;
+  if (at >= parted_rows) return;
+  const int pair = p.tail.whole + (int)(at / (2 * kTile)), each = (g.q_tokens + 2 * kTile - 1) / (2 * kTile);
+  const int place = pair % each, bh = pair / each, h = bh % g.q_heads, b = bh / g.q_heads;
+  const int row = (g.causal ? each - 1 - place : place) * 2 * kTile + (int)(at % (2 * kTile));
+  if (row >= g.q_tokens) return;
+  const int c = threadIdx.x % kLanes * 4, splits = p.tail.splits;
+  const float* lses = p.partial + (int64_t)splits * parted_rows * D + at;
   float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, lses[(int64_t)s * rows_all]);
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, lses[s * parted_rows]);
   float sum = 0.0f, v[4] = {};
   const float base = top == -INFINITY ? 0.0f : top;
   for (int s = 0; s < splits; ++s) {
-    const float w = exp2_approx((lses[(int64_t)s * rows_all] - base) * kLog2e);
-    const float4 o4 = *reinterpret_cast<const float4*>(partial + ((int64_t)s * rows_all + flat) * D + c);
+    const float w = exp2_approx((lses[s * parted_rows] - base) * kLog2e);
+    const float4 o4 = *reinterpret_cast<const float4*>(p.partial + (s * parted_rows + at) * D + c);
     sum += w;
     v[0] = fmaf(w, o4.x, v[0]);
     v[1] = fmaf(w, o4.y, v[1]);
@@ -623,11 +639,11 @@ __global__ void __launch_bounds__(128) join_forward_kernel(const float* partial,
     v[3] = fmaf(w, o4.w, v[3]);
   }
   const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t bh = flat / q_tokens, row = flat - bh * q_tokens, b = bh / q_heads, h = bh - b * q_heads;
-  uint16_t* dst = static_cast<uint16_t*>(out) + b * o.batch + row * o.token + h * o.head + c;
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.o.batch + (int64_t)row * p.o.token + h * p.o.head + c;
   *reinterpret_cast<uint2*>(dst) =
       make_uint2(pack2<kBf16>(v[0] * inverse, v[1] * inverse), pack2<kBf16>(v[2] * inverse, v[3] * inverse));
-  if (c == 0 && lse_out != nullptr) lse_out[flat] = sum == 0.0f ? -INFINITY : base + log2f(sum) * kLn2;
+  if (c == 0 && p.lse != nullptr)
+    p.lse[((int64_t)b * g.q_heads + h) * g.q_tokens + row] = sum == 0.0f ? -INFINITY : base + log2f(sum) * kLn2;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1022,8 +1038,8 @@ template <int D>
 struct QueryShared {
   static constexpr int kStages = 3;
   SharedHead head;
-  uint64_t moved, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full, s_read, dp_full, ds_ready,
-      all_done, side;
+  uint64_t rows_full, moved, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full, s_read, dp_full,
+      ds_ready, all_done, side;
 };
 
 template <int D, bool kBf16>
@@ -1038,6 +1054,7 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
   const int first = (int)((int64_t)all * split / p.q_splits), n = (int)((int64_t)all * (split + 1) / p.q_splits) - first;
   if (threadIdx.x == 0) {
     begin_waits(&s->head, g);
+    mbar_init(&s->rows_full, 2);
     mbar_init(&s->moved, 8);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s->k_full[i], 1);
@@ -1061,9 +1078,16 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
 
   if (warp == kLoadWarp) {
     uint32_t side_uses = 0;
+    // Q and dO pass through the last stage's buffers
+    if (n > 0 && lane == 0) {
+      load_tile<D>(k_tiles + (kStages - 1) * kBytes, &p.q, h, q0, b, &s->rows_full);
+      load_tile<D>(v_tiles + (kStages - 1) * kBytes, &p.dout, h, q0, b, &s->rows_full);
+    }
+    __syncwarp();
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const int st = i % kStages, use = i / kStages, token = (first + i) * kTile;
+      if (i == kStages - 1) wait(wc, &s->moved, 0, 70);
       if (use > 0) wait(wc, &s->k_empty[st], (use - 1) & 1, 71);
       if (token + kTile > k_len && k_len < g.k_tokens) {
         load_cut_tile<D>(k_tiles + st * kBytes, &p.k, hk, token, b, k_len - token, &s->side, side_uses, &s->k_full[st], wc);
@@ -1075,6 +1099,7 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
       if (lane == 0) load_tile<D>(v_tiles + st * kBytes, &p.v, hk, token, b, &s->v_full[st]);
       __syncwarp();
     }
+    if (wc->abort && n > 0) drain_wait(&s->rows_full, 0, kDrainNs);
     if (wc->abort)
       for (int i = max(0, n - kStages); i < n; ++i) {
         drain_wait(&s->k_full[i % kStages], (i / kStages) & 1, kDrainNs);
@@ -1145,8 +1170,11 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
     const float lse2 = f.p_shift - lse2_of(p, first_row, row, q_len);
     const float delta = in ? -p.delta[flat] * f.ds : 0.0f;
     if (n > 0) {
-      // the first warpgroup's threads read their row of Q, the second's of dO
-      move_rows<D>(half == 0 ? p.q_rows : p.do_rows, half == 0 ? p.sq : p.sdo, b, row, h, in, (half == 0 ? q_at : do_at) + lanes);
+      // the first warpgroup's threads move their row of Q, the second's of dO
+      wait(wc, &s->rows_full, 0, 83);
+      move_row<D>((half == 0 ? k_tiles : v_tiles) + (kStages - 1) * kBytes, local, in, (half == 0 ? q_at : do_at) + lanes);
+      // (read before the copies that come into the same place)
+      fence_proxy_async_smem();
       warp_arrive(&s->moved);
     }
     const int seen = g.causal ? min(k_len, row + 1 + k_len - q_len) : k_len;
@@ -1553,14 +1581,23 @@ int parts_of(int64_t ctas, int steps) {
 }
 
 struct Plan {
-  int forward_splits, key_splits, query_splits, few_splits;
+  TailSplit tail;
+  int key_splits, query_splits, few_splits;
   bool few;  // whether a query tile may see few keys (a sample may be shorter than its tensor)
 };
 Plan plan_of(const anemoi_sm100_dense_shape* s, bool key_lengths = false) {
   const int64_t qt = tiles_of(s->q_tokens), kt = tiles_of(s->k_tokens), b = s->batch;
   const int group = s->q_heads / s->k_heads;
   Plan p;
-  p.forward_splits = parts_of((qt + 1) / 2 * s->q_heads * b, (int)kt);
+  // The pairs of tiles behind the last full wave of CTAs are split so that they fill one, too (16,128 tokens of 12 heads: 756
+  // pairs, 16 of them behind five waves; 1,090 us unsplit).  A causal mask's last walks are its shortest.
+  const int64_t pairs = (qt + 1) / 2 * s->q_heads * b, rest = pairs % rows::kSms;
+  const bool few_pairs = pairs < rows::kSms;
+  p.tail = {(int)pairs, (int)pairs, 1};
+  if (rest > 0 && (few_pairs || !s->causal)) {
+    p.tail.splits = parts_of(rest, (int)kt);
+    if (p.tail.splits > 1) p.tail.whole = (int)(pairs - rest);
+  }
   p.key_splits = parts_of(kt * s->k_heads * b, (int)std::min<int64_t>(1 << 20, qt * group));
   p.query_splits = parts_of(qt * s->q_heads * b, (int)kt);
   p.few = kt <= kFewStages || s->causal || key_lengths;
@@ -1591,13 +1628,13 @@ int forward_launch(ForwardParams& p, cudaStream_t st) {
   const size_t smem = (size_t)kForwardTiles<D> * kTileBytes<D> + sizeof(ForwardShared<D>);
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return ANEMOI_SM100_ELAUNCH;
-  const Geometry& g = p.g;
-  kernel<<<dim3((g.q_tokens + 2 * kTile - 1) / (2 * kTile), g.q_heads, g.batch * g.splits), kThreads, smem, st>>>(p);
+  const int parted = p.tail.pairs - p.tail.whole;
+  kernel<<<p.tail.whole + parted * p.tail.splits, kThreads, smem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
-  if (g.splits == 1) return ANEMOI_SM100_OK;
-  const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens, per_block = 128 / (D / 4);
-  if (layer::launch(join_forward_kernel<D, kBf16>, dim3((unsigned)((rows_all + per_block - 1) / per_block)), dim3(128), 0, st,
-                    (const float*)p.partial, g.splits, rows_all, g.q_heads, g.q_tokens, p.o, p.out, p.lse) != cudaSuccess)
+  if (parted == 0) return ANEMOI_SM100_OK;
+  constexpr int kRows = 128 / (D / 4);
+  if (layer::launch(join_forward_kernel<D, kBf16>, dim3((unsigned)(parted * (2 * kTile / kRows))), dim3(128), 0, st, p) !=
+      cudaSuccess)
     return ANEMOI_SM100_ELAUNCH;
   return ANEMOI_SM100_OK;
 }
@@ -1664,9 +1701,8 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 extern "C" int64_t anemoi_sm100_dense_attention_workspace(const anemoi_sm100_dense_shape* s) {
   const int bad = check(s);
   if (bad != ANEMOI_SM100_OK) return bad;
-  const Plan plan = plan_of(s);
-  const int64_t rows_all = (int64_t)s->batch * s->q_heads * s->q_tokens;
-  return plan.forward_splits > 1 ? plan.forward_splits * rows_all * (s->head_dim + 1) * (int64_t)sizeof(float) : 0;
+  const TailSplit t = plan_of(s).tail;
+  return (int64_t)(t.pairs - t.whole) * t.splits * 2 * kTile * (s->head_dim + 1) * (int64_t)sizeof(float);
 }
 
 extern "C" int anemoi_sm100_dense_attention(const anemoi_sm100_dense_shape* s, const void* q, const void* k, const void* v,
@@ -1692,7 +1728,7 @@ extern "C" int anemoi_sm100_dense_attention(const anemoi_sm100_dense_shape* s, c
   if (!encode(&p.q, tq, bf16, d, s->batch) || !encode(&p.k, tk, bf16, d, s->batch) || !encode(&p.v, tv, bf16, d, s->batch))
     return ANEMOI_SM100_EINVAL;
   geometry(p.g, s, q_lengths, k_lengths, status);
-  p.g.splits = plan_of(s).forward_splits;
+  p.tail = plan_of(s).tail;
   p.out = out;
   p.lse = lse;
   p.partial = static_cast<float*>(workspace);
@@ -1760,16 +1796,12 @@ extern "C" int anemoi_sm100_dense_attention_backward(const anemoi_sm100_dense_sh
   }
   p.q_partial = reinterpret_cast<float*>(w);
   p.k_partial = p.q_partial + (plan.query_splits > 1 ? plan.query_splits * q_rows * d : 0);
-  p.q_rows = q;
-  p.do_rows = dout;
   p.lse = lse;
   p.delta = delta;
   p.norms = norms;
   p.dq = dq;
   p.dk = dk;
   p.dv = dv;
-  p.sdo = t[0].s;
-  p.sq = t[1].s;
   p.sdq = t[5].s;
   p.sdk = t[6].s;
   p.sdv = t[7].s;
