@@ -325,7 +325,7 @@ struct ForwardShared {
       o_done[2], side;
 };
 // Every which pair of exponentials takes the polynomial.
-constexpr int kForwardPoly = 4, kBackwardPoly = 4;
+constexpr int kForwardPoly = 4, kBackwardPoly = 4, kFewPoly = 4;
 // Roles of the waits: warpgroups of different register counts cannot share a function.
 enum { kFeedRole = 0, kSoftmaxRole = 1 };
 // Registers per thread: 168 at launch, of which the feeding warps leave most to the softmax warps (a row of 128 scores each).
@@ -1408,9 +1408,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       warp_arrive(&s->s_read[t]);
 #pragma unroll
       for (int j = 0; j < 128; j += 2) {
-        const float2 a = ffma2(make_float2(v[j], v[j + 1]), c2, l2);
-        v[j] = exp2_approx(a.x);
-        v[j + 1] = exp2_approx(a.y);
+        const float2 e = exp2_pair<kFewPoly>(ffma2(make_float2(v[j], v[j + 1]), c2, l2), j / 2);
+        v[j] = e.x;
+        v[j + 1] = e.y;
       }
       wait(wc, &s->dp_full[t], i & 1, 99);
       tc_fence_after_sync();
