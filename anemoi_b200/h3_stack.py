@@ -15,6 +15,10 @@ external to the reference repository); only what the reference fixes is used:
 Assumed, because the reference does not state them: feed-forward width 14,336 and 64 rotary
 channels.  The projections are plain library GEMMs (model glue); the producer fusion, the
 exchange relayouts and the attention are this library's kernels.
+
+``step`` is the inference harness.  ``fused_step`` is the same stack on one GPU with its norms, gates and modulation fused
+(``modulation``), positions of video layouts (``producer.fused_qknorm_axial_rope``) and, by default, dense attention
+(``dense``): every piece has a gradient, so that it is also the forward pass of a tuning step.
 """
 
 from __future__ import annotations
@@ -25,6 +29,9 @@ import torch
 import torch.nn.functional as F
 
 from . import ulysses
+from .dense import dense_attention
+from .modulation import fused_gate_norm_modulate, fused_gate_residual, fused_norm_modulate
+from .producer import AxialRotary, fused_qknorm_axial_rope
 
 
 @dataclass(frozen=True)
@@ -110,6 +117,30 @@ class H3BlockStack:
             x = x + gate1 * (attn.reshape(rows, c.inner) @ blk["wo"])
             h = self._norm(x, c.eps) * (1 + scale2) + shift2
             x = x + gate2 * ((F.silu(h @ blk["w1"]) * (h @ blk["w3"])) @ blk["w2"])
+        return x
+
+    def fused_step(self, x: torch.Tensor, positions: torch.Tensor, rotary: AxialRotary, attention_fn=None) -> torch.Tensor:
+        """One denoising step of ``x`` ``[B, rows, width]`` with the fused kernels; autograd records it where ``x`` or weights
+        in ``blocks`` ask for gradients.
+
+        ``positions`` ``[rows, axes]`` or ``[B, rows, axes]`` (``producer.axial_positions`` for a video layout);
+        ``attention_fn(q, k, v)`` takes and returns ``[B, rows, heads, D]`` (default: ``dense_attention``)."""
+        c = self.config
+        batch, rows, _ = x.shape
+        attention_fn = dense_attention if attention_fn is None else attention_fn
+        mods = [blk["mod"].unbind(0) for blk in self.blocks]
+        h = fused_norm_modulate(x, mods[0][1], mods[0][0], eps=c.eps)
+        for i, blk in enumerate(self.blocks):
+            _, _, gate1, shift2, scale2, gate2 = mods[i]
+            q, k, v = ((h @ blk[name]).view(batch, rows, c.heads, c.head_dim) for name in ("wq", "wk", "wv"))
+            q, k = fused_qknorm_axial_rope(q, k, blk["qn"], blk["kn"], positions, rotary, c.eps)
+            y = attention_fn(q, k, v).reshape(batch, rows, c.inner) @ blk["wo"]
+            x, h = fused_gate_norm_modulate(x, y, gate1, scale2, shift2, eps=c.eps)
+            y = (F.silu(h @ blk["w1"]) * (h @ blk["w3"])) @ blk["w2"]
+            if i + 1 < len(self.blocks):
+                x, h = fused_gate_norm_modulate(x, y, gate2, mods[i + 1][1], mods[i + 1][0], eps=c.eps)
+            else:
+                x = fused_gate_residual(x, y, gate2, eps=c.eps)
         return x
 
 

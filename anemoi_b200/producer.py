@@ -22,6 +22,7 @@ from functools import cached_property, lru_cache
 import torch
 
 from . import native
+from .api import VisualLayout
 
 
 def fused_qknorm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -85,6 +86,15 @@ class AxialRotary:
                 out.append(self.theta ** -power / (2.0 * math.pi))
             first += n
         return (C.c_double * max(1, len(out)))(*out)
+
+
+def axial_positions(layout: VisualLayout, device=None) -> torch.Tensor:
+    """Positions ``(tokens, 3)`` (time, height, width; int32) of a layout's sequence: prefix token i stands at (i, i, i), the
+    video token of frame f, row y, column x at the prefix's length + (f, y, x)."""
+    prefix, (frames, height, width) = layout.prefix_tokens, layout.video_shape
+    axes = [torch.arange(n, dtype=torch.int32, device=device) for n in (frames, height, width)]
+    video = torch.stack(torch.meshgrid(*axes, indexing="ij"), dim=-1).reshape(-1, 3) + prefix
+    return torch.cat((torch.arange(prefix, dtype=torch.int32, device=device)[:, None].expand(prefix, 3), video))
 
 
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -247,4 +257,4 @@ def fused_qknorm_axial_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor 
     return _axial_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, rotary, eps)
 
 
-__all__ = ["AxialRotary", "fused_qknorm_axial_rope", "fused_qknorm_axial_rope_backward", "fused_qknorm_rope"]
+__all__ = ["AxialRotary", "axial_positions", "fused_qknorm_axial_rope", "fused_qknorm_axial_rope_backward", "fused_qknorm_rope"]
