@@ -1603,6 +1603,13 @@ int parts_of(int64_t ctas, int steps) {
   if (ctas >= rows::kSms) return 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>(rows::kSms / ctas, steps / 2));
 }
+// Parts of the gradient's walks, from the cost of a step (2,500 cycles of a key tile's, 1,900 of a query tile's, and 5,000 for
+// a CTA's start and end): none longer than an SM's share of all the work, nor, where there is little, than four steps.  4 heads
+// of 1,024 tokens: two parts each, one wave of CTAs; four parts each, in two waves, took 17 us instead of 13.
+int share_of(double walk, double all, int64_t steps) {
+  const double most = std::max(all / rows::kSms, 10000.0);
+  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)ceil(walk / most), steps / 2));
+}
 
 struct Plan {
   TailSplit tail;
@@ -1622,8 +1629,10 @@ Plan plan_of(const anemoi_sm100_dense_shape* s, bool key_lengths = false) {
     p.tail.splits = parts_of(rest, (int)kt);
     if (p.tail.splits > 1) p.tail.whole = (int)(pairs - rest);
   }
-  p.key_splits = parts_of(kt * s->k_heads * b, (int)std::min<int64_t>(1 << 20, qt * group));
-  p.query_splits = parts_of(qt * s->q_heads * b, (int)kt);
+  const double key_walk = 2500.0 * qt * group, query_walk = 1900.0 * kt;
+  const double all = (key_walk + 5000.0) * kt * s->k_heads * b + (query_walk + 5000.0) * qt * s->q_heads * b;
+  p.key_splits = share_of(key_walk, all, qt * group);
+  p.query_splits = share_of(query_walk, all, kt);
   p.few = kt <= kFewStages || s->causal || key_lengths;
   // one walk for every SM
   const int64_t ctas = (std::min<int64_t>(kt, kFewStages) + 1) / 2 * s->q_heads * b;

@@ -25,6 +25,10 @@ from . import native
 from .executor import _status_word
 
 
+def _packed_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _layout(t: torch.Tensor):
     """What of a tensor decides how a call runs."""
     return t.shape, t.stride(), t.dtype, t.device
@@ -102,7 +106,7 @@ def _forward(q, k, v, scale, causal, query_lengths, key_lengths):
         return (torch.zeros(q.shape, dtype=q.dtype, device=q.device),
                 torch.full(plan.lse_shape, -math.inf, dtype=torch.float32, device=q.device))
     _aligned(q=q, k=k, v=v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _packed_like(q)
     lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=q.device)
     native.dense_attention(plan.shape, q, k, v, q_lengths, k_lengths, plan.forward_strides, out, lse, plan.forward_bytes,
                            _status_word(q.device))
@@ -124,7 +128,7 @@ def dense_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
     if plan.empty:
         return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     _aligned(grad_out=grad_out, q=q, k=k, v=v, out=out)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = (_packed_like(t) for t in (q, k, v))
     native.dense_attention_backward(plan.shape, grad_out, q, k, v, out, lse, q_lengths, k_lengths, strides, dq, dk, dv,
                                     plan.backward_bytes[k_lengths is not None], _status_word(q.device))
     return dq, dk, dv

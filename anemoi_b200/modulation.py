@@ -39,6 +39,10 @@ class GateNormGradients(NamedTuple):
     post_weight: torch.Tensor | None
 
 
+def _packed_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _layout(t: torch.Tensor | None):
     """What of a tensor decides how a call runs."""
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
@@ -210,8 +214,8 @@ def _aligned(**tensors) -> None:
 def _forward(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, with_norm=True):
     plan = _plan(_layout(x), _layout(y), _layout(gate), _layout(scale), _layout(shift), _layout(weight),
                  _layout(post_weight), eps, norm, post_norm)
-    x_out = None if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_norm else None
+    x_out = None if y is None else _packed_like(x)
+    h = _packed_like(x) if with_norm else None
     if plan.rows:
         _aligned(x=x, y=y)
         native.gate_norm_modulate(
@@ -227,8 +231,8 @@ def _backward(dx_out, dh, x_out, y, gate, scale, shift, weight, post_weight, eps
     if dx_out is None and dh is None:
         raise ValueError("one of the outputs' gradients is needed")
     strides = plan.backward_strides(_layout(dx_out), _layout(dh))
-    dx = torch.empty(x_out.shape, dtype=x_out.dtype, device=x_out.device)
-    dy = None if y is None else torch.empty(x_out.shape, dtype=x_out.dtype, device=x_out.device)
+    dx = _packed_like(x_out)
+    dy = None if y is None else _packed_like(x_out)
     make = torch.empty if plan.rows else torch.zeros
     normed = dh is not None
 
@@ -236,8 +240,10 @@ def _backward(dx_out, dh, x_out, y, gate, scale, shift, weight, post_weight, eps
         if t is None or not want:
             return None
         # the argument's own shape, unless one row of it served several groups
-        shape = t.shape if plan.mod_rows[name] == plan.groups else (plan.groups, plan.width)
-        return make(shape, dtype=t.dtype, device=t.device)
+        if plan.mod_rows[name] == plan.groups and plan.rows:
+            return _packed_like(t)
+        return make(t.shape if plan.mod_rows[name] == plan.groups else (plan.groups, plan.width), dtype=t.dtype,
+                    device=t.device)
 
     dgate, dscale, dshift = (sums(gate, "gate", wanted[2]), sums(scale, "scale", wanted[3] and normed),
                              sums(shift, "shift", wanted[4] and normed))

@@ -100,6 +100,10 @@ def axial_positions(layout: VisualLayout, device=None) -> torch.Tensor:
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
+def _packed_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _layout(t: torch.Tensor | None):
     """What of a tensor decides how a call runs."""
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
@@ -188,8 +192,8 @@ def _packed16(t: torch.Tensor | None) -> torch.Tensor | None:
 
 def _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, inplace):
     plan = _axial_plan(_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(positions), rotary, eps)
-    q_out = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = k if inplace or k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out = q if inplace else _packed_like(q)
+    k_out = k if inplace or k is None else _packed_like(k)
     if not plan.empty:
         _aligned(q=q, k=k)
         native.axial_rope(plan.shape, q, k, _packed16(q_weight), _packed16(k_weight), positions.contiguous(),
@@ -200,8 +204,8 @@ def _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, inplace):
 def _axial_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, rotary, eps, wanted=(True, True)):
     plan = _axial_plan(_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(positions), rotary, eps)
     strides = plan.backward_strides(_layout(dq_out), _layout(dk_out))
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dq = _packed_like(q)
+    dk = None if k is None else _packed_like(k)
     make = torch.zeros if plan.empty else torch.empty
     dq_weight, dk_weight = (None if w is None or not want else make(w.shape, dtype=w.dtype, device=w.device)
                             for w, want in zip((q_weight, k_weight), wanted))
