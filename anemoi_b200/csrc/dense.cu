@@ -1588,9 +1588,9 @@ int check(const anemoi_sm100_dense_shape* s) {
   if (s == nullptr || s->batch <= 0 || s->q_heads <= 0 || s->k_heads <= 0 || s->q_heads % s->k_heads || s->q_tokens <= 0 ||
       s->k_tokens <= 0 || (s->head_dim != 64 && s->head_dim != 128) || !(s->scale > 0.0f) || !(s->scale < INFINITY))
     return ANEMOI_SM100_EINVAL;
-  // tile and row counts in 32 bits, with room for the splits
+  // tile and row counts in 32 bits, with room for the splits (2^24 tiles are 2^31 rows)
   if (s->q_tokens > 0x3fffffff || s->k_tokens > 0x3fffffff || s->q_heads > 65535 || s->batch > 4095 ||
-      (int64_t)s->batch * s->q_heads * ((std::max(s->q_tokens, s->k_tokens) + kTile - 1) / kTile) > (1 << 25))
+      (int64_t)s->batch * s->q_heads * ((std::max(s->q_tokens, s->k_tokens) + kTile - 1) / kTile) > (1 << 24))
     return ANEMOI_SM100_ELIMIT;
   return ANEMOI_SM100_OK;
 }

@@ -12,6 +12,10 @@ reads key head ``h // (Hq // Hk)``); strided views with a contiguous last dimens
 ``query_lengths`` / ``key_lengths``: int32 ``[B]`` on the device, how many leading tokens of each sample count (values are
 clamped to the tensors' lengths).  What stands behind them is not used, be it NaN; the outputs' rows there are zeros, and so
 are those of queries that see no key.  ``causal``: query i of a sample sees the keys up to ``i + keys - queries`` of it.
+
+Precision: scores, softmax and sums are fp32; P and dS are rounded to the tensors' type as operands of the tensor cores (in
+fp16 scaled so that small ones keep their bits), the results once at the end.  The kernels' waits are bounded:
+``executor.last_status()`` is non-zero after one gave up, and the results of that call are not valid.
 """
 
 from __future__ import annotations
@@ -21,8 +25,7 @@ from functools import lru_cache
 
 import torch
 
-from . import native
-from .executor import _status_word
+from . import executor, native
 
 
 def _packed_like(t: torch.Tensor) -> torch.Tensor:
@@ -85,6 +88,17 @@ class _Plan:
 _plan = lru_cache(maxsize=256)(_Plan)
 
 
+def _status(device: torch.device) -> torch.Tensor:
+    """The device's status word, which its first call allocates and zeroes (``executor.last_status`` reads it)."""
+    word = executor._STATUS.get(device)
+    if word is None:
+        # recorded into a graph, it would be zero only once the graph had run
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first dense_attention call on a device must come before a capture")
+        word = executor._status_word(device)
+    return word
+
+
 def _aligned(**tensors) -> None:
     for name, t in tensors.items():
         if t.data_ptr() % 16:
@@ -109,7 +123,7 @@ def _forward(q, k, v, scale, causal, query_lengths, key_lengths):
     out = _packed_like(q)
     lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=q.device)
     native.dense_attention(plan.shape, q, k, v, q_lengths, k_lengths, plan.forward_strides, out, lse, plan.forward_bytes,
-                           _status_word(q.device))
+                           _status(q.device))
     return out, lse
 
 
@@ -130,7 +144,7 @@ def dense_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
     _aligned(grad_out=grad_out, q=q, k=k, v=v, out=out)
     dq, dk, dv = (_packed_like(t) for t in (q, k, v))
     native.dense_attention_backward(plan.shape, grad_out, q, k, v, out, lse, q_lengths, k_lengths, strides, dq, dk, dv,
-                                    plan.backward_bytes[k_lengths is not None], _status_word(q.device))
+                                    plan.backward_bytes[k_lengths is not None], _status(q.device))
     return dq, dk, dv
 
 

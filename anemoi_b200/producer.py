@@ -64,8 +64,8 @@ class AxialRotary:
     shared_frequencies: bool = False
 
     def __post_init__(self):
-        if not 1 <= len(self.sections) <= 4 or any(type(n) is not int or n < 0 for n in self.sections):
-            raise ValueError("sections must be 1 to 4 non-negative ints")
+        if type(self.sections) is not tuple or not 1 <= len(self.sections) <= 4 or any(type(n) is not int or n < 0 for n in self.sections):
+            raise ValueError("sections must be a tuple of 1 to 4 non-negative ints")
         if self.pairs > 64 or self.pairs % (4 if self.interleaved else 8):
             raise ValueError("the sections must add up to at most 64 pairs, a multiple of 8 (of 4 with interleaved pairs): "
                              "the sm_100a kernel moves whole 8-channel vectors")

@@ -249,7 +249,7 @@ def test_refusals():
     from anemoi_b200.producer import AxialRotary, _axial_plan, fused_qknorm_axial_rope
 
     for bad in (dict(sections=()), dict(sections=(1,) * 5), dict(sections=(4, 2)), dict(sections=(-8, 16)), dict(sections=(72,)),
-                dict(sections=(8.0,)), dict(sections=(8,), theta=0.0), dict(sections=(8,), theta=math.inf), dict(sections=(4,))):
+                dict(sections=(8.0,)), dict(sections=[8]), dict(sections=(8,), theta=0.0), dict(sections=(8,), theta=math.inf), dict(sections=(4,))):
         with pytest.raises(ValueError):
             AxialRotary(**bad)
     assert AxialRotary((4,), interleaved=True).pairs == 4

@@ -5,6 +5,7 @@ and their results at the end; products are exact, sums are fp32.  fp32 sums over
 and the exponentials (2^-22, of arguments below 2^6 that are good to 2^-17) stay within ``w = 1e-4`` of the sum of the magnitudes
 (1,000 terms x 2^-24 = 6e-5, plus 2^-17 and 2^-22).  With s = the sum of magnitudes that a result adds up:
 
+(longer sums: their terms x 2^-24.)
     out   u s(P |v|)                + u |out| + w s
     dV    u s(P |dO|)               + u |dV|  + w s
     e_ij  |error of dS_ij| <= u |dS_ij| + P_ij |delta_i given - delta_i| + w P_ij (|dO_i| . |v_j| + |dO_i| . |out_i|)
@@ -37,6 +38,7 @@ def _reference(q, k, v, do, out, scale, causal, q_lens, k_lens):
     b, nq, hq, d = q.shape
     nk, hk = k.shape[1:3]
     group = hq // hk
+    w = max(W, max(nk, nq * group) * 2.0 ** -24)
     val = {n: torch.zeros(t.shape, dtype=torch.float64, device=q.device) for n, t in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
     bnd = {n: torch.zeros_like(t) for n, t in val.items()}
     val["lse"] = torch.full((b, hq, nq), -math.inf, dtype=torch.float64, device=q.device)
@@ -61,7 +63,7 @@ def _reference(q, k, v, do, out, scale, causal, q_lens, k_lens):
             o = p @ vs
             val["out"][s, :, h] = o
             mag = p @ vs.abs()
-            bnd["out"][s, :, h] = (u + W) * mag + u * o.abs() + tiny_p * vs.abs().amax(0)
+            bnd["out"][s, :, h] = (u + w) * mag + u * o.abs() + tiny_p * vs.abs().amax(0)
             if do is None:
                 continue
             given = out[s, :, h].double()
@@ -69,13 +71,13 @@ def _reference(q, k, v, do, out, scale, causal, q_lens, k_lens):
             dp = g @ vs.T
             ds = p * (dp - delta[:, None])
             wide = g.abs() @ vs.abs().T + (g.abs() * o.abs()).sum(-1)[:, None]
-            e = u * ds.abs() + p * (used - delta).abs()[:, None] + W * p * wide + torch.where(seen, tiny_ds, 0.0)
+            e = u * ds.abs() + p * (used - delta).abs()[:, None] + w * p * wide + torch.where(seen, tiny_ds, 0.0)
             val["dq"][s, :, h] = scale * ds @ ks
-            bnd["dq"][s, :, h] = scale * (e @ ks.abs() + W * ds.abs() @ ks.abs())
+            bnd["dq"][s, :, h] = scale * (e @ ks.abs() + w * ds.abs() @ ks.abs())
             val["dk"][s, :, h // group] += scale * ds.T @ qs
-            bnd["dk"][s, :, h // group] += scale * (e.T @ qs.abs() + W * ds.abs().T @ qs.abs())
+            bnd["dk"][s, :, h // group] += scale * (e.T @ qs.abs() + w * ds.abs().T @ qs.abs())
             val["dv"][s, :, h // group] += p.T @ g
-            bnd["dv"][s, :, h // group] += (u + W) * p.T @ g.abs() + (2.0 ** -40 * g.abs().sum(0) if half else 0.0)
+            bnd["dv"][s, :, h // group] += (u + w) * p.T @ g.abs() + (2.0 ** -40 * g.abs().sum(0) if half else 0.0)
     for n in ("dq", "dk", "dv"):
         bnd[n] += u * (val[n].abs() + bnd[n])
         if half:
@@ -284,6 +286,48 @@ def test_captured_on_another_stream(native_library):
 
 
 @pytest.mark.gpu
+def test_the_first_call_is_not_captured(native_library):
+    """The status word that a graph would allocate is zero only once that graph has run."""
+    from anemoi_b200 import executor
+    from anemoi_b200.dense import dense_attention
+
+    q, k, v, do = _inputs(1, 40, 40, 1, 1, 64, torch.float16, seed=13)
+    _run(q, k, v, do)
+    word = executor._STATUS.pop(q.device)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="before a capture"):
+                dense_attention(q, k, v)
+    finally:
+        executor._STATUS[q.device] = word
+    assert executor.last_status(q.device) == 0
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(native_library):
+    """Calls of two streams run beside each other with workspaces of their own."""
+    a, b = _inputs(1, 300, 2000, 2, 2, 64, torch.float16, seed=14), _inputs(2, 500, 100, 4, 2, 128, torch.bfloat16, seed=15)
+    want = [_run(*t) for t in (a, b)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(5):
+        for i, t in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i] = _run(*t)
+    torch.cuda.synchronize()
+    for x, y in zip(got, want):
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1]) and all(torch.equal(m, n) for m, n in zip(x[2], y[2]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq, nk, hq, hk", [(40, 5000, 4, 4), (5000, 40, 8, 2), (300, 9000, 2, 1), (2000, 1000, 12, 12)])
+def test_split_walks(native_library, nq, nk, hq, hk):
+    """Few CTAs with long walks: parts of keys and of queries that are joined; some tiles whole beside tiles in parts."""
+    _check(*_inputs(1, nq, nk, hq, hk, 64, torch.bfloat16, seed=nq, do_std=0.05))
+
+
+@pytest.mark.gpu
 def test_empty_sides(native_library):
     q, k, v, do = _inputs(2, 5, 3, 2, 1, 64, torch.bfloat16, seed=12)
     out, lse, grads = _run(q, k[:, :0], v[:, :0], do)
@@ -312,7 +356,7 @@ def test_the_library_refuses(native_library):
                    dict(scale=float("nan")), dict(scale=float("inf")), dict(q_tokens=0), dict(k_tokens=-1)):
         shape = native.DenseShape(**{**good, **change})
         assert native_library.anemoi_sm100_dense_attention_workspace(C.byref(shape)) == -1, change
-    for change in (dict(batch=5000), dict(q_tokens=1 << 30), dict(batch=4000, q_tokens=1 << 20)):
+    for change in (dict(batch=5000), dict(q_tokens=1 << 30), dict(batch=4000, q_tokens=1 << 18)):
         shape = native.DenseShape(**{**good, **change})
         assert native_library.anemoi_sm100_dense_attention_workspace(C.byref(shape)) == -3, change
     shape, strides = native.DenseShape(**good), (C.c_int64 * 12)(*([2048, 256, 64] * 4))
