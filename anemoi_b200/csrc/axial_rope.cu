@@ -262,10 +262,11 @@ __global__ void __launch_bounds__(kThreads, forward_blocks(kRows)) forward_kerne
 // The gradient, the same way.  A block has queries or keys and walks units a grid apart, so that a thread's 8 sums of the
 // weight stay in registers; they are added over its groups at the end, and the blocks' by sums_kernel.  Blocks are many more
 // than fit at once: loads of one are in flight under the arithmetic of others (a ring of copies ahead, in blocks that stay,
-// cost more instructions than it hid: 150 us for 32,256 tokens of 32 heads of 64).
+// cost more instructions than it hid: 150 us for 32,256 tokens of 32 heads of 64; loads of the next unit ahead in registers:
+// 117 to 142; three blocks per SM at 80 registers, which spill: 129; two: 98).
 constexpr int kBackwardRows = 4;
 template <typename T, int D, bool interleaved>
-__global__ void __launch_bounds__(kThreads, 3) backward_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_constant__ RopeParams p) {
   constexpr int kLanes = D / 8, kGroups = kThreads / kLanes, kUnits = 32 / kLanes, kRows = kBackwardRows;
   __shared__ __align__(16) float tables[kThreads / 32][kUnits * D];
   __shared__ float sums[kGroups][D];
@@ -405,7 +406,7 @@ int rows_of(const anemoi_sm100_axial_rope_shape* s) {
   return heads > 4 && rows >= 8 * groups ? 8 : heads > 2 && rows >= 2 * groups ? 4 : 1;
 }
 
-// The gradient's blocks of a sample: as many as its units fill, or as few as leave every SM 32 of them in all (a sum of the
+// The gradient's blocks of a sample: as many as its units fill, or as few as leave every SM 16 of them in all (a sum of the
 // weights has that many parts), each of as many turns.
 struct BackwardPlan {
   int q_blocks, k_blocks;
@@ -414,7 +415,7 @@ BackwardPlan plan_of(const anemoi_sm100_axial_rope_shape* s) {
   const int64_t groups = kThreads / (s->head_dim / 8);
   const int64_t q = (s->tokens * ((s->q_heads + kBackwardRows - 1) / kBackwardRows) + groups - 1) / groups;
   const int64_t k = (s->tokens * ((s->k_heads + kBackwardRows - 1) / kBackwardRows) + groups - 1) / groups;
-  const int64_t turns = ((q + k) * s->batch + kSms * 32 - 1) / (kSms * 32);
+  const int64_t turns = ((q + k) * s->batch + kSms * 16 - 1) / (kSms * 16);
   return {(int)((q + turns - 1) / turns), (int)((k + turns - 1) / turns)};
 }
 

@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
         }
         const float base = m == -INFINITY ? 0.0f : -m * c;
         const float2 c2 = make_float2(c, c), base2 = make_float2(base, base);
-        float2 sum2 = make_float2(0.0f, 0.0f);
+        float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         // (with keys hidden every probability is the unit's: the polynomial has no zero)
         auto form = [&](auto every) {
 #pragma unroll
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
             for (int j = 0; j < 32; j += 2) {
               const float2 e =
                   exp2_pair<decltype(every)::value>(ffma2(make_float2(v[c0 + j], v[c0 + j + 1]), c2, base2), (c0 + j) / 2);
-              sum2 = fadd2(sum2, e);
+              sum2[j / 2 % 2] = fadd2(sum2[j / 2 % 2], e);
               packed[j / 2] = pack2<kBf16>(e.x, e.y);
             }
             if (kApart && c0 == 0 && i > 0) {
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
         } else {
           form(std::integral_constant<int, kForwardPoly>{});
         }
-        sum += sum2.x + sum2.y;
+        sum += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
         tmem_wait_st();
         warp_arrive(&s->p_ready[t]);
       }
