@@ -328,6 +328,21 @@ def test_split_walks(native_library, nq, nk, hq, hk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, d", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("nk", [1, 100, 300, 700])
+@pytest.mark.parametrize("q_lens, k_lens", [(None, None), ([4200, 130, 0, 2001], None), ([4000, 4200, 128, 1], [0, 1, 130, 700])])
+def test_short_walks_of_many_queries(native_library, dtype, d, causal, nk, q_lens, k_lens):
+    """Enough query tiles that a CTA takes several, some without keys: at the start, between others or at the end."""
+    q, k, v, do = _inputs(4, 4200, nk, 16, 4, d, dtype, 12)
+    if q_lens is not None:
+        for t, lens in ((q, q_lens), (do, q_lens), (k, k_lens), (v, k_lens)):
+            for s in range(4 if lens is not None else 0):
+                t[s, lens[s] :] = math.nan
+    _check(q, k, v, do, causal=causal, q_lens=q_lens, k_lens=k_lens)
+
+
+@pytest.mark.gpu
 def test_empty_sides(native_library):
     q, k, v, do = _inputs(2, 5, 3, 2, 1, 64, torch.bfloat16, seed=12)
     out, lse, grads = _run(q, k[:, :0], v[:, :0], do)
