@@ -60,14 +60,14 @@ class _Plan:
         _, k_tokens, k_heads, _ = k[0]
         if k_heads == 0 or q_heads == 0 or q_heads % k_heads:
             raise ValueError("q's heads must be a multiple of k's")
-        scale = dim ** -0.5 if scale is None else float(scale)
+        scale = dim ** -0.5 if scale is None else scale
         if not (scale > 0.0 and math.isfinite(scale)):
             raise ValueError("scale must be positive")
         self.empty = 0 in (batch, q_tokens, k_tokens)
         self.lse_shape = (batch, q_heads, q_tokens)
         self.strides = (q[1][:3], k[1][:3], v[1][:3])
         self.shape = native.DenseShape(batch=batch, q_heads=q_heads, k_heads=k_heads, q_tokens=q_tokens, k_tokens=k_tokens,
-                                       head_dim=dim, causal=int(bool(causal)), is_bf16=int(dtype == torch.bfloat16),
+                                       head_dim=dim, causal=int(causal), is_bf16=int(dtype == torch.bfloat16),
                                        scale=scale)
         self.forward_bytes, self.backward_bytes = (0, (0, 0)) if self.empty else native.dense_attention_bytes(self.shape)
         packed = ((q_tokens * q_heads * dim, q_heads * dim, dim), (k_tokens * k_heads * dim, k_heads * dim, dim))
@@ -85,7 +85,12 @@ class _Plan:
         return native.strides_array([n for t in (grad_out[1][:3], *self.strides, out[1][:3], q, k, k) for n in t])
 
 
-_plan = lru_cache(maxsize=256)(_Plan)
+_found = lru_cache(maxsize=256)(_Plan)
+
+
+def _plan(q, k, v, scale, causal) -> _Plan:
+    # (by values: a tensor as scale would be found by its identity)
+    return _found(_layout(q), _layout(k), _layout(v), None if scale is None else float(scale), bool(causal))
 
 
 def _status(device: torch.device) -> torch.Tensor:
@@ -114,7 +119,7 @@ def _lengths(t: torch.Tensor | None, name: str, q: torch.Tensor) -> torch.Tensor
 
 
 def _forward(q, k, v, scale, causal, query_lengths, key_lengths):
-    plan = _plan(_layout(q), _layout(k), _layout(v), scale, causal)
+    plan = _plan(q, k, v, scale, causal)
     q_lengths, k_lengths = _lengths(query_lengths, "query_lengths", q), _lengths(key_lengths, "key_lengths", q)
     if plan.empty:
         return (torch.zeros(q.shape, dtype=q.dtype, device=q.device),
@@ -132,7 +137,7 @@ def dense_attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
                              query_lengths: torch.Tensor | None = None, key_lengths: torch.Tensor | None = None):
     """``(dq, dk, dv)`` from the gradient of ``out``; ``out`` and ``lse`` are what ``dense_attention`` gave for the same
     arguments.  Equal calls give equal bits."""
-    plan = _plan(_layout(q), _layout(k), _layout(v), scale, causal)
+    plan = _plan(q, k, v, scale, causal)
     q_lengths, k_lengths = _lengths(query_lengths, "query_lengths", q), _lengths(key_lengths, "key_lengths", q)
     if out.dtype != q.dtype or grad_out.dtype != q.dtype or out.device != q.device or grad_out.device != q.device:
         raise ValueError("grad_out and out must have q's dtype and device")
@@ -153,7 +158,7 @@ class _DenseAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, query_lengths, key_lengths, scale, causal):
         out, lse = _forward(q, k, v, scale, causal, query_lengths, key_lengths)
         ctx.save_for_backward(q, k, v, out, lse, query_lengths, key_lengths)
-        ctx.options = dict(scale=scale, causal=causal)
+        ctx.options = dict(scale=None if scale is None else float(scale), causal=bool(causal))
         ctx.mark_non_differentiable(lse)
         return out, lse
 

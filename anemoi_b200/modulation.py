@@ -286,6 +286,7 @@ class _GateNorm(torch.autograd.Function):
 
 def _call(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, with_norm):
     """The outputs that there are, recorded by autograd where an argument asks for it."""
+    eps = float(eps)  # (plans are found by values: a tensor would be found by its identity)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (x, y, gate, scale, shift, weight, post_weight)):
         return _GateNorm.apply(x, y, gate, scale, shift, weight, post_weight, eps, norm, post_norm, with_norm)
@@ -325,7 +326,7 @@ def fused_gate_norm_modulate_backward(dx_out: torch.Tensor | None, dh: torch.Ten
     ``x_out`` is the residual stream that it returned.  ``x`` of the result is the gradient of the stream before the block,
     which is also that of ``x_out``; ``shift``'s has the shape of ``scale`` (None without ``scale``)."""
     # (shift's values are not needed, its shape is scale's)
-    return _backward(dx_out, dh, x_out, y, gate, scale, scale, weight, post_weight, eps, norm, post_norm)
+    return _backward(dx_out, dh, x_out, y, gate, scale, scale, weight, post_weight, float(eps), norm, post_norm)
 
 
 __all__ = ["GateNormGradients", "fused_gate_norm_modulate", "fused_gate_norm_modulate_backward", "fused_gate_residual",

@@ -245,9 +245,16 @@ def fused_qknorm_axial_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: t
 
     ``positions``: ``(seq, axes)`` or ``(B, seq, axes)``, whole or fractional.  New tensors, recorded by autograd; with
     ``inplace`` q and k are overwritten, as ``fused_qknorm_rope`` does, which autograd cannot go through."""
+    eps = float(eps)  # (plans are found by values: a tensor would be found by its identity)
     recorded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
-    if inplace and recorded:
-        raise ValueError("inplace=True overwrites what the gradient needs")
+    if inplace:
+        if recorded:
+            raise ValueError("inplace=True overwrites what the gradient needs")
+        for name, t in (("q", q), ("k", k)):
+            if t is not None and any(size > 1 and step == 0 for size, step in zip(t.shape, t.stride())):
+                raise ValueError(f"inplace=True needs a place of its own for every element of {name}")
+        if k is not None and q.numel() and q.data_ptr() == k.data_ptr():
+            raise ValueError("inplace=True needs q and k apart")
     if not recorded:
         return _axial_forward(q, k, q_weight, k_weight, positions, rotary, eps, bool(inplace))
     return _AxialRope.apply(q, k, q_weight, k_weight, positions, rotary, eps)
@@ -258,7 +265,7 @@ def fused_qknorm_axial_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor 
                                      positions: torch.Tensor, rotary: AxialRotary, eps: float = 1e-6):
     """``(dq, dk, dq_weight, dk_weight)`` of ``fused_qknorm_axial_rope`` from the gradients of its outputs; ``q`` and ``k``
     are its inputs.  Equal calls give equal bits."""
-    return _axial_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, rotary, eps)
+    return _axial_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, rotary, float(eps))
 
 
 __all__ = ["AxialRotary", "axial_positions", "fused_qknorm_axial_rope", "fused_qknorm_axial_rope_backward", "fused_qknorm_rope"]

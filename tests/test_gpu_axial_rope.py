@@ -245,6 +245,24 @@ def test_captured_and_no_tokens(native_library):
     assert not grads[2].any() and grads[0].shape == (1, 0, 6, 128)
 
 
+@pytest.mark.gpu
+def test_an_eps_that_changes_and_places_that_are_shared(native_library):
+    from anemoi_b200.producer import AxialRotary, fused_qknorm_axial_rope
+
+    q, k, qw, kw, *_ = _inputs(1, 50, 4, 4, 128, torch.bfloat16, True, 8)
+    rotary, at, eps = AxialRotary((8, 12, 12)), _grid(50), torch.tensor(0.0)
+    for value in (0.5, 3.0):
+        eps.fill_(value)
+        got, want = (fused_qknorm_axial_rope(q, k, qw, kw, at, rotary, e) for e in (eps, value))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # in place: rows that lie on one another, and queries that are the keys
+    one = q[:, :, :1].expand_as(q)
+    for a, b in ((one, k), (q, one), (q, q)):
+        with pytest.raises(ValueError, match="inplace"):
+            fused_qknorm_axial_rope(a, b, qw, kw, at, rotary, EPS, inplace=True)
+    assert fused_qknorm_axial_rope(one, k, qw, kw, at, rotary, EPS)[0].shape == q.shape
+
+
 def test_refusals():
     from anemoi_b200.producer import AxialRotary, _axial_plan, fused_qknorm_axial_rope
 

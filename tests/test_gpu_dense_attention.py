@@ -351,6 +351,18 @@ def test_empty_sides(native_library):
     assert out.shape == (2, 0, 2, 64) and not grads[1].any() and not grads[2].any()
 
 
+@pytest.mark.gpu
+def test_a_scale_that_changes_in_place(native_library):
+    """Calls are told apart by the value of the scale, not by the object."""
+    from anemoi_b200.dense import dense_attention
+
+    q, k, v, _ = _inputs(1, 200, 300, 2, 2, 64, torch.float16, 14)
+    scale = torch.tensor(0.1)
+    for value in (0.125, 0.5):
+        scale.fill_(value)
+        assert torch.equal(dense_attention(q, k, v, scale=scale), dense_attention(q, k, v, scale=value))
+
+
 def test_refusals():
     """What the call refuses before it looks for a GPU, and the library before it launches anything."""
     from anemoi_b200.dense import dense_attention

@@ -277,6 +277,17 @@ def test_captured(native_library):
     assert all(a is None or torch.equal(a, b) for a, b in zip(got, both()))
 
 
+@pytest.mark.gpu
+def test_an_eps_that_changes_in_place(native_library):
+    """Calls are told apart by the value of eps, not by the object."""
+    from anemoi_b200.modulation import fused_norm_modulate
+
+    x, eps = torch.ones(4, 64, device="cuda", dtype=torch.bfloat16), torch.tensor(0.0)
+    for value in (1.0, 3.0):
+        eps.fill_(value)
+        assert torch.equal(fused_norm_modulate(x, eps=eps), fused_norm_modulate(x, eps=value))
+
+
 def _cpu(*shape, dtype=torch.bfloat16):
     return torch.zeros(*shape, dtype=dtype)
 
