@@ -12,7 +12,9 @@
 // All products run on tcgen05 (M = 128, fp32 accumulators in tensor memory), fed by tiled TMA with 128-byte swizzle straight
 // from the caller's strided tensors.  The backward pass is two kernels: one CTA per key tile sums dK and dV over the queries,
 // one per query tile sums dQ over the keys.  That forms S and dP twice (7 products instead of 5), but every sum is one CTA's,
-// in a fixed order: equal calls give equal bits, which atomic additions into dQ would not.
+// in a fixed order: equal calls give equal bits, which atomic additions into dQ would not.  33,272 tokens of 7 heads of 128:
+// 11.0 ms in a row of calls, 1.26 PFLOP/s of the tensor core at the 1.5 GHz that the power limit leaves (a plain product of
+// matrices keeps 1.4 there), 9.5 ms in a single one.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -306,7 +308,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 
 // Where a CTA stands: tile (of `tiles`), head (of `heads`), then what is left of its index.  A head's tiles follow one another,
 // so that they share keys and values in L2; under a causal mask, whose walks differ, the longest of all heads come first
-// (2 samples, 16 query and 4 key heads, 4,111 tokens: gradient 346 us head by head).
+// (2 samples, 16 query and 4 key heads, 4,111 tokens: gradient 330 us, head by head 346).
 struct Place {
   int tile, head, rest;
 };
@@ -330,6 +332,10 @@ __device__ __forceinline__ int key_end(const Geometry& g, int q0, int q_len, int
 // probabilities are formed, the tensor core runs the other tile's products.  Tensor memory: scores of the tiles at columns
 // 0 and 128, outputs at 256 and 256 + D, and the probabilities in place of the scores (64 columns), or, where D = 64 leaves
 // columns, at 384 and 448: the next scores are then computed as soon as these have been read, not after PV.
+// 16,128 tokens of 12 heads of 64: 964 us, 829 TFLOP/s, 2,830 cycles per stage and pair of tiles: 1,536 of the special-function
+// unit (with a quarter of the exponentials as polynomials; none: 1,052 us, a third: 1,013, half: 1,077), 1,024 of the tensor core,
+// 1,350 issue slots of each scheduler, in two chains per scheduler.  Four (half a row per thread, the halves' maxima exchanged
+// in shared memory) took 1,006 us, tiles that take turns at the exponentials 1,057.
 template <int D>
 struct ForwardShared {
   static constexpr int kStages = D == 64 ? 3 : 2;
@@ -771,7 +777,8 @@ __device__ __forceinline__ float lse2_of(const BackwardParams& p, int64_t flat, 
 // memory as they stand, and the tiles of Q and dO serve both ways (channels as K, tokens as K).  Two warpgroups take
 // 64 columns each.  Tensor memory: S^T [0, 128), dP^T [128, 256) (P^T and dS^T replace them, each half's 32 columns at the
 // half's start), dV at 256, dK at 256 + D.  Order of the tensor core: dV(i), S(i + 1) | dK(i), dP(i + 1): the first pair
-// runs while dS(i) is formed, the second while P(i + 1) is.
+// runs while dS(i) is formed, the second while P(i + 1) is.  A step of D = 128 takes some 2,500 cycles, 2,048 of them the
+// tensor core's four products.
 template <int D>
 struct KeyShared {
   SharedHead head;
@@ -1047,7 +1054,10 @@ __device__ __forceinline__ void key_tile(const BackwardParams& p, uint8_t* smem,
 // ------------------------------------------------------------------------------------------
 // Rows are queries, columns keys.  Q and dO are operands in tensor memory (columns 384 and 384 + D / 2), so that a stage of
 // 128 keys reads K twice and V once from shared memory.  S [0, 128), dP [128, 256) (dS replaces it), dQ at 256.  The
-// scores of the next stage are computed as soon as this one's have been read.
+// scores of the next stage are computed as soon as this one's have been read.  A step of D = 128 takes some 1,900 cycles, 1,536
+// of them the tensor core's three products.  Short walks are bound by L2 instead (2 x 16 heads of 7,800 queries on 512 keys: 1.1 GB
+// of tiles in 218 us); several tiles to a CTA, the next one's rows beside a ring of two, took 211 us there, but 346 instead of
+// 330 where walks are long.
 template <int D>
 struct QueryShared {
   static constexpr int kStages = 3;
@@ -1273,7 +1283,7 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
 // Query tiles that see at most kFewStages stages of keys therefore take delta_i = sum_j P_ij dP_ij in fp32.  A CTA keeps two key
 // tiles, one per warpgroup, and streams query tiles: S at columns 0 and 128, dP at 256 and 384.  Each query tile is read once
 // per two key tiles, as L2 is the bound (5.8 TB/s): for 2 x 16 heads of 7,800 queries on 512 keys one key tile per CTA took
-// 97 us, and a CTA per query tile, most of whose time was its start, 123.  few_sums_kernel adds the key tiles' parts up.
+// 97 us, and a CTA per query tile, most of whose time was its start, 123; this one 77.  few_sums_kernel adds the key tiles' parts up.
 template <int D>
 struct FewShared {
   static constexpr int kStages = D == 64 ? 2 : 1;  // of query tiles
