@@ -507,6 +507,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     const int seen = g.causal ? min(k_len, row + 1 + k_len - q_len) : k_len;  // keys that this row sees
     // (a warp masks a stage that one of its rows does not see whole)
     const int least = __reduce_min_sync(0xffffffffu, seen);
+    // fp16 has no exponents below 2^-14: P goes in times 2^7, which with the 2^8 below is the largest power that it holds
+    constexpr float kLift = kBf16 ? 0.0f : 7.0f;
     float m = -INFINITY, sum = 0.0f;
     const bool live = t < tiles && n > 0;
     if (live) {
@@ -558,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
           sum *= alpha;
           if (move) m = m_new;
         }
-        const float base = m == -INFINITY ? 0.0f : -m * c;
+        const float base = m == -INFINITY ? 0.0f : kLift - m * c;
         const float2 c2 = make_float2(c, c), base2 = make_float2(base, base);
         float2 sum2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         // (with keys hidden every probability is the unit's: the polynomial has no zero)
@@ -595,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const __grid_const
     }
     // all lanes read (the loads are the warp's), rows that exist are written
     const bool given = live && row < q_len && sum != 0.0f;  // (NaN is an answer, too)
-    const float factor = given ? 1.0f / sum : 0.0f, lse = given ? (m * c + log2f(sum)) * kLn2 : -INFINITY;
+    const float factor = given ? 1.0f / sum : 0.0f, lse = given ? (m * c + (log2f(sum) - kLift)) * kLn2 : -INFINITY;
     const int64_t flat = ((int64_t)b * g.q_heads + h) * g.q_tokens + row;
     const int64_t parted_pairs = p.tail.pairs - p.tail.whole;
     const int64_t part_row = (split * parted_pairs + pair - p.tail.whole) * 2 * kTile + row - q0;

@@ -12,8 +12,8 @@ and the exponentials (2^-22, of arguments below 2^6 that are good to 2^-17) stay
     dQ    scale s(e |k|) + u |dQ| + w scale s(|dS| |k|),  dK alike
 
 delta is dO . out of the rounded ``out`` that the call is given, so its exact distance from the formula's is used.  fp16
-operands below 2^-14 lose bits: P times 2^15 is off by 2^-25, P by 2^-40; dS, scaled so that 2 max|dO| max|v| lies above 2^13,
-by 2^-25 2^-13 2 max|dO| max|v|.
+operands below 2^-14 lose bits: P times 2^15 is off by 2^-25, P by 2^-40 (in the forward pass, times 2^7, by 2^-32); dS,
+scaled so that 2 max|dO| max|v| lies above 2^13, by 2^-25 2^-13 2 max|dO| max|v|.
 """
 
 import math
@@ -51,7 +51,6 @@ def _reference(q, k, v, do, out, scale, causal, q_lens, k_lens):
         dos[ql:] = 0
         top_do = dos.norm(dim=-1).max()
         top_v = clean[2].norm(dim=-1).max()
-        tiny_p = nk * 2.0 ** -40 if half else 0.0
         tiny_ds = 2.0 ** -37 * top_do * top_v if half else 0.0
         for h in range(hq):
             qs, ks, vs, g = clean[0][:, h], clean[1][:, h // group], clean[2][:, h // group], dos[:, h]
@@ -63,7 +62,8 @@ def _reference(q, k, v, do, out, scale, causal, q_lens, k_lens):
             o = p @ vs
             val["out"][s, :, h] = o
             mag = p @ vs.abs()
-            bnd["out"][s, :, h] = (u + w) * mag + u * o.abs() + tiny_p * vs.abs().amax(0)
+            # (the forward pass: P relative to a kept maximum, times 2^7, so that 2^8 more is held)
+            bnd["out"][s, :, h] = (u + w) * mag + u * o.abs() + (nk * 2.0 ** -32 if half else 0.0) * vs.abs().amax(0)
             if do is None:
                 continue
             given = out[s, :, h].double()
@@ -198,6 +198,27 @@ def test_one_key_has_no_gradient(native_library, dtype):
     assert torch.equal(out, v.expand_as(out)) and not dq.any() and not dk.any()
     wide = torch.finfo(dtype).eps * do.double().abs().sum(1, keepdim=True)
     assert ((dv.double() - do.double().sum(1, keepdim=True)).abs() <= wide).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nk", [120, 256, 900])
+def test_small_probabilities_survive_in_fp16(native_library, d, nk):
+    """One key whose value is zero has nearly all of the probability; what the others give, 2^-20.6 each, is the answer."""
+    from anemoi_b200.dense import dense_attention
+
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    q, k = torch.zeros(1, 200, 1, d, device="cuda"), torch.zeros(1, nk, 1, d, device="cuda")
+    v = torch.rand(1, nk, 1, d, generator=gen, device="cuda") + 1.0
+    q[..., 0], k[..., 0], k[:, 5, :, 0], v[:, 5] = 8.0, -10.28125, 4.0, 0.0
+    q, k, v = (t.half() for t in (q, k, v))
+    p = torch.softmax(0.125 * k[0, :, 0, 0].double() * 8.0, 0)
+    want = p @ v[0, :, 0].double()
+    u = torch.finfo(torch.float16).eps / 2
+    # as above, with P relative to the largest times 2^7: off by 2^-25 below 2^-14, so by 2^-32 each
+    bound = (2 * u + W) * want + nk * 2.0 ** -32 * v.max().double() + 2.0 ** -25
+    got = dense_attention(q, k, v, scale=0.125)[0, :, 0].double()
+    assert ((got - want).abs() <= bound).all()
 
 
 @pytest.mark.gpu
