@@ -1057,9 +1057,9 @@ __device__ __forceinline__ void key_tile(const BackwardParams& p, uint8_t* smem,
 // Rows are queries, columns keys.  Q and dO are operands in tensor memory (columns 384 and 384 + D / 2), so that a stage of
 // 128 keys reads K twice and V once from shared memory.  S [0, 128), dP [128, 256) (dS replaces it), dQ at 256.  The
 // scores of the next stage are computed as soon as this one's have been read.  A step of D = 128 takes some 1,900 cycles, 1,536
-// of them the tensor core's three products.  Short walks are bound by L2 instead (2 x 16 heads of 7,800 queries on 512 keys: 1.1 GB
-// of tiles in 218 us, some 80 of them at the start and end of CTAs); several tiles to a CTA, the next one's rows through the ring, took
-// 207 us there, but 343 instead of 330 where walks are long.
+// of them the tensor core's three products.  Short walks pay for their start and end: 2 x 16 heads of 7,800 queries take 78 us and
+// 0.305 us per key in all, 234 for 512 keys.  Several tiles to a CTA, the next one's rows through the ring, took 225 there, but
+// 720 instead of 701 for 2,048 keys.
 template <int D>
 struct QueryShared {
   static constexpr int kStages = 3;
