@@ -73,7 +73,7 @@ struct BackwardParams {
   Geometry g;                  // (splits: of the key tiles' queries)
   const float *lse, *delta;    // [B][H][q_tokens]
   float* few_parts;            // [few key tiles][B][H][q_tokens], where query tiles may see few keys (few_kernel)
-  const uint32_t* norms;       // fp16: largest |dO_i|^2 and |v_j|^2 per (sample, key head)
+  uint32_t* norms;             // fp16: largest |dO_i|^2 and |v_j|^2 per (sample, key head)
   void *dq, *dk, *dv;
   float *q_partial, *k_partial;  // with splits: [splits][B][H][q_tokens][D]; [splits][dV, dK][B][Hk][k_tokens][D]
   Strides sdq, sdk, sdv;
@@ -671,25 +671,39 @@ __global__ void __launch_bounds__(128) join_forward_kernel(const __grid_constant
 // ------------------------------------------------------------------------------------------
 // backward: what the kernels need of each row
 // ------------------------------------------------------------------------------------------
+// Query tiles that see at most kFewStages stages of keys have their delta from few_kernel.
+constexpr int kFewStages = 8;
+
+// Stages of keys that the query tile of a row sees.
+__device__ __forceinline__ int stages_of(const Geometry& g, int b, int row) {
+  const int q_len = length_of(g.q_lengths, b, g.q_tokens), k_len = length_of(g.k_lengths, b, g.k_tokens);
+  return (key_end(g, row / kTile * kTile + kTile, q_len, k_len) + kTile - 1) / kTile;
+}
+
 struct RowParams {
   const void *out, *dout, *v;
+  const float* few_parts;  // (or null)
   float* delta;
   uint32_t* norms;
   Strides so, sd, sv;
-  const int32_t *q_lengths, *k_lengths;
-  int batch, q_heads, k_heads, q_tokens, k_tokens, q_blocks;
+  Geometry g;
+  int q_blocks;
 };
 
-// delta_i.  fp16: the largest |dO_i|^2 and |v_j|^2 of each key head, too (a maximum does not depend on the order of atomics).
-// Rows in memory order (heads of a token, tokens, samples), kRowsEach at once per group of D/8 lanes: that many loads in flight.
+// delta_i = dO_i . o_i, or the sum of what few_kernel left (the sums and the cleared maxima in launches of their own: 32 us instead of
+// 29 for the whole gradient of 4 heads of 1,024 tokens).  fp16: the largest |dO_i|^2 and |v_j|^2 of each key head, too (a maximum
+// does not depend on the order of atomics).  Rows in memory order (heads of a token, tokens, samples), kRowsEach at once per group of D/8 lanes: that many loads in flight.
 constexpr int kRowsEach = 4;
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowParams p) {
   using T = std::conditional_t<kBf16, __nv_bfloat16, __half>;
   constexpr int kLanes = D / 8, kGroups = 256 / kLanes;
+  static_assert(kFewStages <= kLanes, "a part per lane");
+  layer::grid_dependency_wait();
+  const Geometry& g = p.g;
   const bool values = (int)blockIdx.x >= p.q_blocks;
-  const uint32_t heads = values ? p.k_heads : p.q_heads, tokens = values ? p.k_tokens : p.q_tokens;
-  const uint32_t all = p.batch * heads * tokens;  // (below 2^32: the host's limit)
+  const uint32_t heads = values ? g.k_heads : g.q_heads, tokens = values ? g.k_tokens : g.q_tokens;
+  const uint32_t all = g.batch * heads * tokens;  // (below 2^32: the host's limit)
   const uint32_t first = (uint32_t)(values ? blockIdx.x - p.q_blocks : blockIdx.x) * (kGroups * kRowsEach) + threadIdx.x / kLanes;
   const int lane = threadIdx.x % kLanes;
   const Strides& sd = values ? p.sv : p.sd;
@@ -698,6 +712,9 @@ __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowPar
   uint4 d_raw[kRowsEach], o_raw[kRowsEach];
   uint32_t h[kRowsEach], b[kRowsEach], i[kRowsEach];
   bool in[kRowsEach], live[kRowsEach];
+  bool few[kRowsEach];
+  float part[kRowsEach];
+  const int64_t parts_apart = (int64_t)g.batch * g.q_heads * g.q_tokens;
 #pragma unroll
   for (int n = 0; n < kRowsEach; ++n) {
     const uint32_t at = first + n * kGroups;
@@ -706,9 +723,17 @@ __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowPar
     h[n] = in[n] ? at - token_row * heads : 0u;
     b[n] = token_row / tokens;
     i[n] = token_row - b[n] * tokens;
-    live[n] = in[n] && (int)i[n] < length_of(values ? p.k_lengths : p.q_lengths, b[n], tokens);
+    live[n] = in[n] && (int)i[n] < length_of(values ? g.k_lengths : g.q_lengths, b[n], tokens);
+    few[n] = false;
+    part[n] = 0.0f;
+    if (p.few_parts != nullptr && !values && live[n]) {
+      const int stages = stages_of(g, b[n], (int)i[n]);
+      few[n] = stages <= kFewStages;
+      if (few[n] && lane < stages)
+        part[n] = p.few_parts[lane * parts_apart + ((int64_t)b[n] * g.q_heads + h[n]) * g.q_tokens + i[n]];
+    }
     d_raw[n] = o_raw[n] = make_uint4(0, 0, 0, 0);
-    if (live[n]) {
+    if (live[n] && !(kBf16 && few[n])) {
       d_raw[n] = rows::load_stream(d_all + b[n] * sd.batch + i[n] * sd.token + h[n] * sd.head);
       if (!values) o_raw[n] = rows::load_stream(o_all + b[n] * p.so.batch + i[n] * p.so.token + h[n] * p.so.head);
     }
@@ -724,6 +749,7 @@ __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowPar
       dot = fmaf(d[j], o[j], dot);
       norm = fmaf(d[j], d[j], norm);
     }
+    if (few[n]) dot = part[n];
 #pragma unroll
     for (int off = kLanes / 2; off > 0; off >>= 1) {
       dot += __shfl_xor_sync(0xffffffffu, dot, off);
@@ -731,10 +757,10 @@ __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowPar
     }
     if (!in[n] || lane != 0) continue;
     if (!values) {
-      p.delta[((int64_t)b[n] * p.q_heads + h[n]) * p.q_tokens + i[n]] = dot;
+      p.delta[((int64_t)b[n] * g.q_heads + h[n]) * g.q_tokens + i[n]] = dot;
     }
     if (!kBf16 && live[n])
-      atomicMax(p.norms + 2 * (b[n] * p.k_heads + (values ? h[n] : h[n] / (p.q_heads / p.k_heads))) + (values ? 1 : 0),
+      atomicMax(p.norms + 2 * (b[n] * g.k_heads + (values ? h[n] : h[n] / (g.q_heads / g.k_heads))) + (values ? 1 : 0),
                 __float_as_uint(norm));
   }
 }
@@ -764,8 +790,6 @@ __device__ __forceinline__ Scaling scaling(const BackwardParams& p, int b, int h
   return s;
 }
 
-// Query tiles that see at most kFewStages stages of keys have their delta from few_kernel.
-constexpr int kFewStages = 8;
 
 // A row's log-sum-exp in units of log 2: +inf where it has no gradient, so that its probabilities come out as zeros.
 __device__ __forceinline__ float lse2_of(const BackwardParams& p, int64_t flat, int row, int q_len) {
@@ -1285,7 +1309,7 @@ __device__ __forceinline__ void query_tile(const BackwardParams& p, uint8_t* sme
 // Query tiles that see at most kFewStages stages of keys therefore take delta_i = sum_j P_ij dP_ij in fp32.  A CTA keeps two key
 // tiles, one per warpgroup, and streams query tiles: S at columns 0 and 128, dP at 256 and 384.  Each query tile is read once
 // per two key tiles, as L2 is the bound (5.8 TB/s): for 2 x 16 heads of 7,800 queries on 512 keys one key tile per CTA took
-// 97 us, and a CTA per query tile, most of whose time was its start, 123; this one 77.  few_sums_kernel adds the key tiles' parts up.
+// 97 us, and a CTA per query tile, most of whose time was its start, 123; this one 77.  row_kernel adds the key tiles' parts up.
 template <int D>
 struct FewShared {
   static constexpr int kStages = D == 64 ? 2 : 1;  // of query tiles
@@ -1313,7 +1337,6 @@ __device__ __forceinline__ TileRange few_tiles(const Geometry& g, int tile, int 
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant__ BackwardParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  layer::grid_dependency_wait();
   constexpr int kBytes = kTileBytes<D>, kStages = FewShared<D>::kStages;
   auto* s = reinterpret_cast<FewShared<D>*>(smem + kFewTiles<D> * kBytes);
   const Geometry& g = p.g;
@@ -1326,6 +1349,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   const int first = range.first + (int)((int64_t)all * split / p.few_splits);
   const int n = range.first + (int)((int64_t)all * (split + 1) / p.few_splits) - first;
   const int tiles = (2 * blockIdx.x + 1) * kTile < k_len ? 2 : 1;
+  // (row_kernel's maxima start from here)
+  if (!kBf16 && blockIdx.x + blockIdx.y + blockIdx.z == 0)
+    for (int i = threadIdx.x; i < g.batch * g.k_heads * 2; i += kThreads) p.norms[i] = 0u;
   if (n == 0 || given_up(g)) return;
   if (threadIdx.x == 0) {
     begin_waits(&s->head, g);
@@ -1468,14 +1494,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   tmem_end(tmem);
 }
 
-// Adds a row's parts up, in order, into its delta.
+// Adds a row's parts up into its delta, where row_kernel has nothing else to do: bf16, few keys everywhere.
 __global__ void __launch_bounds__(256) few_sums_kernel(const float* parts, float* delta, const __grid_constant__ Geometry g) {
   layer::grid_dependency_wait();
   const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x * 256 + threadIdx.x;
-  const int q_len = length_of(g.q_lengths, b, g.q_tokens), k_len = length_of(g.k_lengths, b, g.k_tokens);
-  if (row >= q_len) return;
-  const int stages = (key_end(g, row / kTile * kTile + kTile, q_len, k_len) + kTile - 1) / kTile;
-  if (stages > kFewStages) return;
+  if (row >= length_of(g.q_lengths, b, g.q_tokens)) return;
+  const int stages = stages_of(g, b, row);
   const int64_t rows_all = (int64_t)g.batch * g.q_heads * g.q_tokens, flat = ((int64_t)b * g.q_heads + h) * g.q_tokens + row;
   float part[kFewStages];
 #pragma unroll
@@ -1692,22 +1716,24 @@ int backward_launch(const BackwardParams& p, const RowParams& r, cudaStream_t st
   if (q_blocks + v_blocks > 0x7fffffffLL) return ANEMOI_SM100_ELIMIT;
   RowParams rp = r;
   rp.q_blocks = (int)q_blocks;
-  if (!kBf16 && cudaMemsetAsync(rp.norms, 0, (size_t)g.batch * g.k_heads * 2 * sizeof(uint32_t), st) != cudaSuccess)
-    return ANEMOI_SM100_ELAUNCH;
-  // (bf16 with few keys everywhere needs nothing of it)
-  if (!kBf16 || p.few_parts == nullptr || g.k_tokens > kFewStages * kTile) {
-    row_kernel<D, kBf16><<<(unsigned)(q_blocks + v_blocks), 256, 0, st>>>(rp);
-    if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
-  }
+  rp.few_parts = p.few_parts;
   if (p.few_parts != nullptr) {
-    auto few = few_kernel<D, kBf16>;
     const size_t smem = kFewTiles<D> * (size_t)kTileBytes<D> + sizeof(FewShared<D>);
     if (!allow_shared<few_kernel<D, kBf16>>(smem)) return ANEMOI_SM100_ELAUNCH;
     const dim3 grid((std::min(p.key_tiles, kFewStages) + 1) / 2, g.q_heads, g.batch * p.few_splits);
-    if (layer::launch(few, grid, dim3(kThreads), smem, st, p) != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
-    if (layer::launch(few_sums_kernel, dim3((g.q_tokens + 255) / 256, g.q_heads, g.batch), dim3(256), 0, st,
-                      (const float*)p.few_parts, rp.delta, g) != cudaSuccess)
+    few_kernel<D, kBf16><<<grid, kThreads, smem, st>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+    const cudaError_t left =
+        kBf16 && g.k_tokens <= kFewStages * kTile
+            ? layer::launch(few_sums_kernel, dim3((g.q_tokens + 255) / 256, g.q_heads, g.batch), dim3(256), 0, st,
+                            (const float*)p.few_parts, rp.delta, g)
+            : layer::launch(row_kernel<D, kBf16>, dim3((unsigned)(q_blocks + v_blocks)), dim3(256), 0, st, rp);
+    if (left != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+  } else {
+    if (!kBf16 && cudaMemsetAsync(rp.norms, 0, (size_t)g.batch * g.k_heads * 2 * sizeof(uint32_t), st) != cudaSuccess)
       return ANEMOI_SM100_ELAUNCH;
+    row_kernel<D, kBf16><<<(unsigned)(q_blocks + v_blocks), 256, 0, st>>>(rp);
+    if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
   }
   auto kernel = backward_kernel<D, kBf16>;
   const size_t smem = 6 * (size_t)kTileBytes<D> + std::max(sizeof(KeyShared<D>), sizeof(QueryShared<D>));
@@ -1855,13 +1881,7 @@ extern "C" int anemoi_sm100_dense_attention_backward(const anemoi_sm100_dense_sh
   r.so = t[4].s;
   r.sd = t[0].s;
   r.sv = t[3].s;
-  r.q_lengths = q_lengths;
-  r.k_lengths = k_lengths;
-  r.batch = s->batch;
-  r.q_heads = s->q_heads;
-  r.k_heads = s->k_heads;
-  r.q_tokens = s->q_tokens;
-  r.k_tokens = s->k_tokens;
+  r.g = p.g;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d == 64) return bf16 ? backward_launch<64, true>(p, r, st) : backward_launch<64, false>(p, r, st);
   return bf16 ? backward_launch<128, true>(p, r, st) : backward_launch<128, false>(p, r, st);
