@@ -690,9 +690,10 @@ struct RowParams {
   int q_blocks;
 };
 
-// delta_i = dO_i . o_i, or the sum of what few_kernel left (the sums and the cleared maxima in launches of their own: 32 us instead of
-// 29 for the whole gradient of 4 heads of 1,024 tokens).  fp16: the largest |dO_i|^2 and |v_j|^2 of each key head, too (a maximum
-// does not depend on the order of atomics).  Rows in memory order (heads of a token, tokens, samples), kRowsEach at once per group of D/8 lanes: that many loads in flight.
+// delta_i = dO_i . o_i, or the sum of what few_kernel left (the sums and the cleared maxima in launches of their own: 35 us instead of
+// 31 for the whole gradient of 4 heads of 1,024 tokens).  fp16: the largest |dO_i|^2 and |v_j|^2 of each key head, too (a maximum
+// does not depend on the order of atomics).  Rows in memory order (heads of a token, tokens, samples), kRowsEach at once per group
+// of D/8 lanes: that many loads in flight.
 constexpr int kRowsEach = 4;
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) row_kernel(const __grid_constant__ RowParams p) {
@@ -1337,6 +1338,7 @@ __device__ __forceinline__ TileRange few_tiles(const Geometry& g, int tile, int 
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant__ BackwardParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
+  layer::grid_dependency_wait();
   constexpr int kBytes = kTileBytes<D>, kStages = FewShared<D>::kStages;
   auto* s = reinterpret_cast<FewShared<D>*>(smem + kFewTiles<D> * kBytes);
   const Geometry& g = p.g;
@@ -1721,8 +1723,7 @@ int backward_launch(const BackwardParams& p, const RowParams& r, cudaStream_t st
     const size_t smem = kFewTiles<D> * (size_t)kTileBytes<D> + sizeof(FewShared<D>);
     if (!allow_shared<few_kernel<D, kBf16>>(smem)) return ANEMOI_SM100_ELAUNCH;
     const dim3 grid((std::min(p.key_tiles, kFewStages) + 1) / 2, g.q_heads, g.batch * p.few_splits);
-    few_kernel<D, kBf16><<<grid, kThreads, smem, st>>>(p);
-    if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
+    if (layer::launch(few_kernel<D, kBf16>, grid, dim3(kThreads), smem, st, p) != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
     const cudaError_t left =
         kBf16 && g.k_tokens <= kFewStages * kTile
             ? layer::launch(few_sums_kernel, dim3((g.q_tokens + 255) / 256, g.q_heads, g.batch), dim3(256), 0, st,
