@@ -785,7 +785,7 @@ class _OnDevice:
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:
