@@ -22,7 +22,6 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "../../include/anemoi_sm100.h"
@@ -1580,19 +1579,6 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// The dynamic shared memory that a kernel may have, told to the driver once per device (a microsecond each time).
-template <auto kKernel>
-bool allow_shared(size_t bytes) {
-  static std::atomic<uint64_t> told{0};
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return false;
-  const uint64_t bit = device < 64 ? 1ull << device : 0;
-  if (told.load(std::memory_order_relaxed) & bit) return true;
-  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
-  told.fetch_or(bit, std::memory_order_relaxed);
-  return true;
-}
-
 struct Tensor {
   const void* at;
   int heads, tokens;
@@ -1697,7 +1683,7 @@ template <int D, bool kBf16>
 int forward_launch(ForwardParams& p, cudaStream_t st) {
   auto kernel = forward_kernel<D, kBf16>;
   const size_t smem = (size_t)kForwardTiles<D> * kTileBytes<D> + sizeof(ForwardShared<D>);
-  if (!allow_shared<forward_kernel<D, kBf16>>(smem)) return ANEMOI_SM100_ELAUNCH;
+  if (!rows::allow_shared<forward_kernel<D, kBf16>>(smem)) return ANEMOI_SM100_ELAUNCH;
   const int parted = p.tail.pairs - p.tail.whole;
   kernel<<<p.tail.whole + parted * p.tail.splits, kThreads, smem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
@@ -1721,7 +1707,7 @@ int backward_launch(const BackwardParams& p, const RowParams& r, cudaStream_t st
   rp.few_parts = p.few_parts;
   if (p.few_parts != nullptr) {
     const size_t smem = kFewTiles<D> * (size_t)kTileBytes<D> + sizeof(FewShared<D>);
-    if (!allow_shared<few_kernel<D, kBf16>>(smem)) return ANEMOI_SM100_ELAUNCH;
+    if (!rows::allow_shared<few_kernel<D, kBf16>>(smem)) return ANEMOI_SM100_ELAUNCH;
     const dim3 grid((std::min(p.key_tiles, kFewStages) + 1) / 2, g.q_heads, g.batch * p.few_splits);
     if (layer::launch(few_kernel<D, kBf16>, grid, dim3(kThreads), smem, st, p) != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
     const cudaError_t left =
@@ -1738,7 +1724,7 @@ int backward_launch(const BackwardParams& p, const RowParams& r, cudaStream_t st
   }
   auto kernel = backward_kernel<D, kBf16>;
   const size_t smem = 6 * (size_t)kTileBytes<D> + std::max(sizeof(KeyShared<D>), sizeof(QueryShared<D>));
-  if (!allow_shared<backward_kernel<D, kBf16>>(smem)) return ANEMOI_SM100_ELAUNCH;
+  if (!rows::allow_shared<backward_kernel<D, kBf16>>(smem)) return ANEMOI_SM100_ELAUNCH;
   const int64_t ctas = p.key_ctas + (int64_t)p.query_tiles * g.q_heads * g.batch * p.q_splits;
   if (layer::launch(kernel, dim3((unsigned)ctas), dim3(kThreads), smem, st, p) != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
   // what several CTAs summed: dV, dK, dQ

@@ -722,9 +722,10 @@ int backward_launch(const BackwardParams& p, const RowShape& s, const Split& spl
   const size_t smem = (size_t)kStages * 4 * kR * V * s.threads * 16 +
                       (p.weight_partial != nullptr ? (size_t)slots * 2 * V * s.lanes * 8 * sizeof(float) : 0);
   auto kernel = backward_kernel<T, M, V, kR, kWide, kStages>;
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return ANEMOI_SM100_ELAUNCH;
+  constexpr size_t kMost =
+      (size_t)backward_threads(V, kR, kWide) * V * (kStages * 4 * kR * 16 + 2 * 8 * sizeof(float));
+  static_assert(kMost + kBuffer * sizeof(float) <= 227 * 1024, "what a block may have");
+  if (smem > kMost || !allow_shared<backward_kernel<T, M, V, kR, kWide, kStages>>(kMost)) return ANEMOI_SM100_ELAUNCH;
   kernel<<<split.blocks, s.threads, smem, st>>>(p, s.lanes);
   return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
 }

@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "packed.cuh"
 
 namespace rows {
@@ -211,6 +213,20 @@ __device__ __forceinline__ float column_sum(const float* partial, int64_t stride
 #pragma unroll 8
     for (int i = 0; i < slices; ++i) total += part[i * across + x];
   return total;
+}
+
+// The most dynamic shared memory that any call of a kernel has, told to the driver once per device (a microsecond each time, and
+// a smaller call would take from a larger one of another thread what it is about to use).
+template <auto kKernel>
+bool allow_shared(size_t bytes) {
+  static std::atomic<uint64_t> told{0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (told.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+  told.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 }  // namespace rows

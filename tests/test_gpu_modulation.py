@@ -288,6 +288,37 @@ def test_an_eps_that_changes_in_place(native_library):
         assert torch.equal(fused_norm_modulate(x, eps=eps), fused_norm_modulate(x, eps=value))
 
 
+@pytest.mark.gpu
+def test_calls_of_two_threads(native_library):
+    """Widths that one kernel serves with different amounts of shared memory."""
+    import threading
+
+    from anemoi_b200.modulation import fused_gate_norm_modulate_backward
+
+    failed = []
+
+    def work(width):
+        try:
+            t, d_x, d_h = _inputs((1, 64), 1, width, torch.bfloat16, torch.bfloat16, True, "rms", seed=width)
+            back = [t[k] for k in ("x", "y", "gate", "scale", "weight", "post_weight")]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+                first = fused_gate_norm_modulate_backward(d_x, d_h, *back, post_norm="rms")
+                for _ in range(300):
+                    again = fused_gate_norm_modulate_backward(d_x, d_h, *back, post_norm="rms")
+                    if not all(a is None or torch.equal(a, b) for a, b in zip(first, again)):
+                        failed.append(width)
+        except Exception as error:
+            failed.append(error)
+
+    threads = [threading.Thread(target=work, args=(width,)) for width in (1160, 2048, 4104, 5376)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failed
+
+
 def _cpu(*shape, dtype=torch.bfloat16):
     return torch.zeros(*shape, dtype=dtype)
 
