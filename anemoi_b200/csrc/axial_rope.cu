@@ -21,6 +21,7 @@
 #include <algorithm>
 
 #include "../../include/anemoi_sm100.h"
+#include "layer.cuh"
 #include "rows.cuh"
 
 namespace {
@@ -390,11 +391,12 @@ constexpr int kSumThreads = 1024;  // (few columns, many parts)
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads) sums_kernel(const float* partial, int q_parts, int k_parts, int d,
                                                            void* dq_weight, void* dk_weight) {
+  layer::grid_dependency_wait();
   void* out = blockIdx.y ? dk_weight : dq_weight;
   const int parts = blockIdx.y ? k_parts : q_parts, across = sum_columns(parts), first = blockIdx.x * across;
   if (out == nullptr || first >= d) return;
   const float v = column_sum<kSumThreads>(partial + (blockIdx.y ? (int64_t)q_parts * d : 0), d, parts, first, d);
-  if (threadIdx.x < across) store1(static_cast<T*>(out) + first + threadIdx.x, v);
+  if (threadIdx.x < across && first + (int)threadIdx.x < d) store1(static_cast<T*>(out) + first + threadIdx.x, v);
 }
 
 // Heads per group of lanes: eight (that many loads in flight, one read of weights and angles for them) where heads fill them
@@ -479,9 +481,8 @@ int backward_launch(RopeParams& p, const BackwardPlan& plan, void* dq_weight, vo
   kernel<<<dim3(plan.q_blocks + plan.k_blocks, p.batch), kThreads, 0, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return ANEMOI_SM100_ELAUNCH;
   if (p.weight_partial == nullptr) return ANEMOI_SM100_OK;
-  sums_kernel<T><<<dim3(D / 8, 2), kSumThreads, 0, st>>>(p.weight_partial, plan.q_blocks * (int)p.batch,
-                                                         plan.k_blocks * (int)p.batch, D, dq_weight, dk_weight);
-  return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
+  return layer::launch(sums_kernel<T>, dim3(D / 8, 2), dim3(kSumThreads), 0, st, p.weight_partial, plan.q_blocks * (int)p.batch,
+                       plan.k_blocks * (int)p.batch, D, dq_weight, dk_weight) == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }

@@ -24,6 +24,7 @@
 #include <algorithm>
 
 #include "../../include/anemoi_sm100.h"
+#include "layer.cuh"
 #include "rows.cuh"
 
 namespace {
@@ -617,6 +618,7 @@ struct SumsParams {
 // First the groups' A, S, B sums (where groups have several segments), then the two weights' sums.
 template <typename T, typename M>
 __global__ void __launch_bounds__(kSumThreads) sums_kernel(const __grid_constant__ SumsParams p) {
+  layer::grid_dependency_wait();
   const int group_across = sum_columns(p.per_group_segments), weight_across = sum_columns(p.workers);
   const uint32_t each = ((uint32_t)p.width + group_across - 1) / group_across;
   const uint32_t group_blocks = p.per_group_segments > 1 ? (uint32_t)p.groups * 3 * each : 0;
@@ -760,8 +762,7 @@ int backward_typed(const BackwardParams& p, const SumsParams& q, const RowShape&
   const int64_t grid = (split.per_group_segments > 1 ? 3 * q.groups * each : 0) + (q.weight_partial != nullptr ? 2 * narrow : 0);
   if (grid == 0) return ANEMOI_SM100_OK;
   if (grid > 0x7fffffffLL) return ANEMOI_SM100_ELIMIT;
-  sums_kernel<T, M><<<(unsigned)grid, kSumThreads, 0, st>>>(q);
-  return cudaGetLastError() == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
+  return layer::launch(sums_kernel<T, M>, dim3((unsigned)grid), dim3(kSumThreads), 0, st, q) == cudaSuccess ? ANEMOI_SM100_OK : ANEMOI_SM100_ELAUNCH;
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }

@@ -191,10 +191,10 @@ __device__ __forceinline__ float load1<__nv_bfloat16>(const __nv_bfloat16* p) {
 }
 
 // Sum of a column of `parts` fp32 partial sums, `stride` values apart, by a block of kThreads threads: `across` neighbouring
-// columns (32, or 8 where parts are many: a 32-byte sector), kThreads / across slices of the parts, added in order.  The
-// order depends on `parts` alone, so that equal calls give equal bits.  Threads below `across` return the sum of column
-// `first + threadIdx.x`, others nothing of use.
-__host__ __device__ constexpr int sum_columns(int parts) { return parts > 256 ? 8 : 32; }
+// columns (32; 128 where parts are few, or 8, a 32-byte sector, where they are many), kThreads / across slices of the parts,
+// added in order.  The order depends on `parts` alone, so that equal calls give equal bits.  Threads below `across` return the
+// sum of column `first + threadIdx.x` (zero where there is none), others nothing of use.
+__host__ __device__ constexpr int sum_columns(int parts) { return parts > 256 ? 8 : parts > 32 ? 32 : 128; }
 template <int kThreads>
 __device__ __forceinline__ float column_sum(const float* partial, int64_t stride, int parts, int first, int columns) {
   __shared__ float part[kThreads];
